@@ -46,6 +46,13 @@ extern "C" {
 #define PACKR_DTYPE_BF16 1
 #define PACKR_DTYPE_F16 2 /* weights of packr_from_linear_encode only */
 
+/* ---- activations of packr_linear_act_* ---------------------------------- */
+#define PACKR_ACT_NONE 0
+#define PACKR_ACT_RELU 1
+#define PACKR_ACT_GELU 2      /* z * Phi(z), by the error function */
+#define PACKR_ACT_GELU_TANH 3 /* its tanh form */
+#define PACKR_ACT_SILU 4
+
 const char* packr_error_string(int code);
 int packr_abi_version(void);
 
@@ -206,6 +213,62 @@ int packr_backward_decoded(const float* dY, const void* x, int x_dtype, const ui
 /* 1 when packr_forward takes its predecode route for this problem (given a
  * workspace of packr_forward_workspace_bytes), else 0. */
 int packr_predecode_route(int64_t M, int64_t K, int64_t N, const uint8_t* W_p, const uint16_t* W_f);
+
+/* ---- PackRLinear with bias, activation and residual in its epilogue -------
+ *   z = x @ W + bias;  out = act(z) + residual;  W = bf16(W_f + bf16(lut[W_p]))
+ * at every M (x rounded to bf16 when it is f32), f32 accumulation, one
+ * rounding to out's type.  residual, out and z are contiguous [M, N] of
+ * out_dtype (f32 or bf16); residual and z may be NULL; outputs overlap no
+ * input.
+ * A caller that will run the backward of an activation passes z, which gets
+ * the pre-activation.  activation: PACKR_ACT_*.  M = 0 is a no-op.  x, when it
+ * is bf16 and K % 8 == 0, is read by TMA and must be 16-byte aligned from 5
+ * rows on.  The workspace query takes W_p and W_f because the route depends
+ * on their alignment; 256-byte aligned workspace, PACKR_ERR_WORKSPACE below
+ * the query's size.  The reference runs packr_matmul, then torch kernels for
+ * the bias, activation and residual (packr/layer.py:96-97 and the host
+ * model's own). */
+size_t packr_linear_act_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, const uint8_t* W_p,
+                                        const uint16_t* W_f);
+int packr_linear_act_forward(const void* x, int x_dtype, const uint8_t* W_p, const uint16_t* W_f, const float* lut,
+                             const void* bias, int bias_dtype, int activation, const void* residual, void* out,
+                             void* z, int out_dtype, int64_t M, int64_t K, int64_t N, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/* Its backward: dz = dout * act'(z) (f32, then the bf16 operand of the GEMMs);
+ *   dX[M,K]   = bf16(dz @ W^T)  stored as x's dtype      (NULL: skipped)
+ *   dW_f[K,N] = bf16(x^T @ dz)  fp32 accumulate          (NULL: skipped)
+ *   dlut[256] = sum_{W_p==b} (x^T @ dz) / (count[b] + 1e-8)  (NULL: skipped)
+ *   dbias[N]  = sum_m dz, as dbias_dtype, rows added in a fixed order (NULL: skipped)
+ * The residual's gradient is dout itself.  dout and z are contiguous [M, N] of
+ * out_dtype; z is the forward's (NULL for PACKR_ACT_NONE).  lut_counts and
+ * flags as for packr_backward; with PACKR_BWD_DW_SPLIT dz enters dW as bf16
+ * hi + lo parts. */
+size_t packr_linear_act_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, int flags,
+                                                 const uint8_t* W_p, const uint16_t* W_f);
+int packr_linear_act_backward(const void* dout, const void* z, int out_dtype, int activation, const void* x,
+                              int x_dtype, const uint8_t* W_p, const uint16_t* W_f, const float* lut,
+                              const int32_t* lut_counts, void* dX, uint16_t* dW_f, float* dlut, void* dbias,
+                              int dbias_dtype, int64_t M, int64_t K, int64_t N, int flags, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* ---- layer norm over the last dimension, with a residual sum ---------------
+ *   s = x + residual (f32);  y = (s - mean) * rstd * weight + bias,
+ *   rstd = 1 / sqrt(mean((s - mean)^2) + eps)
+ * x, residual and y: contiguous [M, N] of x_dtype; weight and bias [N] of
+ * w_dtype (either dtype f32 or bf16).  residual, weight and bias may be NULL;
+ * mean and rstd (f32 [M], for the backward) too.  Outputs overlap no input.  M = 0 is a
+ * no-op. */
+int packr_layer_norm_forward(const void* x, const void* residual, int x_dtype, const void* weight, const void* bias,
+                             int w_dtype, float eps, void* y, float* mean, float* rstd, int64_t M, int64_t N,
+                             void* stream);
+/* dx [M, N] of x_dtype (also the residual's gradient), dweight and dbias [N] of
+ * w_dtype; each may be NULL.  mean and rstd are the forward's.  The workspace
+ * (16-byte aligned) is needed for dweight / dbias only: per-CTA column sums,
+ * added in a fixed order. */
+size_t packr_layer_norm_backward_workspace_bytes(int64_t M, int64_t N);
+int packr_layer_norm_backward(const void* dy, const void* x, const void* residual, int x_dtype, const void* weight,
+                              int w_dtype, const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                              int64_t M, int64_t N, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- PackRLinear.from_linear (reference packr/layer.py:106-159) ----------
  * Step 1: the rank_lo-th and rank_hi-th smallest |w| (0-based; rank_hi is

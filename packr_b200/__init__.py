@@ -11,7 +11,8 @@ Every op runs hand-written sm_100a kernels from libpackr_b200.so through its
 C ABI (include/packr_b200.h); there is no CPU fallback.
 """
 from .kernel import packr_matmul
-from .autograd import PackRMatmulFunction, PackRLinearFunction
+from .autograd import PackRMatmulFunction, PackRLinearFunction, PackRLinearActFunction, packr_linear_act
+from .norm import PackRLayerNorm, PackRLayerNormFunction, packr_layer_norm
 from .layer import PackRLinear
 from .layer_patcher import compress_model
 from .config import PackRConfig, SchemeType
@@ -29,6 +30,7 @@ CV2LRTController = VelvetController
 
 __all__ = [
     "PackRConfig", "PackRLinear", "PackRMatmulFunction", "PackRLinearFunction", "packr_matmul", "compress_model",
+    "PackRLinearActFunction", "packr_linear_act", "PackRLayerNorm", "PackRLayerNormFunction", "packr_layer_norm",
     "SchemeType", "FusedQuantizedAdam", "CUDA8BitAdam", "VelvetController", "OffloadManager",
     "PHRConfig", "PHRLinear", "PHRMatmulFunction", "phr_matmul", "CV2LRTController",
 ]

@@ -71,6 +71,16 @@ SIGNATURES = {
     "packr_backward_decoded": (_I32, [_VP, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64,
                                       _I64, _I32, _VP, _SZ, _VP]),
     "packr_predecode_route": (_I32, [_I64, _I64, _I64, _VP, _VP]),
+    "packr_linear_act_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32, _VP, _VP]),
+    "packr_linear_act_forward": (_I32, [_VP, _I32, _VP, _VP, _VP, _VP, _I32, _I32, _VP, _VP, _VP, _I32, _I64, _I64,
+                                        _I64, _VP, _SZ, _VP]),
+    "packr_linear_act_backward_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32, _I32, _VP, _VP]),
+    "packr_linear_act_backward": (_I32, [_VP, _VP, _I32, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I32,
+                                         _I64, _I64, _I64, _I32, _VP, _SZ, _VP]),
+    "packr_layer_norm_forward": (_I32, [_VP, _VP, _I32, _VP, _VP, _I32, _F32, _VP, _VP, _VP, _I64, _I64, _VP]),
+    "packr_layer_norm_backward_workspace_bytes": (_SZ, [_I64, _I64]),
+    "packr_layer_norm_backward": (_I32, [_VP, _VP, _VP, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _VP, _SZ,
+                                         _VP]),
     "packr_abs_order_stats_workspace_bytes": (_SZ, []),
     "packr_abs_order_stats": (_I32, [_VP, _I32, _I64, _I64, _I64, _VP, _VP, _SZ, _VP]),
     "packr_from_linear_encode": (_I32, [_VP, _I32, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
@@ -79,6 +89,7 @@ SIGNATURES = {
                                              _I64, _I32, _VP]),
 }
 PACKR_BWD_DW_SPLIT = 1
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 PACKR_IPC_HANDLE_BYTES = 64
 
 

@@ -20,7 +20,9 @@ from __future__ import annotations
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
+from . import _lib
 from . import kernel as _k
 
 # Off by default: between forward and backward a layer holds only its packed
@@ -113,6 +115,100 @@ class PackRMatmulFunction(torch.autograd.Function):
         if dX is not None and dX.dtype != x.dtype:
             dX = dX.to(x.dtype)
         return dX, None, dW, dlut, None, None, None
+
+
+class PackRLinearActFunction(torch.autograd.Function):
+    """out = act(x @ W + bias) + residual on contiguous 2-D operands; keeps x
+    and, for an activation, z = x @ W + bias in out's dtype."""
+
+    @staticmethod
+    def forward(ctx, x, W_p, W_f, lut, bias, residual, activation, out_dtype, counts):
+        out, z = _k.linear_act_forward(x, W_p, W_f, lut, bias, activation, residual, out_dtype,
+                                       keep_z=activation != _lib.ACTIVATIONS["none"])
+        ctx.save_for_backward(x, W_p, W_f, lut, z, counts)
+        ctx.activation, ctx.out_dtype = activation, out_dtype
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.wf_param = W_f
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        x, W_p, W_f, lut, z, counts = ctx.saved_tensors
+        nx, _, nwf, nlut, nb, nr = ctx.needs_input_grad[:6]
+        g = grad_out if grad_out.dtype == ctx.out_dtype else grad_out.to(ctx.out_dtype)
+        g = g.contiguous()
+        if g.data_ptr() % 16:
+            g = g.clone()
+        dX, dW, dlut, dbias = _k.linear_act_backward(g, z, ctx.activation, x, W_p, W_f, lut, counts, nx, nwf, nlut,
+                                                     ctx.bias_dtype if nb else None,
+                                                     dW_out=grad_sink(ctx.wf_param) if nwf else None)
+        return dX, None, dW, dlut, dbias, grad_out if nr else None, None, None, None
+
+
+def _aligned16(t):
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def packr_linear_act(x, W_p, W_f, lut, bias=None, activation=None, residual=None, out_dtype=torch.float32, counts=None):
+    """act(x @ (W_f + lut[W_p]) + bias) + residual, in one pass over the output,
+    differentiable in x, W_f, lut, bias and residual.
+
+    Args:
+        x:          [..., K] f32 or bf16 (CUDA); f32 is rounded to bf16, the tensor cores' operand
+        W_p:        [K, N] uint8 byte indices (contiguous)
+        W_f:        [K, N] bf16 residual weights
+        lut:        [256] f32 lookup table
+        bias:       [N] bf16 or f32, or None
+        activation: None or "none", "relu", "gelu" (error function), "gelu_tanh", "silu"
+        residual:   [..., N] of out_dtype, or None
+        out_dtype:  torch.float32 (the packed layers' output type) or torch.bfloat16; the
+                    pre-activation kept for the backward has it too
+        counts:     int32 [256] bincount of W_p (PackRLinear.lut_counts), used by the lut
+                    gradient; counted there when None
+
+    W = bf16(W_f + bf16(lut[W_p])) at every row count.  With bf16 x the
+    gradient of the pre-activation enters the weight and lut gradients rounded
+    to bf16, as in PackRLinear; with f32 x as bf16 hi + lo parts
+    (PACKR_DW_PRECISION)."""
+    if not (x.is_cuda and W_p.is_cuda and W_f.is_cuda and lut.is_cuda):
+        raise RuntimeError("packr_linear_act runs on CUDA tensors only (no CPU path in the B200 build)")
+    act = _lib.ACTIVATIONS.get("none" if activation is None else activation)
+    if act is None:
+        raise ValueError(f"packr_linear_act: activation must be one of {sorted(_lib.ACTIVATIONS)}, not {activation!r}")
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"packr_linear_act: unsupported dtype {x.dtype}")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"packr_linear_act: out_dtype must be float32 or bfloat16, not {out_dtype}")
+    if W_p.dtype != torch.uint8 or W_f.dtype != torch.bfloat16 or lut.dtype != torch.float32:
+        raise TypeError("packr_linear_act: W_p must be uint8, W_f bfloat16 and lut float32")
+    if W_p.dim() != 2 or W_p.shape != W_f.shape or tuple(lut.shape) != (256,) or min(W_p.shape) < 1:
+        raise ValueError("packr_linear_act: W_p and W_f must be [K, N] (K, N >= 1) and lut [256]")
+    K, N = W_p.shape
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"packr_linear_act: x's last dimension must be {K}, got {tuple(x.shape)}")
+    lead = x.shape[:-1]
+    if not W_p.is_contiguous():
+        raise ValueError("packr_linear_act: W_p must be contiguous")
+    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype not in (torch.bfloat16, torch.float32)):
+        raise ValueError(f"packr_linear_act: bias must be bf16 or f32 [{N}]")
+    if residual is not None and (residual.shape != lead + (N,) or residual.dtype != out_dtype):
+        raise ValueError(f"packr_linear_act: residual must be {tuple(lead) + (N,)} of {out_dtype}")
+    if counts is not None and (counts.dtype != torch.int32 or tuple(counts.shape) != (256,)
+                               or not counts.is_contiguous()):
+        raise ValueError("packr_linear_act: counts must be contiguous int32 [256]")
+    for t in (W_p, W_f, lut, bias, residual, counts):
+        if t is not None and t.device != x.device:
+            raise ValueError("packr_linear_act: every tensor must be on x's device")
+    x2 = _aligned16(x.reshape(-1, K).contiguous())
+    r2 = None if residual is None else residual.reshape(-1, N).contiguous()
+    W_f, lut = W_f.contiguous(), lut.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, W_f, lut, bias, r2)):
+        out = PackRLinearActFunction.apply(x2, W_p, W_f, lut, bias, r2, act, out_dtype, counts)
+    else:
+        out = _k.linear_act_forward(x2, W_p, W_f, lut, bias, act, r2, out_dtype)[0]
+    return out if x.dim() == 2 else out.reshape(lead + (N,))
 
 
 # Legacy alias (reference packr/__init__.py:32)

@@ -41,6 +41,7 @@
 
 #include <mutex>
 
+#include "activation.cuh"
 #include "sm100.cuh"
 
 namespace packr {
@@ -227,6 +228,7 @@ struct Params {
   // collective) take fewer tiles instead of ending the launch late
   int dyn;
   int* tile_counter;
+  Epilogue epi;              // FWD with the fused epilogue (EPI): replaces `out`
 };
 
 // Workspace for stream-K: partial slots and flags for up to `pairs` CTA pairs.
@@ -539,6 +541,141 @@ __device__ __forceinline__ void store_rows_staged(uint32_t stg, const float* v, 
   __syncwarp();
 }
 
+// As store_rows_staged, for rows or bases without 16-byte alignment and for
+// the last columns: the 32 x 32 block is staged in the warp's buffer and each
+// store instruction writes one row's nval consecutive elements.
+template <int ESIZE>
+__device__ __forceinline__ void store_rows_any(uint32_t stg, const float* v, void* out, int r0, int m_limit,
+                                               long long ld, int gn0, int nval) {
+  constexpr int CPR = 32 * ESIZE / 16;
+  const int lane = threadIdx.x & 31;
+  // 4-byte words of row r, word w at ((w + r) & (words - 1)): conflict-free both ways
+  constexpr int WPR = 32 * ESIZE / 4;
+#pragma unroll
+  for (int j = 0; j < 4 * CPR; ++j)
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(stg + (uint32_t)(lane * 32 * ESIZE + ((j + lane) & (WPR - 1)) * 4)),
+                 "r"(__float_as_uint(v[j]))
+                 : "memory");
+  __syncwarp();
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r) {
+    const int w = ESIZE == 4 ? lane : lane >> 1;
+    uint32_t d;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(d) : "r"(stg + (uint32_t)(r * 32 * ESIZE + ((w + r) & (WPR - 1)) * 4)) : "memory");
+    const long long gr = (long long)r0 + r;
+    if (gr < m_limit && lane < nval) {
+      if (ESIZE == 4)
+        __stcs(static_cast<uint32_t*>(out) + gr * ld + gn0 + lane, d);
+      else
+        __stcs(static_cast<unsigned short*>(out) + gr * ld + gn0 + lane, (unsigned short)(d >> (16 * (lane & 1))));
+    }
+  }
+  __syncwarp();
+}
+
+// The fused epilogue of one warp's 32 x 32 block: f holds the f32 accumulator
+// of row r0 + lane, columns gn0 .. gn0 + 31 (nval of them inside the output).
+__device__ __forceinline__ void epilogue_block(const Params& P, uint32_t stg, float* f, int r0, int gn0, int nval) {
+  const Epilogue& E = P.epi;
+  const int lane = threadIdx.x & 31;
+  const long long row = (long long)r0 + lane;
+  const bool row_ok = row < P.Mg;
+  const bool full = nval == 32 && E.vec;
+  if (P.bias != nullptr) {
+    if (nval == 32 && aligned(P.bias, 16)) {  // the same 32 values in every lane
+      if (P.bias_f32) {
+        const float4* bp = reinterpret_cast<const float4*>(static_cast<const float*>(P.bias) + gn0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 b = __ldg(bp + j);
+          f[4 * j] = __fadd_rn(f[4 * j], b.x);
+          f[4 * j + 1] = __fadd_rn(f[4 * j + 1], b.y);
+          f[4 * j + 2] = __fadd_rn(f[4 * j + 2], b.z);
+          f[4 * j + 3] = __fadd_rn(f[4 * j + 3], b.w);
+        }
+      } else {
+        const uint4* bp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.bias) + gn0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 b = __ldg(bp + j);
+          const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f[8 * j + 2 * i] = __fadd_rn(f[8 * j + 2 * i], __uint_as_float(w[i] << 16));
+            f[8 * j + 2 * i + 1] = __fadd_rn(f[8 * j + 2 * i + 1], __uint_as_float(w[i] & 0xFFFF0000u));
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j < nval) f[j] = __fadd_rn(f[j], load_io(P.bias, gn0 + j, P.bias_f32));
+    }
+  }
+  auto put = [&](void* dst) {
+    if (E.io_f32) {
+      if (full) store_rows_staged<4>(stg, f, dst, r0, P.Mg, P.ld_out, gn0);
+      else store_rows_any<4>(stg, f, dst, r0, P.Mg, P.ld_out, gn0, nval);
+    } else {
+      float h[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) h[j] = __uint_as_float(pack_bf16x2_rne(f[2 * j], f[2 * j + 1]));
+      if (full) store_rows_staged<2>(stg, h, dst, r0, P.Mg, P.ld_out, gn0);
+      else store_rows_any<2>(stg, h, dst, r0, P.Mg, P.ld_out, gn0, nval);
+    }
+  };
+  if (E.z != nullptr) put(E.z);
+  act::apply_all<32>(E.act, f);
+  if (E.residual != nullptr) {
+    if (full) {
+      if (row_ok) {
+        if (E.io_f32) {
+          const float4* rp = reinterpret_cast<const float4*>(static_cast<const float*>(E.residual) + row * P.ld_out + gn0);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 r = __ldcs(rp + j);
+            f[4 * j] = __fadd_rn(f[4 * j], r.x);
+            f[4 * j + 1] = __fadd_rn(f[4 * j + 1], r.y);
+            f[4 * j + 2] = __fadd_rn(f[4 * j + 2], r.z);
+            f[4 * j + 3] = __fadd_rn(f[4 * j + 3], r.w);
+          }
+        } else {
+          const uint4* rp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(E.residual) + row * P.ld_out + gn0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 r = __ldcs(rp + j);
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              f[8 * j + 2 * i] = __fadd_rn(f[8 * j + 2 * i], __uint_as_float(w[i] << 16));
+              f[8 * j + 2 * i + 1] = __fadd_rn(f[8 * j + 2 * i + 1], __uint_as_float(w[i] & 0xFFFF0000u));
+            }
+          }
+        }
+      }
+    } else {
+      // row by row into the staging buffer as f32 (skewed words), then each lane its own row
+#pragma unroll 8
+      for (int r = 0; r < 32; ++r) {
+        const long long gr = (long long)r0 + r;
+        const float v = gr < P.Mg && lane < nval ? load_io(E.residual, gr * P.ld_out + gn0 + lane, E.io_f32) : 0.0f;
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(stg + (uint32_t)(r * 128 + ((lane + r) & 31) * 4)),
+                     "r"(__float_as_uint(v))
+                     : "memory");
+      }
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        uint32_t d;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(d) : "r"(stg + (uint32_t)(lane * 128 + ((j + lane) & 31) * 4)) : "memory");
+        f[j] = __fadd_rn(f[j], __uint_as_float(d));
+      }
+      __syncwarp();
+    }
+  }
+  put(E.out);
+}
+
 // Bounded wait for a stream-K flag written by another CTA pair of the same
 // launch (all pairs are resident at once).  Lane 0 polls with acquire loads
 // and decides; the result is the same in every lane, and the warp barrier
@@ -572,10 +709,13 @@ __device__ __forceinline__ bool wait_flag(const int* f, volatile int* abort_flag
 }
 
 // ------------------------------------------------------------------ kernel
-template <int MODE, int BSRC, int MSUB>
+// EPI: the forward with bias, activation and residual in its epilogue
+// (Params::epi).
+template <int MODE, int BSRC, int MSUB, bool EPI = false>
 __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB>::kThreads, 1)
     packr_gemm_kernel(const Params P, const __grid_constant__ Maps maps) {
   using C = Cfg<MODE, BSRC, MSUB>;
+  static_assert(!EPI || (MODE == FWD && C::kPlainB), "the fused epilogue belongs to the plain forward");
   constexpr int STAGES = C::kStages;
   static_assert(C::kSmemBytes <= 227 * 1024, "shared memory per CTA");
   static_assert(MODE != DW || MSUB == 1, "the DW epilogue's histogram runs per 256-row tile");
@@ -923,6 +1063,45 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB>::kThreads, 1)
           ++n_heads;
         }
         if (!alive) break;
+      }
+      if constexpr (EPI) {
+        // The whole subtile is taken into registers (4 x 32 columns per
+        // warp) and its accumulator handed back before any of the
+        // epilogue's arithmetic: with MSUB = 2 both accumulators are in use,
+        // and the next tile's first MMAs would otherwise wait for the
+        // activation, the residual loads and the stores.
+        uint32_t v[C::kChunksPerEpiWarp][32];
+#pragma unroll
+        for (int c = 0; c < C::kChunksPerEpiWarp; ++c)
+          tmem_ld_32x32b_x32(tmem_base + (uint32_t)(acc * ACC_COLS + (cc0 + c) * 32) + ((uint32_t)(q * 32) << 16), v[c]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(acc ? tempty1 : tempty0);
+#pragma unroll
+        for (int c = 0; c < C::kChunksPerEpiWarp; ++c) {
+          const int cc = cc0 + c;
+          const int gn0 = n0 + cc * 32;
+          if (gn0 >= P.Ng || m0 + q * 32 >= P.Mg) continue;  // warp-uniform
+          if (u.kind == 1) {  // stream-K head: raw partial
+#pragma unroll
+            for (int j = 0; j < 32; ++j) __stcg(my_slot + (cc * 32 + j) * BM + row, __uint_as_float(v[c][j]));
+            continue;
+          }
+          float f[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[c][j]);
+          if (u.kind == 2) {  // the heads' partials, added in pair order
+            for (int h = 1; h <= n_heads; ++h) {
+              const float* const slot =
+                  P.sk_partial + (((size_t)(pair + h) * MSUB + sub) * 2 + rank) * (size_t)(BN * BM);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[j] = __fadd_rn(f[j], __ldcg(slot + (cc * 32 + j) * BM + row));
+            }
+          }
+          epilogue_block(P, stg, f, m0 + q * 32, gn0, min(32, P.Ng - gn0));
+        }
+        continue;
       }
 #pragma unroll
       for (int c = 0; c < C::kChunksPerEpiWarp; ++c) {
@@ -1277,7 +1456,7 @@ int make_map_u8(CUtensorMap* m, const void* base, long long inner, long long row
   return r == CUDA_SUCCESS ? PACKR_OK : PACKR_ERR_INVALID_ARGUMENT;
 }
 
-template <int MODE, int BSRC, int MSUB = 1>
+template <int MODE, int BSRC, int MSUB = 1, bool EPI = false>
 int launch_impl(Params P, const Maps& maps, cudaStream_t stream) {
   using C = Cfg<MODE, BSRC, MSUB>;
   static std::once_flag attr_once[64];
@@ -1297,14 +1476,14 @@ int launch_impl(Params P, const Maps& maps, cudaStream_t stream) {
   cfg.numAttrs = 1;
   int attr_rc = 0;
   std::call_once(attr_once[dev & 63], [&] {
-    attr_rc = cudaFuncSetAttribute(packr_gemm_kernel<MODE, BSRC, MSUB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    attr_rc = cudaFuncSetAttribute(packr_gemm_kernel<MODE, BSRC, MSUB, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    C::kSmemBytes) != cudaSuccess;
     // CTA pairs that can be resident at once (a cluster needs two free SMs
     // of one GPC): the persistent grid is never larger
     cudaLaunchConfig_t q = cfg;
     q.gridDim = dim3(2 * (sm_count() / 2), 1, 1);
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, packr_gemm_kernel<MODE, BSRC, MSUB>, &q) != cudaSuccess || n < 1) {
+    if (cudaOccupancyMaxActiveClusters(&n, packr_gemm_kernel<MODE, BSRC, MSUB, EPI>, &q) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = sm_count() / 2;
     }
@@ -1359,7 +1538,7 @@ int launch_impl(Params P, const Maps& maps, cudaStream_t stream) {
     P.tile_counter = P.sk_flags;
     if (cudaMemsetAsync(P.tile_counter, 0, sizeof(int), stream) != cudaSuccess) return PACKR_ERR_CUDA;
   }
-  if (cudaLaunchKernelEx(&cfg, packr_gemm_kernel<MODE, BSRC, MSUB>, P, maps) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, packr_gemm_kernel<MODE, BSRC, MSUB, EPI>, P, maps) != cudaSuccess) {
     cudaGetLastError();
     return PACKR_ERR_LAUNCH;
   }
@@ -1400,15 +1579,15 @@ int launch(Params P, Maps maps, cudaStream_t stream) {
 
 // FWD / DX over a predecoded bf16 W (maps.b[0] set by the caller: FWD an
 // [K, N] map with 64-row boxes, DX an [K, N] map with 128-row boxes).
-template <int MODE>
+template <int MODE, bool EPI = false>
 int launch_plain(Params P, const Maps& maps, cudaStream_t stream) {
   static_assert(MODE != DW, "DW has its own operands");
   P.out_vec = aligned(P.out, 16);
   P.idx_vec = 0;
   P.n_tiles = (P.Ng + BN - 1) / BN;
   P.k_blocks = (P.Kg + BK - 1) / BK;
-  if (P.Mg >= PACKR_PLAIN_MSUB2_MIN_M) return launch_impl<MODE, B_PLAIN, 2>(P, maps, stream);
-  return launch_impl<MODE, B_PLAIN, 1>(P, maps, stream);
+  if (P.Mg >= PACKR_PLAIN_MSUB2_MIN_M) return launch_impl<MODE, B_PLAIN, 2, EPI>(P, maps, stream);
+  return launch_impl<MODE, B_PLAIN, 1, EPI>(P, maps, stream);
 }
 
 }  // namespace gemm

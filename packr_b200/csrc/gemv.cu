@@ -23,6 +23,7 @@
 // the final pass of the skinny tensor-core forward.
 #include <atomic>
 
+#include "activation.cuh"
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -113,12 +114,16 @@ __host__ __device__ constexpr size_t cluster_smem(int rows_per_cta) {
 #ifndef PACKR_GEMV_MIN_CTAS
 #define PACKR_GEMV_MIN_CTAS 3
 #endif
-template <int MB, int CPT, int U>
+// EPI: the fused linear layer's forward: W = bf16(W_f + bf16(lut[W_p])), as its
+// tensor-core routes decode it (add.rn.bf16x2 of a pair), x rounded to bf16
+// like their operand, and the epilogue of `epi` in place of the bare f32
+// store.
+template <int MB, int CPT, int U, bool EPI>
 __global__ void __launch_bounds__(kThreads, (MB <= 2 ? PACKR_GEMV_MIN_CTAS : 2))
     gemv_cluster_kernel(const void* __restrict__ x, int x_f32, int Mr, const uint8_t* __restrict__ W_p,
                         const uint16_t* __restrict__ W_f, const float* __restrict__ lut,
                         const void* __restrict__ bias, int bias_f32, float* __restrict__ out, int K, int N,
-                        int rows_per_cta, int rows_per_warp) {
+                        int rows_per_cta, int rows_per_warp, const Epilogue epi) {
   static_assert(8 * MB * 32 * CPT <= 256 * 32, "warp sums must fit in the lut region");
   static_assert(kThreads == 256, "one lut entry per thread");
   constexpr int kCols = 32 * CPT;
@@ -136,16 +141,18 @@ __global__ void __launch_bounds__(kThreads, (MB <= 2 ? PACKR_GEMV_MIN_CTAS : 2))
   {
     // thread t loads lut[t] once and writes its 32 lane copies, rotated so
     // that the warp's stores fall in 32 different banks
-    const uint32_t v = __float_as_uint(__half2float(__float2half_rn(__ldg(lut + threadIdx.x))));
+    const uint32_t v = EPI ? f32_to_bf16_rne(__ldg(lut + threadIdx.x))
+                           : __float_as_uint(__half2float(__float2half_rn(__ldg(lut + threadIdx.x))));
 #pragma unroll 8
     for (int l = 0; l < 32; ++l) lut_s[threadIdx.x * 32 + ((l + lane) & 31)] = v;
   }
   for (int i = threadIdx.x; i < nrows_cta * MB; i += kThreads) {
     const int r = i / MB, m = i - r * MB;
     const long long src = (long long)m * K + k0 + r;
-    const float v = m >= Mr ? 0.0f
-                            : x_f32 ? __ldg(static_cast<const float*>(x) + src)
-                                    : bf16_to_f32(__ldg(static_cast<const uint16_t*>(x) + src));
+    float v = m >= Mr ? 0.0f
+                      : x_f32 ? __ldg(static_cast<const float*>(x) + src)
+                              : bf16_to_f32(__ldg(static_cast<const uint16_t*>(x) + src));
+    if (EPI && x_f32) v = __uint_as_float(pack_bf16x2_rne(0.0f, v));
     xs[i] = pk2(v, v);
   }
   __syncthreads();
@@ -167,9 +174,15 @@ __global__ void __launch_bounds__(kThreads, (MB <= 2 ? PACKR_GEMV_MIN_CTAS : 2))
     for (int j = 0; j < CPT / 2; ++j) {
       const uint32_t fw = w.fword(j);
       const uint32_t pw = w.pword(j >> 1) >> (16 * (j & 1));
-      const float f0 = __fadd_rn(__uint_as_float(fw << 16), __uint_as_float(lut_lane[(pw & 0xFFu) * 32]));
-      const float f1 = __fadd_rn(__uint_as_float(fw & 0xFFFF0000u), __uint_as_float(lut_lane[((pw >> 8) & 0xFFu) * 32]));
-      wv[j] = pk2(f0, f1);
+      const uint32_t l0 = lut_lane[(pw & 0xFFu) * 32], l1 = lut_lane[((pw >> 8) & 0xFFu) * 32];
+      if (EPI) {
+        const uint32_t d = gemm::bf16x2_add(fw, gemm::prmt(l0, l1, 0x5410u));
+        wv[j] = pk2(__uint_as_float(d << 16), __uint_as_float(d & 0xFFFF0000u));
+      } else {
+        const float f0 = __fadd_rn(__uint_as_float(fw << 16), __uint_as_float(l0));
+        const float f1 = __fadd_rn(__uint_as_float(fw & 0xFFFF0000u), __uint_as_float(l1));
+        wv[j] = pk2(f0, f1);
+      }
     }
     const f32x2* xr = xs + r * MB;
 #pragma unroll
@@ -260,7 +273,15 @@ __global__ void __launch_bounds__(kThreads, (MB <= 2 ? PACKR_GEMV_MIN_CTAS : 2))
       if (bias != nullptr)
         t = __fadd_rn(t, bias_f32 ? __ldg(static_cast<const float*>(bias) + n)
                                   : bf16_to_f32(__ldg(static_cast<const uint16_t*>(bias) + n)));
-      out[(long long)m * N + n] = t;
+      const long long o = (long long)m * N + n;
+      if (EPI) {
+        if (epi.z != nullptr) store_io(epi.z, o, epi.io_f32, t);
+        act::apply_all<1>(epi.act, &t);
+        if (epi.residual != nullptr) t = __fadd_rn(t, load_io(epi.residual, o, epi.io_f32));
+        store_io(epi.out, o, epi.io_f32, t);
+      } else {
+        out[o] = t;
+      }
     }
   }
   cluster_sync_all();  // no CTA leaves while a peer may still read its sums
@@ -374,10 +395,10 @@ inline bool eligible(long long M, long long K, long long N, const uint8_t* W_p, 
 
 inline size_t workspace_bytes(long long, long long, long long) { return 0; }
 
-template <int MB, int CPT, int U = PACKR_GEMV_ROWS_IN_FLIGHT>
+template <int MB, int CPT, bool EPI, int U = PACKR_GEMV_ROWS_IN_FLIGHT>
 int launch(const Plan& p, const void* x, int x_f32, int Mr, const uint8_t* W_p, const uint16_t* W_f, const float* lut,
-           const void* bias, int bias_f32, float* out, long long K, long long N, cudaStream_t st) {
-  auto kern = gemv_cluster_kernel<MB, CPT, U>;
+           const void* bias, int bias_f32, float* out, long long K, long long N, cudaStream_t st, const Epilogue& epi) {
+  auto kern = gemv_cluster_kernel<MB, CPT, U, EPI>;
   // per-device flag; relaxed atomics: concurrent first calls set the same attributes
   static std::atomic<int> attr_done[64];
   int dev = 0;
@@ -415,36 +436,49 @@ int launch(const Plan& p, const void* x, int x_f32, int Mr, const uint8_t* W_p, 
       continue;
     }
     if (cudaLaunchKernelEx(&cfg, kern, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, (int)K, (int)N,
-                           q.rows_per_cta, q.rows_per_warp) != cudaSuccess)
+                           q.rows_per_cta, q.rows_per_warp, epi) != cudaSuccess)
       return launch_status();
     return launch_status();
   }
 }
 
-template <int MB>
+template <int MB, bool EPI>
 int launch_cpt(const Plan& p, const void* x, int x_f32, int Mr, const uint8_t* W_p, const uint16_t* W_f,
                const float* lut, const void* bias, int bias_f32, float* out, long long K, long long N,
-               cudaStream_t st) {
+               cudaStream_t st, const Epilogue& epi) {
   if constexpr (MB <= 4) {
-    if (p.cpt == 8) return launch<MB, 8>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st);
+    if (p.cpt == 8) return launch<MB, 8, EPI>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st, epi);
   }
   if constexpr (MB <= 8) {
-    if (p.cpt == 4) return launch<MB, 4>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st);
+    if (p.cpt == 4) return launch<MB, 4, EPI>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st, epi);
   }
-  return launch<MB, 2>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st);
+  return launch<MB, 2, EPI>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st, epi);
+}
+
+template <bool EPI>
+int forward_impl(const void* x, int x_f32, const uint8_t* W_p, const uint16_t* W_f, const float* lut, const void* bias,
+                 int bias_f32, float* out, long long M, long long K, long long N, cudaStream_t st,
+                 const Epilogue& epi) {
+  const Plan p = plan(M, K, N);
+  const int Mr = (int)M;
+  switch (p.mb) {
+    case 1: return launch_cpt<1, EPI>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st, epi);
+    case 2: return launch_cpt<2, EPI>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st, epi);
+    case 4: return launch_cpt<4, EPI>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st, epi);
+    case 8: return launch_cpt<8, EPI>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st, epi);
+    default: return launch_cpt<16, EPI>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st, epi);
+  }
 }
 
 int forward(const void* x, int x_f32, const uint8_t* W_p, const uint16_t* W_f, const float* lut, const void* bias,
             int bias_f32, float* out, long long M, long long K, long long N, float* /*unused*/, cudaStream_t st) {
-  const Plan p = plan(M, K, N);
-  const int Mr = (int)M;
-  switch (p.mb) {
-    case 1: return launch_cpt<1>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st);
-    case 2: return launch_cpt<2>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st);
-    case 4: return launch_cpt<4>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st);
-    case 8: return launch_cpt<8>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st);
-    default: return launch_cpt<16>(p, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, K, N, st);
-  }
+  return forward_impl<false>(x, x_f32, W_p, W_f, lut, bias, bias_f32, out, M, K, N, st, Epilogue{});
+}
+
+// The fused linear layer's forward for few rows (see gemv_cluster_kernel).
+int forward_epi(const void* x, int x_f32, const uint8_t* W_p, const uint16_t* W_f, const float* lut, const void* bias,
+                int bias_f32, const Epilogue& epi, long long M, long long K, long long N, cudaStream_t st) {
+  return forward_impl<true>(x, x_f32, W_p, W_f, lut, bias, bias_f32, nullptr, M, K, N, st, epi);
 }
 
 }  // namespace gemv

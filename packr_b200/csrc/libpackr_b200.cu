@@ -10,6 +10,8 @@
 #include "skinny.cu"
 #include "linear.cu"
 #include "static_scratch.cu"
+#include "layer_norm.cu"
+#include "linear_act.cu"
 #include "velvet.cu"
 #include "compress.cu"
 #include "peer.cu"

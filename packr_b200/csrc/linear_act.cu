@@ -1,0 +1,458 @@
+// The linear layer with bias, activation and residual in its epilogue:
+//   z = x @ W + bias,  out = act(z) + residual,  W = bf16(W_f + bf16(lut[W_p]))
+//   dz = dout * act'(z);  dX = dz @ W^T;  dW_f = x^T @ dz;  dbias = column sums
+//   of dz;  dlut = W_p-binned sums of dW_f / (count + 1e-8);  dresidual = dout
+// x bf16 or f32 (rounded to bf16, the tensor cores' operand); residual, out, z
+// and dout of one type.  z, the only tensor kept for the backward besides x,
+// is stored in that type: its rounding moves act'(z) by at most the half step
+// of the type, which is what a bf16 layer followed by a bf16 activation keeps.
+//
+// Routes (forward): up to 4 rows the CUDA-core GEMV; 5..128 rows the skinny
+// tcgen05 GEMM and its reduction; from 129 rows, and wherever W's rows do not
+// allow TMA (N % 16 != 0 or a misaligned base), W is decoded once into the
+// workspace, with rows padded to a multiple of 8, and read by TMA, so that odd
+// widths take the same tensor-core GEMM as even ones.  The backward takes dz
+// in one pass over dout and z (bf16 operand, optional residual part of the
+// split, column sums), then the existing dX and dW GEMMs.
+#include "activation.cuh"
+
+namespace packr {
+namespace linear_act {
+
+using linear::Carve;
+using linear::round8;
+
+// ------------------------------------------------------------------ decode of any W
+// W [K, N] -> bf16 [K, ldw], ldw = round8(N), pad columns zero.  One thread per
+// 8 consecutive columns of a row: byte and 16-bit loads (rows start at any
+// address), one 16-byte store.  Bound by load instructions, not bytes; it
+// serves the widths that the streaming decode (16-byte rows) cannot.
+__global__ void __launch_bounds__(256) decode_any_kernel(const uint8_t* __restrict__ W_p,
+                                                         const uint16_t* __restrict__ W_f,
+                                                         const float* __restrict__ lut, uint4* __restrict__ out,
+                                                         long long K, int N, int chunks_per_row) {
+  __shared__ uint16_t lut_s[256];
+  lut_s[threadIdx.x] = (uint16_t)f32_to_bf16_rne(__ldg(lut + threadIdx.x));
+  __syncthreads();
+  const long long total = K * chunks_per_row;
+  for (long long c = (long long)blockIdx.x * 256 + threadIdx.x; c < total; c += (long long)gridDim.x * 256) {
+    const long long r = c / chunks_per_row;
+    const int n0 = (int)(c - r * chunks_per_row) * 8;
+    const long long off = r * N + n0;
+    uint32_t f[8], p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool in = n0 + j < N;
+      f[j] = in ? __ldg(W_f + off + j) : 0u;
+      p[j] = in ? __ldg(W_p + off + j) : 0u;
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = gemm::bf16x2_add(f[2 * j] | (f[2 * j + 1] << 16),
+                              (uint32_t)lut_s[p[2 * j]] | ((uint32_t)lut_s[p[2 * j + 1]] << 16));
+      if (n0 + 2 * j >= N) w[j] = 0u;
+      else if (n0 + 2 * j + 1 >= N) w[j] &= 0xFFFFu;
+    }
+    out[c] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// bf16 W [K, round8(N)] for the plain GEMMs.
+int decode(const uint8_t* W_p, const uint16_t* W_f, const float* lut, uint16_t* out, long long K, long long N,
+           cudaStream_t st) {
+  if (gemm::wtma_ok(W_p, W_f, N)) return gemm::predecode(W_p, W_f, lut, out, K, N, st);
+  const int cpr = (int)(round8(N) / 8);
+  const long long blocks = (K * cpr + 255) / 256;
+  const long long cap = 16LL * sm_count();
+  decode_any_kernel<<<(int)(blocks < cap ? blocks : cap), 256, 0, st>>>(W_p, W_f, lut, reinterpret_cast<uint4*>(out), K,
+                                                                        (int)N, cpr);
+  return launch_status();
+}
+
+// ------------------------------------------------------------------ dz
+// dz = dout * act'(z) for a slab of rows:
+//   hi[r, c] = bf16(dz), lo[r, c] = bf16(dz - hi) (optional; the difference is
+//   exact in f32), colsum[slab][c] = sum over the slab's rows of dz (optional).
+// A thread owns 8 columns and walks its slab's rows, two rows' loads in
+// flight; sums of different slabs are added in order by a second launch.
+// hi == nullptr: only the column sums (a bf16 dout without activation is the
+// GEMMs' operand as it stands).
+constexpr int kDzUnroll = 2;
+template <bool F32, int ACT>
+__global__ void __launch_bounds__(256) dz_kernel(const void* __restrict__ dout, const void* __restrict__ z, int M,
+                                                 int N, int rows_per_slab, uint16_t* __restrict__ hi,
+                                                 uint16_t* __restrict__ lo, long long ld, int vec,
+                                                 float* __restrict__ colsum) {
+  const long long c0 = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8;
+  if (c0 >= N) return;
+  const int r0 = blockIdx.y * rows_per_slab;
+  const int r1 = min(M, r0 + rows_per_slab);
+  const int nc = (int)min(8ll, (long long)N - c0);
+  const bool v8 = vec && nc == 8;
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  auto load = [&](const void* src, int r, float* v) {
+    const long long off = (long long)r * N + c0;
+    if (v8) {
+      prep::load8<F32>(src, off, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < nc ? load_io(src, off + j, F32) : 0.0f;
+    }
+  };
+  auto emit = [&](int r, float* d) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] += d[j];
+    if (hi == nullptr) return;
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      h[j] = pack_bf16x2_rne(d[2 * j], d[2 * j + 1]);
+      l[j] = pack_bf16x2_rne(__fsub_rn(d[2 * j], __uint_as_float(h[j] << 16)),
+                             __fsub_rn(d[2 * j + 1], __uint_as_float(h[j] & 0xFFFF0000u)));
+    }
+    // ld is a multiple of 8: the padding of a ragged row is written as zero
+    *reinterpret_cast<uint4*>(hi + (long long)r * ld + c0) = make_uint4(h[0], h[1], h[2], h[3]);
+    if (lo != nullptr) *reinterpret_cast<uint4*>(lo + (long long)r * ld + c0) = make_uint4(l[0], l[1], l[2], l[3]);
+  };
+  for (int r = r0; r < r1; r += kDzUnroll) {
+    float d[kDzUnroll][8], zz[kDzUnroll][8];
+#pragma unroll
+    for (int u = 0; u < kDzUnroll; ++u) {
+      if (r + u < r1) {
+        load(dout, r + u, d[u]);
+        if (ACT != PACKR_ACT_NONE) load(z, r + u, zz[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kDzUnroll; ++u) {
+      if (r + u < r1) {
+        if (ACT != PACKR_ACT_NONE) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[u][j] *= act::slope<ACT>(zz[u][j]);
+        }
+        emit(r + u, d[u]);
+      }
+    }
+  }
+  if (colsum != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < nc) colsum[(long long)blockIdx.y * N + c0 + j] = acc[j];
+  }
+}
+
+struct DzPlan {
+  int threads, slabs, rows_per_slab;
+  unsigned col_blocks;
+};
+// About four CTAs of 256 threads' worth per SM, at least 8 rows a slab.
+inline DzPlan dz_plan(long long M, long long N) {
+  DzPlan p{};
+  const long long chunks = (N + 7) / 8;
+  p.threads = (int)(chunks >= 256 ? 256 : (chunks + 31) / 32 * 32);
+  p.col_blocks = (unsigned)((chunks + p.threads - 1) / p.threads);
+  long long want = 4LL * sm_count() * 256 / ((long long)p.col_blocks * p.threads);
+  const long long most = (M + 7) / 8;
+  if (want > most) want = most;
+  if (want > 1024) want = 1024;
+  if (want < 1) want = 1;
+  p.rows_per_slab = (int)((M + want - 1) / want);
+  p.slabs = (int)((M + p.rows_per_slab - 1) / p.rows_per_slab);
+  return p;
+}
+
+template <bool F32>
+int dz_launch(int a, const void* dout, const void* z, long long M, long long N, uint16_t* hi, uint16_t* lo,
+              long long ld, float* colsum, cudaStream_t st) {
+  const DzPlan p = dz_plan(M, N);
+  const dim3 grid(p.col_blocks, (unsigned)p.slabs);
+  const int vec = (N & 7) == 0 && aligned(dout, 16) && aligned(z, 16);
+#define PACKR_DZ(A)                                                                                                  \
+  dz_kernel<F32, A><<<grid, p.threads, 0, st>>>(dout, z, (int)M, (int)N, p.rows_per_slab, hi, lo, ld, vec, colsum)
+  switch (a) {
+    case PACKR_ACT_RELU: PACKR_DZ(PACKR_ACT_RELU); break;
+    case PACKR_ACT_GELU: PACKR_DZ(PACKR_ACT_GELU); break;
+    case PACKR_ACT_GELU_TANH: PACKR_DZ(PACKR_ACT_GELU_TANH); break;
+    case PACKR_ACT_SILU: PACKR_DZ(PACKR_ACT_SILU); break;
+    default: PACKR_DZ(PACKR_ACT_NONE); break;
+  }
+#undef PACKR_DZ
+  return launch_status();
+}
+
+// ------------------------------------------------------------------ plans
+enum Route { GEMV, SKINNY, PLAIN };
+
+inline Route route(long long M, long long K, long long N, const uint8_t* W_p, const uint16_t* W_f) {
+  if (linear::skinny_eligible(M, N) && gemm::wtma_ok(W_p, W_f, N)) return SKINNY;
+  if (gemv::eligible(M, K, N, W_p, W_f)) return GEMV;
+  return PLAIN;
+}
+
+struct Fwd {
+  uint16_t *xh, *wd;
+  float *part, *skp;
+  int* skf;
+};
+
+size_t plan_forward(Carve& c, Fwd& p, Route r, long long M, long long K, long long N, int x_dtype) {
+  p = Fwd{};
+  if (r == GEMV) return 0;
+  p.xh = linear::x_needs_copy(x_dtype, K) ? c.take<uint16_t>((size_t)M * round8(K)) : nullptr;
+  if (r == SKINNY) {
+    p.part = c.take<float>(gemm::skinny_partial_bytes(M, K, N) / sizeof(float));
+  } else {
+    p.wd = c.take<uint16_t>((size_t)K * round8(N));
+    p.skp = c.take<float>(gemm::sk_partial_bytes(linear::sk_pairs(), linear::plain_msub(M)) / sizeof(float));
+    p.skf = c.take<int>(gemm::sk_flag_bytes(linear::sk_pairs()) / sizeof(int));
+  }
+  return c.off;
+}
+
+struct Bwd {
+  uint16_t *dh, *dl, *xh, *xl, *wd;
+  float *part, *skp, *colsum, *dlut_sum;
+  int* skf;
+  int32_t* counts;
+};
+
+size_t plan_backward(Carve& c, Bwd& p, long long M, long long K, long long N, int x_dtype, int flags, bool direct,
+                     bool skinny, bool dx, bool dw, bool dlut, bool dbias, bool have_counts) {
+  p = Bwd{};
+  const bool need_x = dw || dlut;
+  const bool split = (flags & PACKR_BWD_DW_SPLIT) != 0 && need_x;
+  if (dx && skinny) {
+    p.part = c.take<float>(gemm::skinny_partial_bytes(M, N, K) / sizeof(float));
+  } else if (dx) {
+    p.wd = c.take<uint16_t>((size_t)K * round8(N));
+    p.skp = c.take<float>(gemm::sk_partial_bytes(linear::sk_pairs(), linear::plain_msub(M)) / sizeof(float));
+    p.skf = c.take<int>(gemm::sk_flag_bytes(linear::sk_pairs()) / sizeof(int));
+  }
+  p.dh = direct ? nullptr : c.take<uint16_t>((size_t)M * round8(N));
+  p.dl = split && !direct ? c.take<uint16_t>((size_t)M * round8(N)) : nullptr;
+  p.xh = need_x && linear::x_needs_copy(x_dtype, K) ? c.take<uint16_t>((size_t)M * round8(K)) : nullptr;
+  p.xl = need_x && split && x_dtype == PACKR_DTYPE_F32 ? c.take<uint16_t>((size_t)M * round8(K)) : nullptr;
+  p.colsum = dbias ? c.take<float>((size_t)dz_plan(M, N).slabs * N) : nullptr;
+  p.dlut_sum = dlut ? c.take<float>(256) : nullptr;
+  p.counts = dlut && !have_counts ? c.take<int32_t>(256) : nullptr;
+  return c.off;
+}
+
+inline bool act_ok(int a) { return a >= PACKR_ACT_NONE && a <= PACKR_ACT_SILU; }
+inline bool io_ok(int d) { return d == PACKR_DTYPE_F32 || d == PACKR_DTYPE_BF16; }
+inline size_t io_size(int d) { return d == PACKR_DTYPE_F32 ? 4 : 2; }
+
+// x as the GEMMs' bf16 operand (a copy in xh, with its residual part in xl,
+// when its type or row length needs one).
+int operand_x(const void* x, int x_dtype, long long M, long long K, uint16_t* xh, uint16_t* xl, const void** a,
+              long long* lda, cudaStream_t s) {
+  *a = x;
+  *lda = K;
+  if (xh == nullptr) return PACKR_OK;
+  *a = xh;
+  *lda = round8(K);
+  // grid.y of the copy holds 65535 blocks of 32 rows
+  for (long long r = 0; r < M; r += 65535LL * prep::kRowsPerCta) {
+    const long long n = M - r < 65535LL * prep::kRowsPerCta ? M - r : 65535LL * prep::kRowsPerCta;
+    const char* src = static_cast<const char*>(x) + (size_t)(r * K) * io_size(x_dtype);
+    int st = prep::split_rows(src, x_dtype == PACKR_DTYPE_F32, K, n, K, xh + r * round8(K),
+                              xl ? xl + r * round8(K) : nullptr, round8(K), nullptr, s);
+    if (st != PACKR_OK) return st;
+  }
+  return PACKR_OK;
+}
+
+}  // namespace linear_act
+}  // namespace packr
+
+extern "C" size_t packr_linear_act_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, const uint8_t* W_p,
+                                                   const uint16_t* W_f) {
+  using namespace packr;
+  if (M <= 0 || K <= 0 || N <= 0) return 0;
+  linear::Carve c{nullptr};
+  linear_act::Fwd p;
+  return linear_act::plan_forward(c, p, linear_act::route(M, K, N, W_p, W_f), M, K, N, x_dtype);
+}
+
+extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_t* W_p, const uint16_t* W_f,
+                                        const float* lut, const void* bias, int bias_dtype, int activation,
+                                        const void* residual, void* out, void* z, int out_dtype, int64_t M, int64_t K,
+                                        int64_t N, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace packr;
+  using namespace packr::linear_act;
+  int st = linear::check_common(x, x_dtype, W_p, W_f, lut, M, K, N);
+  if (st != PACKR_OK) return st;
+  if (!act_ok(activation) || !io_ok(out_dtype) || (bias != nullptr && !io_ok(bias_dtype)))
+    return PACKR_ERR_INVALID_ARGUMENT;
+  if (M > 0 && out == nullptr) return PACKR_ERR_INVALID_ARGUMENT;
+  const size_t ob = io_size(out_dtype);
+  if (!aligned(out, ob) || !aligned(residual, ob) || !aligned(z, ob) ||
+      (bias != nullptr && !aligned(bias, io_size(bias_dtype))))
+    return PACKR_ERR_ALIGNMENT;
+  if ((st = check_device()) != PACKR_OK) return st;
+  if (M == 0) return PACKR_OK;
+  cudaStream_t s = as_stream(stream);
+  const Route r = route(M, K, N, W_p, W_f);
+  Carve c{static_cast<uint8_t*>(workspace)};
+  Fwd p;
+  const size_t need = linear_act::plan_forward(c, p, r, M, K, N, x_dtype);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, linear::kAlign)))
+    return PACKR_ERR_WORKSPACE;
+  Epilogue e{};
+  e.residual = residual;
+  e.out = out;
+  e.z = z;
+  e.io_f32 = out_dtype == PACKR_DTYPE_F32;
+  e.act = activation;
+  e.vec = aligned(out, 16) && aligned(residual, 16) && aligned(z, 16) && (N * ob) % 16 == 0;
+  const int bias_f32 = bias_dtype == PACKR_DTYPE_F32;
+  if (r == GEMV)
+    return gemv::forward_epi(x, x_dtype == PACKR_DTYPE_F32, W_p, W_f, lut, bias, bias_f32, e, M, K, N, s);
+  const void* a;
+  long long lda;
+  if ((st = operand_x(x, x_dtype, M, K, p.xh, nullptr, &a, &lda, s)) != PACKR_OK) return st;
+  if (r == SKINNY)
+    return gemm::skinny_forward_epi(static_cast<const uint16_t*>(a), lda, W_p, W_f, lut, bias, bias_f32, e, M, K, N,
+                                    p.part, s);
+  gemm::Maps maps;
+  if ((st = gemm::make_map(&maps.a[0], a, K, M, lda * 2, gemm::BM)) != PACKR_OK) return st;
+  if ((st = gemm::make_map(&maps.b[0], p.wd, N, K, round8(N) * 2, 64)) != PACKR_OK) return st;
+  if ((st = decode(W_p, W_f, lut, p.wd, K, N, s)) != PACKR_OK) return st;
+  gemm::Params P{};
+  P.Mg = (int)M;
+  P.Ng = (int)N;
+  P.Kg = (int)K;
+  P.nseg = 1;
+  P.ld_out = N;
+  P.bias = bias;
+  P.bias_f32 = bias_f32;
+  P.epi = e;
+  P.sk_partial = p.skp;
+  P.sk_flags = p.skf;
+  P.sk_slots = linear::sk_pairs();
+  return gemm::launch_plain<gemm::FWD, true>(P, maps, s);
+}
+
+extern "C" size_t packr_linear_act_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, int flags,
+                                                            const uint8_t* W_p, const uint16_t* W_f) {
+  using namespace packr;
+  if (M <= 0 || K <= 0 || N <= 0) return 0;
+  linear::Carve c{nullptr};
+  linear_act::Bwd p;
+  const bool skinny = linear::skinny_dx_eligible(M, N) && gemm::wtma_ok(W_p, W_f, N);
+  return linear_act::plan_backward(c, p, M, K, N, x_dtype, flags, false, skinny, true, true, true, true, false);
+}
+
+extern "C" int packr_linear_act_backward(const void* dout, const void* z, int out_dtype, int activation, const void* x,
+                                         int x_dtype, const uint8_t* W_p, const uint16_t* W_f, const float* lut,
+                                         const int32_t* lut_counts, void* dX, uint16_t* dW_f, float* dlut, void* dbias,
+                                         int dbias_dtype, int64_t M, int64_t K, int64_t N, int flags, void* workspace,
+                                         size_t workspace_bytes, void* stream) {
+  using namespace packr;
+  using namespace packr::linear_act;
+  int st = linear::check_common(x, x_dtype, W_p, W_f, lut, M, K, N);
+  if (st != PACKR_OK) return st;
+  if (!act_ok(activation) || !io_ok(out_dtype) || (dbias != nullptr && !io_ok(dbias_dtype)) ||
+      (flags & ~PACKR_BWD_DW_SPLIT) != 0)
+    return PACKR_ERR_INVALID_ARGUMENT;
+  if (M > 0 && (dout == nullptr || (activation != PACKR_ACT_NONE && z == nullptr))) return PACKR_ERR_INVALID_ARGUMENT;
+  const size_t ob = io_size(out_dtype);
+  if (!aligned(dout, ob) || !aligned(z, ob) || !aligned(dX, io_size(x_dtype)) || !aligned(dW_f, 2) ||
+      !aligned(dlut, 4) || !aligned(lut_counts, 4) || (dbias != nullptr && !aligned(dbias, io_size(dbias_dtype))))
+    return PACKR_ERR_ALIGNMENT;
+  if ((st = check_device()) != PACKR_OK) return st;
+  cudaStream_t s = as_stream(stream);
+  const bool dx = dX != nullptr, dw = dW_f != nullptr, dl = dlut != nullptr, db = dbias != nullptr;
+  if (M == 0) {  // empty batch: every gradient is zero
+    if (dw && cudaMemsetAsync(dW_f, 0, (size_t)K * N * 2, s) != cudaSuccess) return PACKR_ERR_CUDA;
+    if (dl && cudaMemsetAsync(dlut, 0, 256 * 4, s) != cudaSuccess) return PACKR_ERR_CUDA;
+    if (db && cudaMemsetAsync(dbias, 0, (size_t)N * io_size(dbias_dtype), s) != cudaSuccess) return PACKR_ERR_CUDA;
+    return PACKR_OK;
+  }
+  if (!dx && !dw && !dl && !db) return PACKR_OK;
+  // a bf16 dout without activation is the GEMMs' operand as it stands (and
+  // its split residual part is zero)
+  const bool direct = activation == PACKR_ACT_NONE && out_dtype == PACKR_DTYPE_BF16 && (N & 7) == 0 && aligned(dout, 16);
+  const bool skinny = linear::skinny_dx_eligible(M, N) && gemm::wtma_ok(W_p, W_f, N);
+  Carve c{static_cast<uint8_t*>(workspace)};
+  Bwd p;
+  const size_t need = linear_act::plan_backward(c, p, M, K, N, x_dtype, flags, direct, skinny, dx, dw, dl, db,
+                                                lut_counts != nullptr);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, linear::kAlign)))
+    return PACKR_ERR_WORKSPACE;
+  const long long ldN = round8(N);
+  const uint16_t* dh = direct ? static_cast<const uint16_t*>(dout) : p.dh;
+  if (!direct || db) {
+    const void* zz = activation != PACKR_ACT_NONE ? z : nullptr;
+    st = out_dtype == PACKR_DTYPE_F32 ? dz_launch<true>(activation, dout, zz, M, N, p.dh, p.dl, ldN, p.colsum, s)
+                                      : dz_launch<false>(activation, dout, zz, M, N, p.dh, p.dl, ldN, p.colsum, s);
+    if (st != PACKR_OK) return st;
+  }
+  if (db) {
+    const int slabs = dz_plan(M, N).slabs;
+    st = dbias_dtype == PACKR_DTYPE_F32
+             ? norm::reduce_cols(p.colsum, slabs, 1, N, static_cast<float*>(dbias), static_cast<float*>(nullptr), s)
+             : norm::reduce_cols(p.colsum, slabs, 1, N, static_cast<uint16_t*>(dbias),
+                                 static_cast<uint16_t*>(nullptr), s);
+    if (st != PACKR_OK) return st;
+  }
+  if (dx && skinny) {
+    st = gemm::skinny_dx(dh, ldN, W_p, W_f, lut, dX, x_dtype == PACKR_DTYPE_F32, M, K, N, p.part, s);
+    if (st != PACKR_OK) return st;
+  } else if (dx) {
+    gemm::Maps maps;
+    if ((st = gemm::make_map(&maps.a[0], dh, N, M, ldN * 2, gemm::BM)) != PACKR_OK) return st;
+    if ((st = gemm::make_map(&maps.b[0], p.wd, N, K, ldN * 2, gemm::BN_CTA)) != PACKR_OK) return st;
+    if ((st = decode(W_p, W_f, lut, p.wd, K, N, s)) != PACKR_OK) return st;
+    gemm::Params P{};
+    P.Mg = (int)M;
+    P.Ng = (int)K;
+    P.Kg = (int)N;
+    P.nseg = 1;
+    P.out = dX;
+    P.ld_out = K;
+    P.out_f32 = x_dtype == PACKR_DTYPE_F32;
+    P.sk_partial = p.skp;
+    P.sk_flags = p.skf;
+    P.sk_slots = linear::sk_pairs();
+    if ((st = gemm::launch_plain<gemm::DX>(P, maps, s)) != PACKR_OK) return st;
+  }
+  if (dw || dl) {
+    const void* xa;
+    long long ldx;
+    if ((st = operand_x(x, x_dtype, M, K, p.xh, p.xl, &xa, &ldx, s)) != PACKR_OK) return st;
+    // reduction segments: x.dh [+ x.dl] [+ xl.dh]
+    gemm::Maps maps;
+    int nseg = 0;
+    auto add_seg = [&](const void* a, const void* b) -> int {
+      int rc = gemm::make_map(&maps.a[nseg], a, K, M, ldx * 2, 64);
+      if (rc == PACKR_OK) rc = gemm::make_map(&maps.b[nseg], b, N, M, ldN * 2, 64);
+      ++nseg;
+      return rc;
+    };
+    if ((st = add_seg(xa, dh)) != PACKR_OK) return st;
+    if (p.dl != nullptr && (st = add_seg(xa, p.dl)) != PACKR_OK) return st;
+    if (p.xl != nullptr && (st = add_seg(p.xl, dh)) != PACKR_OK) return st;
+    if (dl && cudaMemsetAsync(p.dlut_sum, 0, 256 * 4, s) != cudaSuccess) return PACKR_ERR_CUDA;
+    gemm::Params P{};
+    P.Mg = (int)K;
+    P.Ng = (int)N;
+    P.Kg = (int)M;
+    P.nseg = nseg;
+    P.out = dW_f;
+    P.ld_out = N;
+    P.hist_idx = dl ? W_p : nullptr;
+    P.dlut_sum = p.dlut_sum;
+    if ((st = gemm::launch<gemm::DW>(P, maps, s)) != PACKR_OK) return st;
+  }
+  if (dl) {
+    const int32_t* counts = lut_counts;
+    if (counts == nullptr) {
+      if ((st = prep::bincount256(W_p, K * N, p.counts, s)) != PACKR_OK) return st;
+      counts = p.counts;
+    }
+    return prep::finalize(dlut, p.dlut_sum, counts, nullptr, nullptr, 0, s);
+  }
+  return PACKR_OK;
+}

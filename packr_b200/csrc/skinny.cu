@@ -416,5 +416,68 @@ int skinny_forward(const uint16_t* x_bf16, long long ldx, const uint8_t* W_p, co
   return launch_status();
 }
 
+// The final pass of the skinny forward for the fused linear layer: splits
+// added in order, bias, then the epilogue (Epilogue).  One thread per 4
+// consecutive columns of one row (N % 16 == 0 on this route).
+__global__ void __launch_bounds__(256) skinny_reduce_epi_kernel(const float* __restrict__ partial, int splits, int M,
+                                                                int N, const void* __restrict__ bias, int bias_f32,
+                                                                const Epilogue epi) {
+  const int qpr = N / 4;
+  const long long q = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (q >= (long long)M * qpr) return;
+  const int m = (int)(q / qpr);
+  const int n = (int)(q - (long long)m * qpr) * 4;
+  const long long o = (long long)m * N + n;
+  const long long step = (long long)M * N;
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (epi.residual != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = load_io(epi.residual, o + j, epi.io_f32);
+  }
+  int sp = 0;
+  for (; sp + 4 <= splits; sp += 4) {  // four splits in flight
+    float4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __ldcs(reinterpret_cast<const float4*>(partial + o + (sp + i) * step));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[0] = __fadd_rn(s[0], v[i].x);
+      s[1] = __fadd_rn(s[1], v[i].y);
+      s[2] = __fadd_rn(s[2], v[i].z);
+      s[3] = __fadd_rn(s[3], v[i].w);
+    }
+  }
+  for (; sp < splits; ++sp) {
+    const float4 v = __ldcs(reinterpret_cast<const float4*>(partial + o + sp * step));
+    s[0] = __fadd_rn(s[0], v.x);
+    s[1] = __fadd_rn(s[1], v.y);
+    s[2] = __fadd_rn(s[2], v.z);
+    s[3] = __fadd_rn(s[3], v.w);
+  }
+  if (bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = __fadd_rn(s[j], load_io(bias, n + j, bias_f32));
+  }
+  if (epi.z != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) store_io(epi.z, o + j, epi.io_f32, s[j]);
+  }
+  act::apply_all<4>(epi.act, s);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) store_io(epi.out, o + j, epi.io_f32, __fadd_rn(s[j], r[j]));
+}
+
+// skinny_forward with the fused linear layer's epilogue.
+int skinny_forward_epi(const uint16_t* x_bf16, long long ldx, const uint8_t* W_p, const uint16_t* W_f,
+                       const float* lut, const void* bias, int bias_f32, const Epilogue& epi, long long M, long long K,
+                       long long N, float* partial, cudaStream_t st) {
+  SkPlan pl;
+  int rc = skinny_run<FWD>(x_bf16, ldx, W_p, W_f, lut, M, K, N, partial, pl, st);
+  if (rc != PACKR_OK) return rc;
+  skinny_reduce_epi_kernel<<<gemv::reduce_blocks(M, N), 256, 0, st>>>(partial, pl.splits, (int)M, (int)N, bias,
+                                                                      bias_f32, epi);
+  return launch_status();
+}
+
 }  // namespace gemm
 }  // namespace packr

@@ -14,6 +14,7 @@ tensors raise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -29,6 +30,21 @@ DW_PRECISION = os.environ.get("PACKR_DW_PRECISION", "auto")
 
 def _stream(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _raw_stream(device) -> int:
+    """Handle of torch's current stream on `device`."""
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _on_device(device):
+    """torch.cuda.device(device), at no cost when it is current already."""
+    if device.index == torch.cuda.current_device():
+        return _NO_SWITCH
+    return torch.cuda.device(device)
+
+
+_NO_SWITCH = contextlib.nullcontext()
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -289,6 +305,68 @@ def from_linear_encode(weight: torch.Tensor, codebook: torch.Tensor, scale: torc
                                           _ptr(W_p), _ptr(W_f), _ptr(lut), _stream(dev))
     _lib.check("packr_from_linear_encode", rc)
     return W_p, W_f, lut
+
+
+def linear_act_forward(x: torch.Tensor, W_p: torch.Tensor, W_f: torch.Tensor, lut: torch.Tensor,
+                       bias: torch.Tensor | None, activation: int, residual: torch.Tensor | None,
+                       out_dtype: torch.dtype, keep_z: bool = False):
+    """(out, z) with z = x @ W + bias and out = act(z) + residual, both [M, N]
+    of out_dtype (z None unless keep_z).  x is contiguous 2-D, activation a
+    PACKR_ACT_* code."""
+    lib = _lib.load()
+    M, K = x.shape
+    N = W_p.shape[1]
+    dev = x.device
+    out = torch.empty(M, N, dtype=out_dtype, device=dev)
+    z = torch.empty(M, N, dtype=out_dtype, device=dev) if keep_z else None
+    xd = _dtype_code(x)
+    wp, wf = W_p.data_ptr(), W_f.data_ptr()
+    with _on_device(dev):
+        nbytes = lib.packr_linear_act_workspace_bytes(M, K, N, xd, wp, wf)
+        ws = _workspace(nbytes, dev)
+        code = lib.packr_linear_act_forward(
+            x.data_ptr(), xd, wp, wf, lut.data_ptr(), None if bias is None else bias.data_ptr(),
+            _dtype_code(bias) if bias is not None else 0, activation, None if residual is None else residual.data_ptr(),
+            out.data_ptr(), None if z is None else z.data_ptr(), _dtype_code(out), M, K, N,
+            None if ws is None else ws.data_ptr(), nbytes, _raw_stream(dev))
+    _lib.check("packr_linear_act_forward", code)
+    return out, z
+
+
+def linear_act_backward(dout: torch.Tensor, z: torch.Tensor | None, activation: int, x: torch.Tensor,
+                        W_p: torch.Tensor, W_f: torch.Tensor, lut: torch.Tensor, counts: torch.Tensor | None,
+                        need_dx: bool, need_dw: bool, need_dlut: bool, dbias_dtype: torch.dtype | None,
+                        dW_out: torch.Tensor | None = None):
+    """Returns (dX, dW_f, dlut, dbias); entries not requested are None (dbias:
+    dbias_dtype None).  dout is contiguous [M, N] of the forward's out_dtype;
+    dW_out as in backward()."""
+    lib = _lib.load()
+    M, K = x.shape
+    N = W_p.shape[1]
+    dev = x.device
+    dX = torch.empty(M, K, dtype=x.dtype, device=dev) if need_dx else None
+    if need_dw and dW_out is not None:
+        if (dW_out.dtype != torch.bfloat16 or tuple(dW_out.shape) != (K, N) or not dW_out.is_contiguous()
+                or dW_out.device != dev):
+            raise ValueError("dW_out must be a contiguous bf16 [K, N] tensor on x's device")
+        dW = dW_out
+    else:
+        dW = torch.empty(K, N, dtype=torch.bfloat16, device=dev) if need_dw else None
+    dlut = torch.empty(256, dtype=torch.float32, device=dev) if need_dlut else None
+    dbias = torch.empty(N, dtype=dbias_dtype, device=dev) if dbias_dtype is not None else None
+    if not (need_dx or need_dw or need_dlut or dbias is not None):
+        return None, None, None, None
+    xd = _dtype_code(x)
+    flags = _lib.PACKR_BWD_DW_SPLIT if dw_split_for(x.dtype) else 0
+    with _on_device(dev):
+        nbytes = lib.packr_linear_act_backward_workspace_bytes(M, K, N, xd, flags, _ptr(W_p), _ptr(W_f))
+        ws = _workspace(nbytes, dev)
+        code = lib.packr_linear_act_backward(
+            _ptr(dout), _ptr(z), _dtype_code(dout), activation, _ptr(x), xd, _ptr(W_p), _ptr(W_f), _ptr(lut),
+            _ptr(counts), _ptr(dX), _ptr(dW), _ptr(dlut), _ptr(dbias),
+            _dtype_code(dbias) if dbias is not None else 0, M, K, N, flags, _ptr(ws), nbytes, _stream(dev))
+    _lib.check("packr_linear_act_backward", code)
+    return dX, dW, dlut, dbias
 
 
 def packr_matmul(x, W_p, W_f, lut, bias=None):

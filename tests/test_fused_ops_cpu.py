@@ -1,0 +1,133 @@
+"""What the fused feed-forward operators refuse, without a GPU, and their
+64-bit reference forms against torch's own functions."""
+import ctypes
+
+import pytest
+import torch
+
+import packr_b200 as packr
+from packr_b200 import _lib
+from fused_reference import ACTS, act64, linear64, norm64, slope64, weights64
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(2, 8)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        packr.packr_layer_norm(x)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        packr.packr_linear_act(x, torch.zeros(8, 4, dtype=torch.uint8), torch.zeros(8, 4, dtype=torch.bfloat16),
+                               torch.zeros(256))
+
+
+def _fake(n=64):
+    """An address that no refused call reads."""
+    return ctypes.c_void_p(0x7F0000000000 + n)
+
+
+def test_linear_act_c_entry_refuses_bad_arguments():
+    lib = _lib.load()
+    a = _fake()
+
+    def fwd(x=a, xd=1, wp=a, wf=a, lut=a, bias=None, bd=0, act=0, res=None, out=a, z=None, od=1, M=4, K=8, N=8):
+        return lib.packr_linear_act_forward(x, xd, wp, wf, lut, bias, bd, act, res, out, z, od, M, K, N, None, 0, None)
+
+    assert fwd(M=-1) == 2 and fwd(K=0) == 2 and fwd(N=0) == 2 and fwd(N=1 << 31) == 2
+    assert fwd(xd=2) == 1 and fwd(od=2) == 1 and fwd(od=-1) == 1 and fwd(act=5) == 1 and fwd(act=-1) == 1
+    assert fwd(bias=a, bd=2) == 1
+    for name in ("x", "wp", "wf", "lut", "out"):
+        assert fwd(**{name: None}) == 1, name
+    odd = _fake(1)
+    for name in ("wf", "lut", "out", "res", "z", "x"):
+        assert fwd(**{name: odd}) == 3, name
+    assert fwd(od=0, out=_fake(2)) == 3 and fwd(bias=_fake(2), bd=0) == 3
+
+    def bwd(dout=a, z=a, od=1, act=2, x=a, xd=1, M=4, K=8, N=8, flags=0, db=None, dbd=0, dw=a):
+        return lib.packr_linear_act_backward(dout, z, od, act, x, xd, a, a, a, None, a, dw, None, db, dbd, M, K, N,
+                                             flags, None, 0, None)
+
+    assert bwd(M=-1) == 2 and bwd(act=9) == 1 and bwd(flags=2) == 1 and bwd(dout=None) == 1
+    assert bwd(z=None) == 1  # an activation's backward needs z
+    assert bwd(db=a, dbd=2) == 1 and bwd(dout=odd) == 3 and bwd(dw=odd) == 3 and bwd(db=_fake(2), dbd=0) == 3
+
+
+def test_layer_norm_c_entry_refuses_bad_arguments():
+    lib = _lib.load()
+    a, odd = _fake(), _fake(1)
+
+    def fwd(x=a, res=None, xd=1, w=a, b=a, wd=1, eps=1e-5, y=a, mean=None, M=4, N=8):
+        return lib.packr_layer_norm_forward(x, res, xd, w, b, wd, eps, y, mean, None, M, N, None)
+
+    assert fwd(M=-1) == 2 and fwd(N=0) == 2 and fwd(M=1 << 31) == 2 and fwd(N=1 << 31) == 2
+    assert fwd(xd=2) == 1 and fwd(wd=3) == 1 and fwd(eps=-1.0) == 1 and fwd(eps=float("nan")) == 1
+    assert fwd(x=None) == 1 and fwd(y=None) == 1
+    for name in ("x", "res", "y", "w", "b", "mean"):
+        assert fwd(**{name: odd}) == 3, name
+
+    def bwd(dy=a, x=a, xd=1, wd=1, mean=a, rstd=a, dx=a, M=4, N=8):
+        return lib.packr_layer_norm_backward(dy, x, None, xd, a, wd, mean, rstd, dx, a, a, M, N, None, 0, None)
+
+    assert bwd(M=-1) == 2 and bwd(N=0) == 2 and bwd(xd=2) == 1 and bwd(wd=2) == 1
+    for name in ("dy", "x", "mean", "rstd"):
+        assert bwd(**{name: None}) == 1, name
+    assert bwd(dx=odd) == 3 and bwd(mean=_fake(2)) == 3
+
+
+def test_workspace_queries_of_empty_problems():
+    lib = _lib.load()
+    assert lib.packr_layer_norm_backward_workspace_bytes(0, 8) == 0
+    assert lib.packr_layer_norm_backward_workspace_bytes(-3, 8) == 0
+    assert lib.packr_linear_act_workspace_bytes(0, 8, 8, 1, None, None) == 0
+    assert lib.packr_linear_act_backward_workspace_bytes(4, 0, 8, 1, 0, None, None) == 0
+
+
+def test_activation_names():
+    assert _lib.ACTIVATIONS == {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def test_module_takes_one_dimension():
+    with pytest.raises(ValueError):
+        packr.PackRLayerNorm((4, 8))
+    with pytest.raises(ValueError):
+        packr.PackRLayerNorm.from_layer_norm(torch.nn.LayerNorm((4, 8)))
+    with pytest.raises(TypeError):
+        packr.PackRLayerNorm.from_layer_norm(torch.nn.Linear(4, 4))
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_reference_forms_follow_torch(act):
+    f = {"none": lambda z: z, "relu": torch.relu, "gelu": torch.nn.functional.gelu, "silu": torch.nn.functional.silu,
+         "gelu_tanh": lambda z: torch.nn.functional.gelu(z, approximate="tanh")}[act]
+    z = torch.linspace(-8, 8, 801, dtype=torch.float64).requires_grad_(True)
+    assert torch.allclose(act64(z, act), f(z), rtol=1e-12, atol=1e-14)
+    want = torch.autograd.grad(f(z).sum(), z)[0]
+    assert torch.allclose(slope64(z, act), want, rtol=1e-9, atol=1e-11)
+    # the Lipschitz bounds that the tolerances use
+    s = slope64(z, act)
+    assert s.abs().max() <= 1.13
+    if act != "relu":
+        assert (s.diff() / z.detach().diff()).abs().max() <= 0.8
+
+
+def test_reference_norm_and_linear_follow_torch():
+    g = torch.Generator().manual_seed(0)
+    x, r, dy = (torch.randn(5, 24, generator=g) for _ in range(3))
+    w, b = torch.randn(24, generator=g), torch.randn(24, generator=g)
+    s = (x.double() + r.double()).requires_grad_(True)
+    wd, bd = w.double().requires_grad_(True), b.double().requires_grad_(True)
+    y = torch.nn.functional.layer_norm(s, (24,), wd, bd, 1e-5)
+    dx, dw, db = torch.autograd.grad(y, [s, wd, bd], dy.double())
+    got = norm64(x, r, w, b, 1e-5, dy)
+    for k, v in (("y", y), ("dx", dx), ("dweight", dw), ("dbias", db)):
+        assert torch.allclose(got[k][0], v, rtol=1e-10, atol=1e-12), k
+    W_p = torch.randint(0, 256, (24, 16), generator=g, dtype=torch.uint8)
+    W_f, lut = torch.randn(24, 16, generator=g).bfloat16(), torch.randn(256, generator=g)
+    W = weights64(W_p, W_f, lut)
+    assert torch.equal(W.bfloat16(), W_f + lut[W_p.long()].bfloat16())  # the layer's decode (a bf16 sum)
+    W = W.requires_grad_(True)
+    xb = x.bfloat16()
+    xd, bias, dout = xb.double().requires_grad_(True), torch.randn(16, generator=g), torch.randn(5, 16, generator=g)
+    out = torch.nn.functional.gelu(xd @ W + bias.double())
+    dx, dw = torch.autograd.grad(out, [xd, W], dout.double())
+    got = linear64(xb, W_p, W_f, lut, bias, "gelu", None, torch.float32, dout)
+    for k, v in (("out", out), ("dx", dx), ("dW_f", dw)):
+        assert torch.allclose(got[k][0], v, rtol=1e-10, atol=1e-12), k

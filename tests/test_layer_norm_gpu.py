@@ -1,0 +1,192 @@
+"""packr_layer_norm on the GPU against its 64-bit form, forward and backward,
+at the sizes, types and alignments where its paths differ."""
+import pytest
+import torch
+
+import packr_b200 as packr
+from fused_reference import check, norm64
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+TYPES = [(BF16, BF16), (BF16, F32), (F32, F32), (F32, BF16)]
+
+
+def case(M, N, xt, wt, seed=0, residual=True, affine="wb", offset=0.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    return {"x": (n(M, N) * 2 + offset).to(xt), "residual": n(M, N).to(xt) if residual else None,
+            "weight": (1 + 0.2 * n(N)).to(wt) if "w" in affine else None,
+            "bias": (0.3 * n(N)).to(wt) if "b" in affine else None, "dy": n(M, N).to(xt)}
+
+
+def run(c, eps=1e-5, need=("x", "residual", "weight", "bias")):
+    leaves = {k: c[k].detach().requires_grad_(True) for k in need if c[k] is not None}
+    args = {**c, **leaves}
+    y = packr.packr_layer_norm(args["x"], args["weight"], args["bias"], eps, args["residual"])
+    if not leaves:
+        return {"y": y}
+    grads = torch.autograd.grad(y, list(leaves.values()), c["dy"])
+    return {"y": y, **dict(zip(("d" + k for k in leaves), grads))}
+
+
+def compare(c, got, eps=1e-5):
+    # bf16: one rounding of the result, at most 2^-8 / sqrt(3) in the 2-norm
+    rel = 2.4e-3 if c["x"].dtype == BF16 else None
+    want = norm64(c["x"], c["residual"], c["weight"], c["bias"], eps, c["dy"])
+    for k, v in got.items():
+        ref = want["dx" if k == "dresidual" else k]
+        check(k, v, ref, rel if k in ("y", "dx", "dresidual") and c["x"].shape[1] > 8 else None)
+
+
+@pytest.mark.parametrize("xt,wt", TYPES)
+@pytest.mark.parametrize("M,N", [(1, 1), (3, 2), (5, 7), (1, 64), (2, 255), (33, 256), (7, 257), (64, 768), (9, 1000),
+                                 (40, 1001), (17, 4096), (5, 4104), (3, 8192), (2, 8200), (3, 8193), (2, 16384)])
+def test_sizes(cuda, M, N, xt, wt):
+    c = case(M, N, xt, wt, seed=M * 31 + N)
+    compare(c, run(c))
+
+
+@pytest.mark.parametrize("xt,wt", [(BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("N", [16385, 20000])
+def test_rows_wider_than_the_register_path(cuda, N, xt, wt):
+    for residual in (True, False):
+        c = case(3, N, xt, wt, seed=N, residual=residual)
+        compare(c, run(c))
+
+
+@pytest.mark.parametrize("affine", ["wb", "w", "b", ""])
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("N", [96, 8200])
+def test_optional_inputs(cuda, affine, residual, N):
+    c = case(21, N, BF16, BF16, seed=3, residual=residual, affine=affine)
+    compare(c, run(c))
+
+
+@pytest.mark.parametrize("M,N", [(5000, 64), (3000, 768), (2001, 1001), (700, 4096)])
+def test_many_rows(cuda, M, N):
+    """More rows than one wave of CTAs: the column sums of many slabs."""
+    c = case(M, N, BF16, F32, seed=9)
+    compare(c, run(c))
+
+
+@pytest.mark.parametrize("need", [("x",), ("weight",), ("bias",), ("residual",), ("weight", "bias"), ()])
+def test_only_the_gradients_asked_for(cuda, need):
+    c = case(50, 200, F32, F32, seed=5)
+    got = run(c, need=need)
+    assert set(got) == {"y"} | {"d" + k for k in need}
+    compare(c, got)
+
+
+def test_large_offset_and_constant_rows(cuda):
+    """A mean far above the spread loses nothing but the input's own bits, and
+    a constant row (variance 0) gives the bias."""
+    c = case(8, 512, F32, F32, seed=1, residual=False, offset=300.0)
+    compare(c, run(c))
+    x = torch.full((4, 96), 7.5, device="cuda")
+    b = torch.randn(96, device="cuda")
+    assert torch.equal(packr.packr_layer_norm(x, torch.ones(96, device="cuda"), b), b.expand(4, 96))
+
+
+def test_non_finite_rows_stay_in_their_rows(cuda):
+    c = case(6, 300, BF16, BF16, seed=2)
+    clean = run(c)
+    for bad in (float("inf"), float("nan")):
+        c["x"][2, 17] = bad
+        got = run(c)
+        for k in ("y", "dx"):
+            assert torch.isnan(got[k][2]).any()
+            keep = [0, 1, 3, 4, 5]
+            assert torch.equal(got[k][keep], clean[k][keep])
+
+
+def test_empty_batch_and_leading_dimensions(cuda):
+    w = torch.ones(32, device="cuda", requires_grad=True)
+    b = torch.zeros(32, device="cuda", requires_grad=True)
+    x = torch.zeros(0, 32, device="cuda", requires_grad=True)
+    y = packr.packr_layer_norm(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y, [x, w, b], torch.zeros_like(y))
+    assert y.shape == (0, 32) and gx.shape == (0, 32) and not gw.any() and not gb.any()
+    c = case(12, 32, F32, F32, seed=4)
+    flat = packr.packr_layer_norm(c["x"], c["weight"], c["bias"], residual=c["residual"])
+    cube = packr.packr_layer_norm(c["x"].view(3, 4, 32), c["weight"], c["bias"], residual=c["residual"].view(3, 4, 32))
+    assert torch.equal(cube, flat.view(3, 4, 32))
+    assert torch.equal(packr.packr_layer_norm(c["x"][0], c["weight"], c["bias"], residual=c["residual"][0]), flat[0])
+
+
+def test_strided_and_misaligned_inputs(cuda):
+    g = torch.Generator(device="cuda").manual_seed(8)
+    wide = torch.randn(40, 300, generator=g, device="cuda").bfloat16()
+    x, res = wide[:, 3:131], wide[:, 150:278]
+    w = torch.randn(257, generator=g, device="cuda").bfloat16()[1:129]
+    got = packr.packr_layer_norm(x, w, residual=res)
+    assert torch.equal(got, packr.packr_layer_norm(x.contiguous(), w.clone(), residual=res.contiguous()))
+    # contiguous but starting 2 bytes after a 16-byte boundary
+    flat = torch.randn(64 * 128 + 1, generator=g, device="cuda").bfloat16()
+    odd = flat[1:].view(64, 128)
+    want = norm64(odd, None, w, None, 1e-5)
+    check("y", packr.packr_layer_norm(odd, w), want["y"], 2.4e-3)
+
+
+def test_results_do_not_depend_on_timing(cuda):
+    c = case(3000, 768, BF16, F32, seed=6)
+    a, b = run(c), run(c)
+    for k in a:
+        assert torch.equal(a[k], b[k]), k
+
+
+def test_other_stream_and_captured_graph(cuda):
+    c = case(100, 640, BF16, BF16, seed=7)
+    want = run(c)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = run(c)
+    s.synchronize()
+    for k in want:
+        assert torch.equal(got[k], want[k])
+    args = (c["x"], c["weight"], c["bias"], 1e-5, c["residual"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = packr.packr_layer_norm(*args)
+    c2 = case(100, 640, BF16, BF16, seed=17)
+    for k in ("x", "residual", "weight", "bias"):
+        c[k].copy_(c2[k])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, run(c2, need=())["y"])
+
+
+def test_gradient_against_differences(cuda):
+    """Directional derivative of sum(y * dy) by central differences of the
+    64-bit form, against the kernel's f32 gradients."""
+    c = case(7, 129, F32, F32, seed=12)
+    got = run(c)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for k in ("x", "residual", "weight", "bias"):
+        v = torch.randn(c[k].shape, generator=g, device="cuda").double()
+        h = 1e-5
+
+        def f(t):
+            d = {**{q: c[q].double() for q in ("x", "residual", "weight", "bias")}, k: c[k].double() + t * v}
+            s = d["x"] + d["residual"]
+            y = (s - s.mean(1, keepdim=True)) / torch.sqrt(s.var(1, unbiased=False, keepdim=True) + 1e-5) * d["weight"] + d["bias"]
+            return float((y * c["dy"].double()).sum())
+
+        num = (f(h) - f(-h)) / (2 * h)
+        terms = got["d" + k].double() * v
+        # f32 gradients: 2^-18 of the summed magnitudes; differences: h^2
+        assert abs(float(terms.sum()) - num) <= 2.0 ** -18 * float(terms.abs().sum()) + 1e-6 * (1 + abs(num))
+
+
+def test_module_follows_torch(cuda):
+    ref = torch.nn.LayerNorm(96, eps=1e-12).cuda()
+    with torch.no_grad():
+        ref.weight.normal_()
+        ref.bias.normal_()
+    m = packr.PackRLayerNorm.from_layer_norm(ref)
+    assert m.weight is ref.weight and m.bias is ref.bias and list(m.state_dict()) == list(ref.state_dict())
+    x, r = torch.randn(4, 5, 96, device="cuda"), torch.randn(4, 5, 96, device="cuda")
+    want = norm64(x.view(20, 96), r.view(20, 96), m.weight, m.bias, 1e-12)
+    check("y", m(x, residual=r), want["y"])
+    assert repr(m).startswith("PackRLayerNorm((96,)")

@@ -1,0 +1,245 @@
+"""packr_linear_act on the GPU against its 64-bit form: every route of the
+forward and the backward, types, activations, odd sizes."""
+import pytest
+import torch
+
+import packr_b200 as packr
+from packr_b200.synthetic import linear_case
+from fused_reference import ACTS, check, linear64
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+# bf16 results: one rounding, at most 2^-8 / sqrt(3) in the 2-norm; gradients
+# through a kept bf16 z and a bf16 operand: two more of the same size
+REL_OUT, REL_GRAD = 2.4e-3, 4.2e-3
+
+
+def case(M, K, N, xt, out, seed=0, bias=BF16, residual=True):
+    c = linear_case(M, K, N, x_dtype=xt, bias=True, seed=seed, device="cuda", fanin_scaled=True)
+    g = torch.Generator(device="cuda").manual_seed(seed + 1000)
+    c["bias"] = None if bias is None else (torch.randn(N, generator=g, device="cuda") * 0.3).to(bias)
+    c["residual"] = torch.randn(M, N, generator=g, device="cuda").to(out) if residual else None
+    c["dout"] = torch.randn(M, N, generator=g, device="cuda").to(out)
+    return c
+
+
+def call(c, act, out, **kw):
+    return packr.packr_linear_act(c["x"], c["W_p"], c["W_f"], c["lut"], c["bias"], activation=act,
+                                  residual=c["residual"], out_dtype=out, **kw)
+
+
+def grads(c, act, out, need=("x", "W_f", "bias", "lut", "residual"), **kw):
+    leaves = {k: c[k].detach().requires_grad_(True) for k in need if c[k] is not None}
+    y = call({**c, **leaves}, act, out, **kw)
+    got = torch.autograd.grad(y, list(leaves.values()), c["dout"])
+    return {"out": y, **dict(zip(("d" + k for k in leaves), got))}
+
+
+def compare(c, got, act, out):
+    want = linear64(c["x"], c["W_p"], c["W_f"], c["lut"], c["bias"], act, c["residual"], out,
+                    c["dout"] if len(got) > 1 else None, x_split=c["x"].dtype == F32)
+    for k, v in got.items():
+        if k == "dresidual":
+            assert torch.equal(v, c["dout"])
+            continue
+        rel = REL_OUT if k == "out" and out == BF16 else REL_GRAD if k in ("dx", "dW_f") else None
+        check(k, v, want[k], rel if v.numel() > 2000 else None)
+
+
+# up to 4 rows, 5..128, above; widths that TMA reads and that it does not
+SIZES = [(1, 64, 64), (1, 1000, 1001), (2, 256, 130), (4, 130, 96), (3, 33, 20), (5, 128, 64), (7, 100, 33),
+         (16, 64, 1000), (100, 768, 1001), (128, 200, 256), (129, 64, 512), (200, 1000, 520), (257, 72, 1111),
+         (300, 40, 50), (1, 1, 1), (130, 1, 3), (1030, 128, 272)]
+
+
+@pytest.mark.parametrize("xt,out", [(BF16, BF16), (BF16, F32), (F32, F32), (F32, BF16)])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_forward(cuda, M, K, N, xt, out):
+    c = case(M, K, N, xt, out, seed=M + K + N)
+    act = ACTS[(M + K + N) % len(ACTS)]
+    compare(c, {"out": call(c, act, out)}, act, out)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M", [2, 24, 150])
+def test_activations(cuda, act, M):
+    for out in (F32, BF16):
+        c = case(M, 96, 160, BF16, out, seed=M, bias=F32)
+        compare(c, grads(c, act, out), act, out)
+
+
+@pytest.mark.parametrize("xt,out", [(BF16, BF16), (BF16, F32), (F32, F32)])
+@pytest.mark.parametrize("M,K,N", [(1, 64, 64), (3, 130, 33), (100, 768, 1001), (64, 256, 320), (150, 200, 272),
+                                   (513, 100, 77), (1100, 264, 528)])
+def test_gradients(cuda, M, K, N, xt, out):
+    for i, act in enumerate(("none", "gelu", "silu")):
+        c = case(M, K, N, xt, out, seed=M + i, residual=i != 1, bias=None if i == 2 else BF16)
+        compare(c, grads(c, act, out), act, out)
+
+
+@pytest.mark.parametrize("need", [("x",), ("W_f",), ("lut",), ("bias",), ("residual",), ("x", "bias")])
+def test_only_the_gradients_asked_for(cuda, need):
+    c = case(140, 128, 144, BF16, BF16, seed=2)
+    got = grads(c, "gelu", BF16, need=need)
+    assert set(got) == {"out"} | {"d" + k for k in need}
+    compare(c, got, "gelu", BF16)
+
+
+def test_counts_given_or_counted(cuda):
+    c = case(40, 128, 144, BF16, BF16, seed=2)
+    counts = torch.bincount(c["W_p"].view(-1), minlength=256).int()
+    a = grads(c, "none", BF16, counts=counts)["dlut"]
+    b = grads(c, "none", BF16)["dlut"]
+    assert torch.allclose(a, b, rtol=1e-4, atol=1e-6)  # f32 atomics over CTAs: their order may differ
+
+
+def test_split_weight_gradient_of_f32_inputs(cuda):
+    """f32 x and f32 out: z is kept in f32 and dW takes hi + lo parts, so the
+    f32 lut gradient is good to 2^-14, not to the bf16 operand's 2^-8."""
+    c = case(200, 192, 320, F32, F32, seed=3)
+    got = grads(c, "gelu", F32)
+    want = linear64(c["x"], c["W_p"], c["W_f"], c["lut"], c["bias"], "gelu", c["residual"], F32, c["dout"], x_split=True)
+    v = want["dlut"][0]
+    assert float((got["dlut"].double() - v).norm() / v.norm()) < 2.0 ** -14
+
+
+def test_wide_range_of_preactivations(cuda):
+    """Saturated and tail values of every activation, infinities included,
+    through bias alone (x = 0)."""
+    z = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e-3, -1e-3, 0.5, -0.5, 3.0, -3.0, 5.5, -5.5, 9.0, -9.0, 13.0, -13.0,
+                      40.0, -40.0, 1e4, -1e4, 3e18, -3e18], device="cuda")
+    N = z.numel()
+    for M in (1, 20, 200):
+        x = torch.zeros(M, 8, device="cuda")
+        W_p, lut = torch.zeros(8, N, dtype=torch.uint8, device="cuda"), torch.zeros(256, device="cuda")
+        W_f = torch.zeros(8, N, dtype=BF16, device="cuda")
+        for act in ACTS:
+            y = packr.packr_linear_act(x, W_p, W_f, lut, z, activation=act)
+            want = linear64(x, W_p, W_f, lut, z, act, None, F32)["out"]
+            check(act, y, want)
+        zi = z.clone()
+        zi[0], zi[1] = float("inf"), float("nan")
+        for act in ACTS:
+            y = packr.packr_linear_act(x, W_p, W_f, lut, zi, activation=act)
+            assert y[:, 0].eq(float("inf")).all() and y[:, 1].isnan().all() and not y[:, 2:].isnan().any()
+
+
+def test_non_finite_rows_stay_in_their_rows(cuda):
+    for M in (3, 60, 200):
+        c = case(M, 64, 96, BF16, BF16, seed=M)
+        clean = call(c, "gelu", BF16)
+        c["x"][1, 5] = float("nan")
+        got = call(c, "gelu", BF16)
+        keep = [i for i in range(M) if i != 1]
+        assert got[1].isnan().all() and torch.equal(got[keep], clean[keep])
+
+
+def test_matches_the_plain_layer(cuda):
+    """Without activation and residual the f32 result is PackRLinear's on the
+    routes that decode W alike (from 5 rows on), bit for bit on the plain one."""
+    c = case(300, 256, 512, BF16, F32, seed=4, residual=False)
+    assert torch.equal(call(c, None, F32), packr.packr_matmul(c["x"], c["W_p"], c["W_f"], c["lut"], c["bias"]))
+
+
+def test_empty_batch_and_leading_dimensions(cuda):
+    c = case(0, 64, 96, BF16, BF16, seed=1)
+    got = grads(c, "gelu", BF16)
+    assert got["out"].shape == (0, 96) and got["dx"].shape == (0, 64)
+    assert not got["dW_f"].any() and not got["dbias"].any() and not got["dlut"].any()
+    c = case(24, 64, 96, BF16, BF16, seed=1)
+    flat = call(c, "silu", BF16)
+    cube = call({**c, "x": c["x"].view(2, 3, 4, 64), "residual": c["residual"].view(2, 3, 4, 96)}, "silu", BF16)
+    assert torch.equal(cube, flat.view(2, 3, 4, 96))
+    one = call({**c, "x": c["x"][0], "residual": c["residual"][0]}, "silu", BF16)
+    assert one.shape == (96,)
+
+
+def test_strided_and_misaligned_inputs(cuda):
+    c = case(150, 64, 96, BF16, BF16, seed=6)
+    want = call(c, "gelu", BF16)
+    wide = torch.zeros(150, 200, dtype=BF16, device="cuda")
+    wide[:, 3:67] = c["x"]
+    wide[:, 101:197] = c["residual"]
+    assert torch.equal(call({**c, "x": wide[:, 3:67], "residual": wide[:, 101:197]}, "gelu", BF16), want)
+    flat = torch.empty(150 * 64 + 1, dtype=BF16, device="cuda")
+    flat[1:] = c["x"].view(-1)
+    assert torch.equal(call({**c, "x": flat[1:].view(150, 64)}, "gelu", BF16), want)
+    # a residual and weights that start off a 16-byte boundary
+    flat = torch.empty(150 * 96 + 1, dtype=BF16, device="cuda")
+    flat[1:] = c["residual"].view(-1)
+    assert torch.equal(call({**c, "residual": flat[1:].view(150, 96)}, "gelu", BF16), want)
+    wf = torch.empty(64 * 96 + 1, dtype=BF16, device="cuda")
+    wf[1:] = c["W_f"].view(-1)
+    wp = torch.empty(64 * 96 + 3, dtype=torch.uint8, device="cuda")
+    wp[3:] = c["W_p"].view(-1)
+    for M in (1, 20, 150):
+        d = {**c, "x": c["x"][:M], "residual": c["residual"][:M], "dout": c["dout"][:M],
+             "W_f": wf[1:].view(64, 96), "W_p": wp[3:].view(64, 96)}
+        compare(d, grads(d, "gelu", BF16), "gelu", BF16)
+
+
+def test_upstream_gradient_of_any_layout(cuda):
+    """A broadcast (stride 0) or transposed upstream gradient."""
+    c = case(130, 64, 96, BF16, BF16, seed=6)
+    ones = {**c, "dout": torch.ones((), dtype=BF16, device="cuda").expand(130, 96)}
+    compare(ones, grads(ones, "gelu", BF16), "gelu", BF16)
+    turned = {**c, "dout": c["dout"].t().contiguous().t()}
+    compare(turned, grads(turned, "none", BF16), "none", BF16)
+
+
+def test_weight_gradient_lands_in_the_optimizer_buffer(cuda):
+    c = case(40, 64, 96, BF16, BF16, seed=2)
+    W_f = torch.nn.Parameter(c["W_f"])
+    buf = torch.zeros(64 * 96 + 256, dtype=BF16, device="cuda")
+    W_f._packr_grad_sink = (buf, 256)
+    out = call({**c, "W_f": W_f}, "gelu", BF16)
+    out.backward(c["dout"])
+    assert W_f.grad.data_ptr() == buf[256:].data_ptr()
+    assert torch.equal(W_f.grad, grads(c, "gelu", BF16, need=("W_f",))["dW_f"])
+
+
+def test_other_stream_and_captured_graph(cuda):
+    for M in (2, 40, 200):
+        c = case(M, 128, 256, BF16, BF16, seed=M)
+        want = call(c, "gelu", BF16)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got = call(c, "gelu", BF16)
+        s.synchronize()
+        assert torch.equal(got, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = call(c, "gelu", BF16)
+        c2 = case(M, 128, 256, BF16, BF16, seed=M + 50)
+        for k in ("x", "residual", "W_p", "W_f", "lut", "bias"):
+            c[k].copy_(c2[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, call(c2, "gelu", BF16))
+
+
+def test_gradient_against_differences(cuda):
+    """Directional derivatives of sum(out * dout) by central differences of the
+    64-bit form; the bf16 operands of the backward cost up to 2^-7 of the
+    summed magnitudes' norm."""
+    from fused_reference import act64, weights64
+    for act in ("gelu", "gelu_tanh", "silu", "none"):
+        c = case(33, 64, 80, F32, F32, seed=5)
+        c["x"] = c["x"].bfloat16().float()
+        got = grads(c, act, F32)
+        W = weights64(c["W_p"], c["W_f"], c["lut"])
+        base = {"x": c["x"].double(), "W_f": W, "bias": c["bias"].double(), "residual": c["residual"].double()}
+        g = torch.Generator(device="cuda").manual_seed(1)
+        for k in base:
+            v = torch.randn(base[k].shape, generator=g, device="cuda").double()
+
+            def f(t):
+                d = {**base, k: base[k] + t * v}
+                y = act64(d["x"] @ d["W_f"] + d["bias"], act) + d["residual"]
+                return float((y * c["dout"].double()).sum())
+
+            num = (f(1e-5) - f(-1e-5)) / 2e-5
+            terms = got["d" + k].double() * v
+            assert abs(float(terms.sum()) - num) <= 2.0 ** -7 * float(terms.norm()) * 4 + 1e-5 * (1 + abs(num)), (act, k)
