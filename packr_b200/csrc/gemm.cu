@@ -40,6 +40,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "activation.cuh"
 #include "sm100.cuh"
@@ -141,7 +142,9 @@ enum BSrc { B_RING = 0, B_WTMA = 1, B_PLAIN = 2 };
 // B stage feeds two pair MMAs (two 256-row subtiles), halving the decode and
 // lut traffic per FLOP; the two subtiles' accumulators then fill TMEM (no
 // double buffering across tiles, but each subtile is released separately).
-template <int MODE, int BSRC, int MSUB>
+// EPI: the forward with bias, activation and residual in its epilogue, io type
+// bf16 (1) or f32 (2); 0: the others.
+template <int MODE, int BSRC, int MSUB, int EPI = 0>
 struct Cfg {
   static constexpr bool kDecode = MODE != DW && BSRC != B_PLAIN;
   static constexpr bool kWtma = kDecode && BSRC == B_WTMA;
@@ -153,7 +156,9 @@ struct Cfg {
   static constexpr int kStageBytes = kABytes + B_BYTES + kWpBytes;
   // DW's histogram epilogue is the heavier one: two warps per TMEM lane
   // quarter, each taking half of the tile's columns.
-  static constexpr int kEpiWarps = kDecode ? 4 : 8;
+  // The fused epilogue is latency-bound (staging, residual loads, special
+  // functions): four warps per quarter, two 32-column chunks each.
+  static constexpr int kEpiWarps = kDecode ? 4 : (EPI ? 16 : 8);
   // The TMA-fed modes and DW pass each 32-row output block through a 4 KB
   // per-warp shared-memory buffer, so that global stores cover whole rows
   // segments of 128 (f32) or 64 (bf16) bytes instead of 16 bytes per row
@@ -164,7 +169,7 @@ struct Cfg {
   // GEMMs only (for DW the split-tile fix-up measured slower than the wave
   // quantisation it removes)
   static constexpr bool kStreamK = kPlainB;
-  static constexpr int kStgBytes = kStageOut ? kEpiWarps * 4096 : 0;
+  static constexpr int kStgBytes = kStageOut ? kEpiWarps * (EPI ? 2048 : 4096) : 0;
   static constexpr int kChunksPerEpiWarp = (BN / 32) / (kEpiWarps / 4);
   static constexpr int kDecWarp0 = 2 + kEpiWarps;             // first decode warp
   static constexpr int kDecWarps = kWtma ? DEC_WARPS_TMA : DEC_WARPS;
@@ -233,7 +238,7 @@ struct Params {
 
 // Workspace for stream-K: partial slots and flags for up to `pairs` CTA pairs.
 inline size_t sk_partial_bytes(int pairs, int msub) { return (size_t)pairs * msub * 2 * BN * BM * sizeof(float); }
-inline size_t sk_flag_bytes(int pairs) { return (size_t)pairs * 2 * 8 * sizeof(int); }
+inline size_t sk_flag_bytes(int pairs, int epi_warps = 8) { return (size_t)pairs * 2 * epi_warps * sizeof(int); }
 
 // One unit of a pair's work: k-blocks [k0, k1) of one tile.
 struct Unit {
@@ -320,6 +325,7 @@ struct Bars {
   uint64_t qfull[TILE_Q];   // tile number published                 (count 1)
   uint64_t qempty[TILE_Q];  // read by every consumer of both CTAs    (count kQConsumers)
   int qtile[TILE_Q];        // tile number, or -1 after the last tile
+  int qk0[TILE_Q], qk1[TILE_Q], qkind[TILE_Q];  // fused epilogue: the rest of the unit
   uint32_t tmem_base;
   int abort;
 };
@@ -541,140 +547,127 @@ __device__ __forceinline__ void store_rows_staged(uint32_t stg, const float* v, 
   __syncwarp();
 }
 
-// As store_rows_staged, for rows or bases without 16-byte alignment and for
-// the last columns: the 32 x 32 block is staged in the warp's buffer and each
-// store instruction writes one row's nval consecutive elements.
-template <int ESIZE>
-__device__ __forceinline__ void store_rows_any(uint32_t stg, const float* v, void* out, int r0, int m_limit,
-                                               long long ld, int gn0, int nval) {
-  constexpr int CPR = 32 * ESIZE / 16;
-  const int lane = threadIdx.x & 31;
-  // 4-byte words of row r, word w at ((w + r) & (words - 1)): conflict-free both ways
-  constexpr int WPR = 32 * ESIZE / 4;
-#pragma unroll
-  for (int j = 0; j < 4 * CPR; ++j)
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(stg + (uint32_t)(lane * 32 * ESIZE + ((j + lane) & (WPR - 1)) * 4)),
-                 "r"(__float_as_uint(v[j]))
-                 : "memory");
-  __syncwarp();
-#pragma unroll 8
-  for (int r = 0; r < 32; ++r) {
-    const int w = ESIZE == 4 ? lane : lane >> 1;
-    uint32_t d;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(d) : "r"(stg + (uint32_t)(r * 32 * ESIZE + ((w + r) & (WPR - 1)) * 4)) : "memory");
-    const long long gr = (long long)r0 + r;
-    if (gr < m_limit && lane < nval) {
-      if (ESIZE == 4)
-        __stcs(static_cast<uint32_t*>(out) + gr * ld + gn0 + lane, d);
-      else
-        __stcs(static_cast<unsigned short*>(out) + gr * ld + gn0 + lane, (unsigned short)(d >> (16 * (lane & 1))));
-    }
-  }
-  __syncwarp();
-}
+// The fused epilogue of one warp's 32 x 16 block.  The accumulator (lane l:
+// row l) goes through the warp's 2 KB staging buffer and comes back with 4 consecutive columns per lane, 8 rows per
+// step, so that the lane's bias stays in registers over the rows and the
+// residual, z and out are touched in whole 32- or 64-byte row segments.  Lanes
+// of a block without 16-byte rows, or of the last columns, own one column each
+// instead.
+template <bool F32>
+struct EpiBlock {
+  typedef typename std::conditional<F32, float4, uint2>::type Quad;  // 4 elements of the io type
 
-// The fused epilogue of one warp's 32 x 32 block: f holds the f32 accumulator
-// of row r0 + lane, columns gn0 .. gn0 + 31 (nval of them inside the output).
-__device__ __forceinline__ void epilogue_block(const Params& P, uint32_t stg, float* f, int r0, int gn0, int nval) {
-  const Epilogue& E = P.epi;
-  const int lane = threadIdx.x & 31;
-  const long long row = (long long)r0 + lane;
-  const bool row_ok = row < P.Mg;
-  const bool full = nval == 32 && E.vec;
-  if (P.bias != nullptr) {
-    if (nval == 32 && aligned(P.bias, 16)) {  // the same 32 values in every lane
-      if (P.bias_f32) {
-        const float4* bp = reinterpret_cast<const float4*>(static_cast<const float*>(P.bias) + gn0);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float4 b = __ldg(bp + j);
-          f[4 * j] = __fadd_rn(f[4 * j], b.x);
-          f[4 * j + 1] = __fadd_rn(f[4 * j + 1], b.y);
-          f[4 * j + 2] = __fadd_rn(f[4 * j + 2], b.z);
-          f[4 * j + 3] = __fadd_rn(f[4 * j + 3], b.w);
-        }
-      } else {
-        const uint4* bp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.bias) + gn0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 b = __ldg(bp + j);
-          const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f[8 * j + 2 * i] = __fadd_rn(f[8 * j + 2 * i], __uint_as_float(w[i] << 16));
-            f[8 * j + 2 * i + 1] = __fadd_rn(f[8 * j + 2 * i + 1], __uint_as_float(w[i] & 0xFFFF0000u));
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < nval) f[j] = __fadd_rn(f[j], load_io(P.bias, gn0 + j, P.bias_f32));
-    }
+  static __device__ __forceinline__ void unpack(const float4& v, float* f) {
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
   }
-  auto put = [&](void* dst) {
-    if (E.io_f32) {
-      if (full) store_rows_staged<4>(stg, f, dst, r0, P.Mg, P.ld_out, gn0);
-      else store_rows_any<4>(stg, f, dst, r0, P.Mg, P.ld_out, gn0, nval);
-    } else {
-      float h[16];
+  static __device__ __forceinline__ void unpack(const uint2& v, float* f) {
+    f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+    f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xFFFF0000u);
+  }
+  static __device__ __forceinline__ void pack(const float* f, float4& v) { v = make_float4(f[0], f[1], f[2], f[3]); }
+  static __device__ __forceinline__ void pack(const float* f, uint2& v) {
+    v = make_uint2(pack_bf16x2_rne(f[0], f[1]), pack_bf16x2_rne(f[2], f[3]));
+  }
+
+  // 16 columns: v holds the half's accumulator of row r0 + lane, gn0 its first
+  // column, nval (<= 16) of which lie inside the output.
+  static __device__ __forceinline__ void half(const Params& P, uint32_t stg, const uint32_t* v, int r0, int gn0,
+                                              int nval) {
+    const int lane = threadIdx.x & 31;
+    const Epilogue& E = P.epi;
+    const bool quads = nval == 16 && E.vec;
+    const int col = gn0 + (lane & 3) * 4;
+    const int row = r0 + (lane >> 2);                                 // and + 8, + 16, + 24
+    const long long q0 = ((long long)row * P.ld_out + col) / 4;       // in quads
+    const long long qs = 2 * P.ld_out;                                // 8 rows
+    Quad res[4];
+    if (quads && E.residual != nullptr) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) h[j] = __uint_as_float(pack_bf16x2_rne(f[2 * j], f[2 * j + 1]));
-      if (full) store_rows_staged<2>(stg, h, dst, r0, P.Mg, P.ld_out, gn0);
-      else store_rows_any<2>(stg, h, dst, r0, P.Mg, P.ld_out, gn0, nval);
+      for (int i = 0; i < 4; ++i)
+        if (row + 8 * i < P.Mg) res[i] = __ldg(reinterpret_cast<const Quad*>(E.residual) + q0 + i * qs);
     }
-  };
-  if (E.z != nullptr) put(E.z);
-  act::apply_all<32>(E.act, f);
-  if (E.residual != nullptr) {
-    if (full) {
-      if (row_ok) {
-        if (E.io_f32) {
-          const float4* rp = reinterpret_cast<const float4*>(static_cast<const float*>(E.residual) + row * P.ld_out + gn0);
+    const int sw = (lane >> 1) & 3;  // 16-byte chunks of a row XOR-swizzled by row
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 r = __ldcs(rp + j);
-            f[4 * j] = __fadd_rn(f[4 * j], r.x);
-            f[4 * j + 1] = __fadd_rn(f[4 * j + 1], r.y);
-            f[4 * j + 2] = __fadd_rn(f[4 * j + 2], r.z);
-            f[4 * j + 3] = __fadd_rn(f[4 * j + 3], r.w);
-          }
-        } else {
-          const uint4* rp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(E.residual) + row * P.ld_out + gn0);
+    for (int j = 0; j < 4; ++j)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stg + (uint32_t)(lane * 64 + ((j ^ sw) << 4))),
+                   "r"(v[4 * j]), "r"(v[4 * j + 1]), "r"(v[4 * j + 2]), "r"(v[4 * j + 3])
+                   : "memory");
+    __syncwarp();
+    if (quads) {
+      float b[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint4 r = __ldcs(rp + j);
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+      for (int j = 0; j < 4; ++j) b[j] = P.bias != nullptr ? load_io(P.bias, col + j, P.bias_f32) : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              f[8 * j + 2 * i] = __fadd_rn(f[8 * j + 2 * i], __uint_as_float(w[i] << 16));
-              f[8 * j + 2 * i + 1] = __fadd_rn(f[8 * j + 2 * i + 1], __uint_as_float(w[i] & 0xFFFF0000u));
+      for (int i = 0; i < 4; i += 2) {
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int r = (i + k) * 8 + (lane >> 2);
+          float4 a;
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(a.x), "=f"(a.y), "=f"(a.z), "=f"(a.w)
+                       : "r"(stg + (uint32_t)(r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4)))
+                       : "memory");
+          f[4 * k] = __fadd_rn(a.x, b[0]);
+          f[4 * k + 1] = __fadd_rn(a.y, b[1]);
+          f[4 * k + 2] = __fadd_rn(a.z, b[2]);
+          f[4 * k + 3] = __fadd_rn(a.w, b[3]);
+        }
+        auto put = [&](void* dst) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (row + 8 * (i + k) < P.Mg) {
+              Quad o;
+              pack(f + 4 * k, o);
+              __stcs(reinterpret_cast<Quad*>(dst) + q0 + (i + k) * qs, o);
             }
           }
+        };
+        if (E.z != nullptr) put(E.z);
+        act::apply_all<8>(E.act, f);
+        if (E.residual != nullptr) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float r[4];
+            unpack(res[i + k], r);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[4 * k + j] = __fadd_rn(f[4 * k + j], r[j]);
+          }
         }
+        put(E.out);
       }
     } else {
-      // row by row into the staging buffer as f32 (skewed words), then each lane its own row
-#pragma unroll 8
-      for (int r = 0; r < 32; ++r) {
-        const long long gr = (long long)r0 + r;
-        const float v = gr < P.Mg && lane < nval ? load_io(E.residual, gr * P.ld_out + gn0 + lane, E.io_f32) : 0.0f;
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(stg + (uint32_t)(r * 128 + ((lane + r) & 31) * 4)),
-                     "r"(__float_as_uint(v))
-                     : "memory");
-      }
-      __syncwarp();
+      const int w = lane & 15;
+      const bool col_in = w < nval;
+      const float b = P.bias != nullptr && col_in ? load_io(P.bias, gn0 + w, P.bias_f32) : 0.0f;
+#pragma unroll 1
+      for (int i = 0; i < 16; i += 4) {
+        float f[4], r4[4];
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        uint32_t d;
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(d) : "r"(stg + (uint32_t)(lane * 128 + ((j + lane) & 31) * 4)) : "memory");
-        f[j] = __fadd_rn(f[j], __uint_as_float(d));
+        for (int k = 0; k < 4; ++k) {
+          const int r = (i + k) * 2 + (lane >> 4);
+          const long long o = (long long)(r0 + r) * P.ld_out + gn0 + w;
+          const bool in = col_in && r0 + r < P.Mg;
+          r4[k] = E.residual != nullptr && in ? load_io(E.residual, o, F32) : 0.0f;
+          asm volatile("ld.shared.f32 %0, [%1];"
+                       : "=f"(f[k])
+                       : "r"(stg + (uint32_t)(r * 64 + (((w >> 2) ^ ((r >> 1) & 3)) << 4) + (w & 3) * 4))
+                       : "memory");
+          f[k] = __fadd_rn(f[k], b);
+          if (E.z != nullptr && in) store_io(E.z, o, F32, f[k]);
+        }
+        act::apply_all<4>(E.act, f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = (i + k) * 2 + (lane >> 4);
+          if (col_in && r0 + r < P.Mg)
+            store_io(E.out, (long long)(r0 + r) * P.ld_out + gn0 + w, F32, __fadd_rn(f[k], r4[k]));
+        }
       }
-      __syncwarp();
     }
+    __syncwarp();  // the buffer is free for the next half
   }
-  put(E.out);
-}
+};
 
 // Bounded wait for a stream-K flag written by another CTA pair of the same
 // launch (all pairs are resident at once).  Lane 0 polls with acquire loads
@@ -709,13 +702,12 @@ __device__ __forceinline__ bool wait_flag(const int* f, volatile int* abort_flag
 }
 
 // ------------------------------------------------------------------ kernel
-// EPI: the forward with bias, activation and residual in its epilogue
-// (Params::epi).
-template <int MODE, int BSRC, int MSUB, bool EPI = false>
-__global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB>::kThreads, 1)
+template <int MODE, int BSRC, int MSUB, int EPI = 0>
+__global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
     packr_gemm_kernel(const Params P, const __grid_constant__ Maps maps) {
-  using C = Cfg<MODE, BSRC, MSUB>;
-  static_assert(!EPI || (MODE == FWD && C::kPlainB), "the fused epilogue belongs to the plain forward");
+  using C = Cfg<MODE, BSRC, MSUB, EPI>;
+  static_assert(EPI == 0 || (MODE == FWD && C::kPlainB), "the fused epilogue belongs to the plain forward");
+  static_assert(EPI == 0 || C::kEpiWarps == 16, "four warps per TMEM quarter, 64 columns each");
   constexpr int STAGES = C::kStages;
   static_assert(C::kSmemBytes <= 227 * 1024, "shared memory per CTA");
   static_assert(MODE != DW || MSUB == 1, "the DW epilogue's histogram runs per 256-row tile");
@@ -814,6 +806,45 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB>::kThreads, 1)
     mbar_arrive_release_cluster(mapa(smem_u32(&bars->qempty[slot]), 0));
     return true;
   };
+  // Kernels with the fused epilogue pass every unit through the queue, static
+  // schedules too: the even CTA's producer alone walks the schedule, so that
+  // the epilogue warps, which hold accumulators in registers, carry none of its
+  // state.  False past the last unit or on an abort.
+  auto unit_push = [&](int i, Sched& sc, Unit& x) -> bool {
+    const int slot = i % TILE_Q;
+    const uint32_t ph = (uint32_t)(i / TILE_Q) & 1u;
+    if (!mbar_wait_cluster(&bars->qempty[slot], ph ^ 1u, abort_flag)) return false;
+    bool more;
+    if (dyn) {
+      x = Unit{atomicAdd(P.tile_counter, 1), 0, kb_total, 0};
+      more = x.tile < num_tiles;
+    } else {
+      more = next_unit(sc, x);
+    }
+    if (!more) x.tile = -1;
+    bars->qtile[slot] = x.tile;
+    bars->qk0[slot] = x.k0;
+    bars->qk1[slot] = x.k1;
+    bars->qkind[slot] = x.kind;
+    st_shared_cluster_u32(mapa(smem_u32(&bars->qtile[slot]), 1), (uint32_t)x.tile);
+    st_shared_cluster_u32(mapa(smem_u32(&bars->qk0[slot]), 1), (uint32_t)x.k0);
+    st_shared_cluster_u32(mapa(smem_u32(&bars->qk1[slot]), 1), (uint32_t)x.k1);
+    st_shared_cluster_u32(mapa(smem_u32(&bars->qkind[slot]), 1), (uint32_t)x.kind);
+    mbar_arrive_release_cluster(mapa(smem_u32(&bars->qfull[slot]), 0));
+    mbar_arrive_release_cluster(mapa(smem_u32(&bars->qfull[slot]), 1));
+    return more;
+  };
+  auto unit_pop = [&](int i, Unit& x) -> bool {
+    const int slot = i % TILE_Q;
+    const uint32_t ph = (uint32_t)(i / TILE_Q) & 1u;
+    if (!mbar_wait_cluster(&bars->qfull[slot], ph, abort_flag)) return false;
+    x.tile = *reinterpret_cast<volatile int*>(&bars->qtile[slot]);
+    x.k0 = *reinterpret_cast<volatile int*>(&bars->qk0[slot]);
+    x.k1 = *reinterpret_cast<volatile int*>(&bars->qk1[slot]);
+    x.kind = *reinterpret_cast<volatile int*>(&bars->qkind[slot]);
+    mbar_arrive_release_cluster(mapa(smem_u32(&bars->qempty[slot]), 0));
+    return x.tile >= 0;
+  };
   auto whole_tile = [&](int t, Unit& x) {
     x.tile = t;
     x.k0 = 0;
@@ -829,7 +860,9 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB>::kThreads, 1)
       Sched sc = make_sched(P, pair, npairs);
       Unit u;
       for (int qi = 0; ok; ++qi) {
-        if (dyn) {
+        if (EPI != 0) {
+          if (!(rank == 0 ? unit_push(qi, sc, u) : unit_pop(qi, u))) break;
+        } else if (dyn) {
           int t = -1;
           if (rank == 0) {
             t = q_push(qi);
@@ -904,7 +937,9 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB>::kThreads, 1)
       Sched sc = make_sched(P, pair, npairs);
       Unit u;
       for (; ok; ++t_local) {
-        if (dyn) {
+        if (EPI != 0) {
+          if (!unit_pop(t_local, u)) break;
+        } else if (dyn) {
           int t = -1;
           if (!q_pop(t_local, t) || t < 0) break;
           whole_tile(t, u);
@@ -956,6 +991,92 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB>::kThreads, 1)
         }
       }
       umma_commit_pair(&bars->drain, PAIR_MASK);
+    }
+  } else if (EPI != 0 && warp < C::kDecWarp0) {
+    // ------------------------------------------------ fused epilogue (both CTAs)
+    // Each warp takes its two 32-column chunks of a 128-row subtile into
+    // registers and hands the accumulator back before any of the epilogue's
+    // arithmetic, so that the next tile's MMAs wait for a TMEM read only, also
+    // with MSUB = 2, whose two accumulators fill TMEM.
+    if constexpr (EPI != 0) {
+      const int q = warp & 3, ew = warp - 2;
+      const int row = q * 32 + lane;
+      const uint32_t stg = smem_u32(sAux) + (uint32_t)(C::kStgOff + ew * 2048);
+      const uint32_t tempty0 = mapa(smem_u32(&bars->tempty[0]), 0);
+      const uint32_t tempty1 = mapa(smem_u32(&bars->tempty[1]), 0);
+      bool alive = true;
+      for (int t_local = 0; alive; ++t_local) {
+        // lane 0 reads the queue, every lane gets the same answer
+        Unit u{-1, 0, 0, 0};
+        if (lane == 0 && !unit_pop(t_local, u)) u.tile = -1;
+        u.tile = __shfl_sync(0xFFFFFFFFu, u.tile, 0);
+        u.kind = __shfl_sync(0xFFFFFFFFu, u.kind, 0);
+        if (u.tile < 0) break;
+        const int n0 = (u.tile / P.m_tiles) * BN + (ew >> 2) * 64;
+        int n_heads = 0;
+#pragma unroll 1
+        for (int sub = 0; sub < MSUB; ++sub) {
+          const int acc = MSUB == 1 ? (t_local & 1) : sub;
+          const uint32_t aph = MSUB == 1 ? ((uint32_t)(t_local >> 1) & 1u) : ((uint32_t)t_local & 1u);
+          // this warp's 32 rows of the subtile
+          const int r0 = (u.tile % P.m_tiles) * (2 * BM * MSUB) + sub * 2 * BM + (int)rank * BM + q * 32;
+          if (P.epi.residual != nullptr && r0 + lane < P.Mg && n0 < P.Ng)  // towards L2 while the MMAs run
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(P.epi.residual) +
+                                                          ((long long)(r0 + lane) * P.ld_out + n0) * (EPI == 2 ? 4 : 2)));
+          if (!mbar_wait_warp(&bars->tfull[acc], aph, abort_flag, kEpilogueSleepNs)) {
+            alive = false;
+            break;
+          }
+          if (u.kind == 2 && sub == 0) {  // stream-K tail: wait for every following pair's head partial
+            const long long tile_end = (long long)(u.tile + 1) * kb_total;
+            for (int q2 = pair + 1; alive && q2 < npairs && sk_start(P, q2, npairs) < tile_end; ++q2) {
+              alive = wait_flag(P.sk_flags + (q2 * 2 + (int)rank) * C::kEpiWarps + ew, abort_flag);
+              ++n_heads;
+            }
+            if (!alive) break;
+          }
+          tc_fence_after();
+          uint32_t v[64];
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            tmem_ld_32x32b_x32(tmem_base + (uint32_t)(acc * ACC_COLS + (ew >> 2) * 64 + c * 32) + ((uint32_t)(q * 32) << 16),
+                               *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(acc ? tempty1 : tempty0);
+          // stream-K partials [col][row], coalesced along rows
+          const long long slot0 = (((long long)pair * MSUB + sub) * 2 + rank) * (BN * BM) + (ew >> 2) * 64 * BM + row;
+          if (u.kind == 1) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) __stcg(P.sk_partial + slot0 + j * BM, __uint_as_float(v[j]));
+            continue;
+          }
+          for (int h = 1; h <= n_heads; ++h) {  // the heads' partials, added in pair order
+            const float* const slot = P.sk_partial + slot0 + (long long)h * (MSUB * 2 * BN * BM);
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] = __float_as_uint(__fadd_rn(__uint_as_float(v[j]), __ldcg(slot + j * BM)));
+          }
+          // four blocks of 16 columns; a rolled loop (the registers shift down
+          // by a block) keeps the epilogue's code small and its values few
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const int gn0 = n0 + c * 16;
+            const int nval = min(16, P.Ng - gn0);
+            if (nval > 0 && r0 < P.Mg) EpiBlock<EPI == 2>::half(P, stg, v, r0, gn0, nval);
+#pragma unroll
+            for (int j = 0; j < 48; ++j) v[j] = v[j + 16];
+          }
+        }
+        if (alive && u.kind == 1) {  // publish this warp's part of the head partial
+          __threadfence();
+          __syncwarp();
+          if (lane == 0) {
+            int* f = P.sk_flags + (pair * 2 + (int)rank) * C::kEpiWarps + ew;
+            asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(f), "r"(1) : "memory");
+          }
+        }
+      }
     }
   } else if (warp < C::kDecWarp0) {
     // ------------------------------------------------ epilogue (both CTAs)
@@ -1063,45 +1184,6 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB>::kThreads, 1)
           ++n_heads;
         }
         if (!alive) break;
-      }
-      if constexpr (EPI) {
-        // The whole subtile is taken into registers (4 x 32 columns per
-        // warp) and its accumulator handed back before any of the
-        // epilogue's arithmetic: with MSUB = 2 both accumulators are in use,
-        // and the next tile's first MMAs would otherwise wait for the
-        // activation, the residual loads and the stores.
-        uint32_t v[C::kChunksPerEpiWarp][32];
-#pragma unroll
-        for (int c = 0; c < C::kChunksPerEpiWarp; ++c)
-          tmem_ld_32x32b_x32(tmem_base + (uint32_t)(acc * ACC_COLS + (cc0 + c) * 32) + ((uint32_t)(q * 32) << 16), v[c]);
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(acc ? tempty1 : tempty0);
-#pragma unroll
-        for (int c = 0; c < C::kChunksPerEpiWarp; ++c) {
-          const int cc = cc0 + c;
-          const int gn0 = n0 + cc * 32;
-          if (gn0 >= P.Ng || m0 + q * 32 >= P.Mg) continue;  // warp-uniform
-          if (u.kind == 1) {  // stream-K head: raw partial
-#pragma unroll
-            for (int j = 0; j < 32; ++j) __stcg(my_slot + (cc * 32 + j) * BM + row, __uint_as_float(v[c][j]));
-            continue;
-          }
-          float f[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[c][j]);
-          if (u.kind == 2) {  // the heads' partials, added in pair order
-            for (int h = 1; h <= n_heads; ++h) {
-              const float* const slot =
-                  P.sk_partial + (((size_t)(pair + h) * MSUB + sub) * 2 + rank) * (size_t)(BN * BM);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) f[j] = __fadd_rn(f[j], __ldcg(slot + (cc * 32 + j) * BM + row));
-            }
-          }
-          epilogue_block(P, stg, f, m0 + q * 32, gn0, min(32, P.Ng - gn0));
-        }
-        continue;
       }
 #pragma unroll
       for (int c = 0; c < C::kChunksPerEpiWarp; ++c) {
@@ -1456,9 +1538,9 @@ int make_map_u8(CUtensorMap* m, const void* base, long long inner, long long row
   return r == CUDA_SUCCESS ? PACKR_OK : PACKR_ERR_INVALID_ARGUMENT;
 }
 
-template <int MODE, int BSRC, int MSUB = 1, bool EPI = false>
+template <int MODE, int BSRC, int MSUB = 1, int EPI = 0>
 int launch_impl(Params P, const Maps& maps, cudaStream_t stream) {
-  using C = Cfg<MODE, BSRC, MSUB>;
+  using C = Cfg<MODE, BSRC, MSUB, EPI>;
   static std::once_flag attr_once[64];
   static int resident_pairs[64];
   int dev = 0;
@@ -1579,15 +1661,34 @@ int launch(Params P, Maps maps, cudaStream_t stream) {
 
 // FWD / DX over a predecoded bf16 W (maps.b[0] set by the caller: FWD an
 // [K, N] map with 64-row boxes, DX an [K, N] map with 128-row boxes).
-template <int MODE, bool EPI = false>
+template <int MODE>
 int launch_plain(Params P, const Maps& maps, cudaStream_t stream) {
   static_assert(MODE != DW, "DW has its own operands");
   P.out_vec = aligned(P.out, 16);
   P.idx_vec = 0;
   P.n_tiles = (P.Ng + BN - 1) / BN;
   P.k_blocks = (P.Kg + BK - 1) / BK;
-  if (P.Mg >= PACKR_PLAIN_MSUB2_MIN_M) return launch_impl<MODE, B_PLAIN, 2, EPI>(P, maps, stream);
-  return launch_impl<MODE, B_PLAIN, 1, EPI>(P, maps, stream);
+  if (P.Mg >= PACKR_PLAIN_MSUB2_MIN_M) return launch_impl<MODE, B_PLAIN, 2>(P, maps, stream);
+  return launch_impl<MODE, B_PLAIN, 1>(P, maps, stream);
+}
+
+// Subtiles of the fused forward's tiles.
+#ifndef PACKR_EPI_MSUB2_MIN_K
+#define PACKR_EPI_MSUB2_MIN_K 2048
+#endif
+inline int epi_msub(long long M, long long K) {
+  return M >= PACKR_PLAIN_MSUB2_MIN_M && K >= PACKR_EPI_MSUB2_MIN_K ? 2 : 1;
+}
+
+// The plain forward with the fused epilogue P.epi.
+int launch_plain_epi(Params P, const Maps& maps, cudaStream_t stream) {
+  P.n_tiles = (P.Ng + BN - 1) / BN;
+  P.k_blocks = (P.Kg + BK - 1) / BK;
+  if (epi_msub(P.Mg, P.Kg) == 2)
+    return P.epi.io_f32 ? launch_impl<FWD, B_PLAIN, 2, 2>(P, maps, stream)
+                        : launch_impl<FWD, B_PLAIN, 2, 1>(P, maps, stream);
+  return P.epi.io_f32 ? launch_impl<FWD, B_PLAIN, 1, 2>(P, maps, stream)
+                      : launch_impl<FWD, B_PLAIN, 1, 1>(P, maps, stream);
 }
 
 }  // namespace gemm

@@ -204,8 +204,8 @@ size_t plan_forward(Carve& c, Fwd& p, Route r, long long M, long long K, long lo
     p.part = c.take<float>(gemm::skinny_partial_bytes(M, K, N) / sizeof(float));
   } else {
     p.wd = c.take<uint16_t>((size_t)K * round8(N));
-    p.skp = c.take<float>(gemm::sk_partial_bytes(linear::sk_pairs(), linear::plain_msub(M)) / sizeof(float));
-    p.skf = c.take<int>(gemm::sk_flag_bytes(linear::sk_pairs()) / sizeof(int));
+    p.skp = c.take<float>(gemm::sk_partial_bytes(linear::sk_pairs(), gemm::epi_msub(M, K)) / sizeof(float));
+    p.skf = c.take<int>(gemm::sk_flag_bytes(linear::sk_pairs(), 16) / sizeof(int));
   }
   return c.off;
 }
@@ -331,7 +331,7 @@ extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_
   P.sk_partial = p.skp;
   P.sk_flags = p.skf;
   P.sk_slots = linear::sk_pairs();
-  return gemm::launch_plain<gemm::FWD, true>(P, maps, s);
+  return gemm::launch_plain_epi(P, maps, s);
 }
 
 extern "C" size_t packr_linear_act_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, int flags,
