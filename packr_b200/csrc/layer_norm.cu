@@ -8,18 +8,29 @@
 // x, residual, y, dy, dx share one type (bf16 or f32), weight, bias and their
 // gradients another; sums and statistics are f32.
 //
-// Bound by HBM: one read of each input and one write of each output.  A row
-// lives in the registers of `blockDim.x` threads, E elements each, so mean and
-// centred variance are two exact passes over registers; `blockDim.y` rows are
-// in flight per CTA and the next row's loads are issued before the current
-// row's reductions.  The backward recomputes h from x and residual instead of
-// a stored sum: the sum would have to be rounded (bf16) or read back at twice
-// the width, for the same number of bytes.  Its CTAs are persistent: a thread
-// owns the same E columns in every row it visits and carries their dweight /
-// dbias sums in registers (E = 16: in its own shared-memory words); the CTAs'
-// sums go to the workspace and a second launch adds them in a fixed order, so
-// results do not depend on timing.  Rows wider than the register path are
-// walked in strides of the CTA, three passes over L2-resident data.
+// Bound by HBM: one read of each input and one write of each output.
+// * A row lives in the registers of `blockDim.x` threads, E elements each, so
+//   mean and centred variance are two exact passes over registers;
+//   `blockDim.y` rows are in flight per CTA, and CTAs are persistent.
+// * Loads: each thread copies its own 16-byte chunks of the following rows into
+//   its own shared-memory slots with cp.async, `stages` deep (no barrier: a
+//   thread reads only what it copied).  Registers alone held 32 KB in flight
+//   per SM at 4096 columns, 70 % of HBM's rate.
+// * Rows of any length use the same 16-byte chunks: chunks are laid on the
+//   16-byte grid of the tensor, so a row may begin and end inside one (its
+//   phase).  The rows of a CTA are a multiple of 8 (f32: 4) apart, which gives
+//   them one phase, so a thread's columns, weights and column sums stay its
+//   own over the whole launch; elements of neighbouring rows in the two edge
+//   chunks are loaded and dropped, and never read past the tensor's end.
+// * The backward recomputes h from x and residual instead of a stored sum: the
+//   sum would have to be rounded (bf16) or read back at twice the width, for
+//   the same number of bytes.  A thread carries its columns' dweight / dbias
+//   sums in registers (rows beyond 8192 columns: in its own shared-memory
+//   words); the CTAs' sums go to the workspace and a second launch adds them in
+//   a fixed order, so results do not depend on timing.
+// Rows wider than 16384, and tensors that do not start on a 16-byte boundary,
+// are walked by one CTA per row in passes over L2-resident data.
+#include "activation.cuh"
 #include "common.cuh"
 
 namespace packr {
@@ -28,6 +39,7 @@ namespace norm {
 constexpr int kMaxRowThreads = 1024;
 constexpr long long kMaxRegN = 16LL * kMaxRowThreads;  // widest row held in registers
 constexpr int kMaxGroups = 8;                          // rows in flight per CTA (named barriers 1..8)
+constexpr int kMaxSmem = 220 * 1024;                   // dynamic shared memory a CTA may ask for
 
 template <class T>
 struct Elem;
@@ -42,100 +54,217 @@ struct Elem<uint16_t> {  // bf16 bit pattern
   static __device__ __forceinline__ uint16_t put(float v) { return (uint16_t)(pack_bf16x2_rne(v, 0.0f) & 0xFFFFu); }
 };
 
-// One thread's E elements of a row.  VEC: vectors of VW = 16 / sizeof(x type)
-// elements, vector v of thread t covering columns (v * nt + t) * VW ..; else
-// element e is column e * nt + t (any N, any alignment; still coalesced).
-template <class T, int E>
-struct Raw {
-  static constexpr int kWords = E * (int)sizeof(T) / 4;
-  uint32_t w[kWords];
-  __device__ __forceinline__ float at(int e) const {
-    if (sizeof(T) == 4) return __uint_as_float(w[e]);
-    return __uint_as_float((e & 1) ? (w[e >> 1] & 0xFFFF0000u) : (w[e >> 1] << 16));
-  }
-  __device__ __forceinline__ void set_scalar(int e, T v) {
-    if (sizeof(T) == 4) {
-      w[e] = __float_as_uint(Elem<T>::get(v));
-    } else if (e & 1) {
-      w[e >> 1] |= __float_as_uint(Elem<T>::get(v));
-    } else {
-      w[e >> 1] = __float_as_uint(Elem<T>::get(v)) >> 16;
-    }
-  }
-};
+// Pairs of f32 (first element in the low half) for the packed add, multiply and
+// fma: the kernels are within 2x of the issue rate when each element takes an
+// instruction of its own.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pk2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void upk2(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 sub2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2 splat(float a) { return pk2(a, a); }
+__device__ __forceinline__ float both(f32x2 v) {
+  float a, b;
+  upk2(v, a, b);
+  return a + b;
+}
 
-// Columns of a thread's elements when the x type has XB bytes.
-template <int XB, int E, bool VEC>
-struct Cols {
-  static constexpr int VW = 16 / XB;
-  static __device__ __forceinline__ int col(int e, int t, int nt) {
-    return VEC ? ((e / VW) * nt + t) * VW + e % VW : e * nt + t;
-  }
-  static __device__ __forceinline__ bool valid(int e, int t, int nt, int N) { return col(e, t, nt) < N; }
-};
+// A 16-byte chunk as pairs.
+__device__ __forceinline__ void unpack(const uint4 q, f32x2* v, float) {
+  v[0] = pk2(__uint_as_float(q.x), __uint_as_float(q.y));
+  v[1] = pk2(__uint_as_float(q.z), __uint_as_float(q.w));
+}
+__device__ __forceinline__ void unpack(const uint4 q, f32x2* v, uint16_t) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = pk2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint4 pack(const f32x2* v, float) {
+  uint4 q;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(q.x), "=r"(q.y) : "l"(v[0]));
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(q.z), "=r"(q.w) : "l"(v[1]));
+  return q;
+}
+__device__ __forceinline__ uint32_t pack_pair(f32x2 v) {
+  float a, b;
+  upk2(v, a, b);
+  return pack_bf16x2_rne(a, b);
+}
+__device__ __forceinline__ uint4 pack(const f32x2* v, uint16_t) {
+  return make_uint4(pack_pair(v[0]), pack_pair(v[1]), pack_pair(v[2]), pack_pair(v[3]));
+}
 
-// Loads the thread's E elements of row p (P: element type, XB: bytes of the x
-// type, which sets the column layout).  Elements past N read as zero.
-template <class P, int XB, int E, bool VEC, bool STREAM>
-__device__ __forceinline__ void load_row(Raw<P, E>& r, const P* __restrict__ p, int t, int nt, int N) {
-  using C = Cols<XB, E, VEC>;
+// Which elements a thread holds: chunk v of thread t covers VW = 16 /
+// sizeof(T) columns from (v * nt + t) * VW - phase.  Rows of whole chunks
+// (RAGGED false) have phase 0 and chunks that are inside or outside as a whole.
+template <class T, int E, bool RAGGED>
+struct Layout {
+  static constexpr int VW = 16 / (int)sizeof(T);
+  static constexpr int NV = E / VW;
+  static constexpr uint32_t kFull = (1u << E) - 1u;
+  int t, nt, phase, N;
+  uint32_t mask;  // elements inside the row
+  bool full;
+  __device__ __forceinline__ Layout(int t_, int nt_, long long row, int N_) : t(t_), nt(nt_), phase(0), N(N_), mask(0) {
+    if (RAGGED) phase = (int)(row * N % VW);
 #pragma unroll
-  for (int i = 0; i < Raw<P, E>::kWords; ++i) r.w[i] = 0u;
-  if (VEC) {
-    constexpr int VW = C::VW;
-    constexpr int kWordsPerVec = VW * (int)sizeof(P) / 4;  // 2, 4 or 8
+    for (int e = 0; e < E; ++e) mask |= (uint32_t)(col(e) >= 0 && col(e) < N) << e;
+    full = mask == kFull;
+  }
+  __device__ __forceinline__ int col(int e) const { return ((e / VW) * nt + t) * VW + e % VW - phase; }
+  __device__ __forceinline__ bool inside(int e) const { return mask >> e & 1u; }
+  __device__ __forceinline__ bool any(int v) const { return (mask >> (v * VW) & ((1u << VW) - 1u)) != 0; }
+  __device__ __forceinline__ bool whole(int v) const {
+    return RAGGED ? (~mask >> (v * VW) & ((1u << VW) - 1u)) == 0 : any(v);
+  }
+  __device__ __forceinline__ void clear_outside(f32x2* x) const {
+    if (!full) {
 #pragma unroll
-    for (int v = 0; v < E / VW; ++v) {
-      const int c = (v * nt + t) * VW;
-      if (c >= N) continue;
-      uint32_t* d = r.w + v * kWordsPerVec;
-      if constexpr (kWordsPerVec == 2) {
-        const uint2 q = __ldg(reinterpret_cast<const uint2*>(p + c));
-        d[0] = q.x; d[1] = q.y;
-      } else {
-#pragma unroll
-        for (int k = 0; k < kWordsPerVec; k += 4) {
-          const uint4* src = reinterpret_cast<const uint4*>(p + c) + k / 4;
-          const uint4 q = STREAM ? __ldcs(src) : __ldg(src);
-          d[k] = q.x; d[k + 1] = q.y; d[k + 2] = q.z; d[k + 3] = q.w;
-        }
+      for (int e = 0; e < E; e += 2) {
+        float a, b;
+        upk2(x[e / 2], a, b);
+        x[e / 2] = pk2(inside(e) ? a : 0.0f, inside(e + 1) ? b : 0.0f);
       }
     }
-  } else {
+  }
+  // the thread's values of a [N] vector, `absent` where there is none
+  __device__ __forceinline__ void load_vector(const void* p, int f32, float absent, f32x2* x) const {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = e * nt + t;
-      if (c < N) r.set_scalar(e, STREAM ? __ldcs(p + c) : __ldg(p + c));
+    for (int e = 0; e < E; e += 2) {
+      float a = absent, b = absent;
+      if (p != nullptr && inside(e)) a = load_io(p, col(e), f32);
+      if (p != nullptr && inside(e + 1)) b = load_io(p, col(e + 1), f32);
+      x[e / 2] = pk2(a, b);
+    }
+  }
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {  // the rest of the 16 bytes: zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_wait(int ahead) {  // all but the newest `ahead` groups have landed
+  if (ahead >= 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (ahead == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// This thread's chunks of NT tensors, row after row: `at` is the element index
+// of its first chunk in the current row, the same in every tensor (chunk v lies
+// v * nt * VW further).  RING: the rows pass through shared memory, `stages`
+// deep; slot of stage s, tensor a, chunk v: ((s * NT + a) * NV + v) * pitch from
+// the thread's first.  Without RING chunks are loaded when they are read.
+template <class T, int E, bool RAGGED, int NT, bool RING>
+struct Rows {
+  using L = Layout<T, E, RAGGED>;
+  const T* p[NT];
+  long long at, stride;   // elements; stride: to the thread's next row
+  long long total;        // elements of each tensor
+  uint32_t smem, pitch;
+  // bytes of a chunk, from element i on, that lie inside the tensor
+  __device__ __forceinline__ int bytes_in(long long i) const {
+    const long long n = (total - i) * (long long)sizeof(T);
+    return n < 16 ? (int)n : 16;
+  }
+  // copies the row `ahead` rows on into stage `stage`; `last`: it is the tensor's last row
+  __device__ __forceinline__ void issue(const L& l, int ahead, int stage, bool last) const {
+    const long long i0 = at + ahead * stride;
+    const uint32_t dst = smem + stage * (NT * L::NV) * pitch;
+#pragma unroll
+    for (int v = 0; v < L::NV; ++v) {
+      if (!l.any(v)) continue;  // its slots hold zeros from the start
+      const long long i = i0 + (long long)v * l.nt * L::VW;
+      const int n = RAGGED && last ? bytes_in(i) : 16;
+#pragma unroll
+      for (int a = 0; a < NT; ++a) cp16(dst + (a * L::NV + v) * pitch, p[a] + i, n);
+    }
+  }
+  // zeros in the slots of chunks outside the row, which no copy writes
+  __device__ __forceinline__ void clear(const L& l, int stages) const {
+#pragma unroll
+    for (int v = 0; v < L::NV; ++v) {
+      if (l.any(v)) continue;
+      for (int k = 0; k < stages * NT; ++k)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem + (k * L::NV + v) * pitch), "r"(0) : "memory");
+    }
+  }
+  __device__ __forceinline__ void get(const L& l, int stage, int a, f32x2* x) const {
+#pragma unroll
+    for (int v = 0; v < L::NV; ++v) {
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (RING) {
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                     : "r"(smem + ((stage * NT + a) * L::NV + v) * pitch)
+                     : "memory");
+      } else if (l.any(v)) {
+        const long long i = at + (long long)v * l.nt * L::VW;
+        if (!RAGGED || bytes_in(i) == 16) {
+          q = __ldcs(reinterpret_cast<const uint4*>(p[a] + i));
+        } else {
+          f32x2 f[L::VW / 2];
+#pragma unroll
+          for (int j = 0; j < L::VW; j += 2)
+            f[j / 2] = pk2(i + j < total ? Elem<T>::get(p[a][i + j]) : 0.0f,
+                           i + j + 1 < total ? Elem<T>::get(p[a][i + j + 1]) : 0.0f);
+          q = pack(f, T());
+        }
+      }
+      unpack(q, x + v * (L::VW / 2), T());
+    }
+  }
+};
+
+// at: element index of the thread's first chunk.
+template <class T, int E, bool RAGGED>
+__device__ __forceinline__ void store_row(const Layout<T, E, RAGGED>& l, T* __restrict__ out, long long at,
+                                          const f32x2* x) {
+  using L = Layout<T, E, RAGGED>;
+#pragma unroll
+  for (int k = 0; k < L::NV; ++k) {
+    T* p = out + at + (long long)k * l.nt * L::VW;
+    if (l.whole(k)) {
+      __stcs(reinterpret_cast<uint4*>(p), pack(x + k * (L::VW / 2), T()));
+    } else if (RAGGED && l.any(k)) {
+#pragma unroll
+      for (int j = 0; j < L::VW; j += 2) {
+        float a, b;
+        upk2(x[(k * L::VW + j) / 2], a, b);
+        if (l.inside(k * L::VW + j)) p[j] = Elem<T>::put(a);
+        if (l.inside(k * L::VW + j + 1)) p[j + 1] = Elem<T>::put(b);
+      }
     }
   }
 }
 
-template <class T, int E, bool VEC>
-__device__ __forceinline__ void store_row(T* __restrict__ p, const float* v, int t, int nt, int N) {
-  using C = Cols<(int)sizeof(T), E, VEC>;
-  if (VEC) {
-    constexpr int VW = C::VW;
+template <int n>
+__device__ __forceinline__ float sum_all(const f32x2* x) {
+  f32x2 s = x[0];
 #pragma unroll
-    for (int k = 0; k < E / VW; ++k) {
-      const int c = (k * nt + t) * VW;
-      if (c >= N) continue;
-      const float* s = v + k * VW;
-      uint4 q;
-      if (sizeof(T) == 4) {
-        q = make_uint4(__float_as_uint(s[0]), __float_as_uint(s[1]), __float_as_uint(s[2]), __float_as_uint(s[3]));
-      } else {
-        q = make_uint4(pack_bf16x2_rne(s[0], s[1]), pack_bf16x2_rne(s[2], s[3]),
-                       pack_bf16x2_rne(s[VW - 4], s[VW - 3]), pack_bf16x2_rne(s[VW - 2], s[VW - 1]));
-      }
-      __stcs(reinterpret_cast<uint4*>(p + c), q);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = e * nt + t;
-      if (c < N) p[c] = Elem<T>::put(v[e]);
-    }
-  }
+  for (int k = 1; k < n; ++k) s = add2(s, x[k]);
+  return both(s);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -150,82 +279,117 @@ __device__ __forceinline__ void group_sync(int group, int nt) {
 }
 
 // Sum over the row group's threads, the same value in each; `buf` holds one
-// float per warp of the group.  The caller alternates two buffers.
+// float per warp of the group, 32 in all, zeros past the last.  The caller
+// alternates two buffers.
 __device__ __forceinline__ float group_sum(float v, float* buf, int group, int nt, int t) {
   v = warp_sum(v);
   if (nt == 32) return v;
   if ((t & 31) == 0) buf[t >> 5] = v;
   group_sync(group, nt);
-  const int lane = t & 31;
-  return warp_sum(lane < (nt >> 5) ? buf[lane] : 0.0f);
+  const float4* b = reinterpret_cast<const float4*>(buf);
+  float s = 0.0f;
+  for (int i = 0; i * 128 < nt; ++i) {
+    const float4 q = b[i];
+    s += (q.x + q.y) + (q.z + q.w);
+  }
+  return s;
 }
 
-template <class T, class W, int E, bool VEC, bool RES>
-__global__ void __launch_bounds__(kMaxRowThreads, 1)
-    fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const W* __restrict__ weight,
-               const W* __restrict__ bias, float eps, T* __restrict__ y, float* __restrict__ mean_out,
-               float* __restrict__ rstd_out, long long M, int N) {
-  using C = Cols<(int)sizeof(T), E, VEC>;
-  __shared__ float bufs[kMaxGroups][2][32];
+// CTAs per SM that the register bounds are set for: TMAX is the most threads of
+// a CTA (256; 512 beyond 4096 columns, 1024 beyond 8192).  Two or three small
+// CTAs hide one another's reductions.
+__host__ __device__ constexpr int ctas_per_sm(bool bwd, int e, int tmax) {
+  return tmax > 256 ? 1 : bwd && e == 16 ? 2 : 3;
+}
+
+template <class T, int E, bool RAGGED, bool RES, int TMAX>
+__global__ void __launch_bounds__(TMAX, ctas_per_sm(false, E, TMAX))
+    fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, const void* __restrict__ weight,
+               const void* __restrict__ bias, int wf, float eps, T* __restrict__ y, float* __restrict__ mean_out,
+               float* __restrict__ rstd_out, long long M, int N, int stages) {
+  using L = Layout<T, E, RAGGED>;
+  constexpr bool RING = TMAX <= 512;
+  constexpr int P = E / 2;  // pairs
+  __shared__ __align__(16) float bufs[kMaxGroups][2][32];
+  extern __shared__ __align__(16) uint8_t ring[];
   const int t = threadIdx.x, nt = blockDim.x, group = threadIdx.y;
   const long long step = (long long)gridDim.x * blockDim.y;
   long long row = (long long)blockIdx.x * blockDim.y + group;
   if (row >= M) return;  // named barriers count this group's threads only
-  Raw<T, E> rx, rr;
-  load_row<T, sizeof(T), E, VEC, true>(rx, x + row * N, t, nt, N);
-  if (RES) load_row<T, sizeof(T), E, VEC, true>(rr, res + row * N, t, nt, N);
-  Raw<W, E> rw, rb;
-  if (weight) load_row<W, sizeof(T), E, VEC, false>(rw, weight, t, nt, N);
-  if (bias) load_row<W, sizeof(T), E, VEC, false>(rb, bias, t, nt, N);
+  const L l(t, nt, row, N);
+  Rows<T, E, RAGGED, RES ? 2 : 1, RING> in;
+  in.p[0] = x;
+  if (RES) in.p[RES ? 1 : 0] = res;
+  in.at = row * N + l.col(0);
+  in.stride = step * N;
+  in.total = M * N;
+  in.pitch = (uint32_t)(nt * blockDim.y) * 16;
+  in.smem = (uint32_t)__cvta_generic_to_shared(ring) + (uint32_t)(group * nt + t) * 16;
+  int left = (int)((M - 1 - row) / step);        // rows after this one
+  const bool ends = row + left * step == M - 1;  // the last of them is the tensor's last
+  if (RING) {
+    in.clear(l, stages);
+    for (int s = 0; s < stages - 1; ++s) {
+      if (s <= left) in.issue(l, s, s, ends && s == left);
+      cp_commit();
+    }
+  }
+  for (int k = t; k < 64; k += nt) bufs[group][0][k] = 0.0f;  // both buffers
+  group_sync(group, nt);
+  f32x2 w[P], b[P];
+  l.load_vector(weight, wf, 1.0f, w);
+  l.load_vector(bias, wf, 0.0f, b);
   const float inv_n = 1.0f / (float)N;
-  for (; row < M; row += step) {
-    float v[E];
-    float sum = 0.0f;
+  for (int s = 0;; row += step, in.at += in.stride, --left) {
+    if (RING) {
+      if (stages - 1 <= left) in.issue(l, stages - 1, s == 0 ? stages - 1 : s - 1, ends && stages - 1 == left);
+      cp_commit();
+      cp_wait(stages - 1);
+    }
+    f32x2 v[P];
+    in.get(l, s, 0, v);
+    if (RES) {
+      f32x2 r[P];
+      in.get(l, s, RES ? 1 : 0, r);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      v[e] = RES ? __fadd_rn(rx.at(e), rr.at(e)) : rx.at(e);
-      sum += v[e];
+      for (int k = 0; k < P; ++k) v[k] = add2(v[k], r[k]);
     }
-    if (row + step < M) {  // the next row's loads, in flight during this row's reductions
-      load_row<T, sizeof(T), E, VEC, true>(rx, x + (row + step) * N, t, nt, N);
-      if (RES) load_row<T, sizeof(T), E, VEC, true>(rr, res + (row + step) * N, t, nt, N);
-    }
-    const float mean = group_sum(sum, bufs[group][0], group, nt, t) * inv_n;
-    float m2 = 0.0f;
+    if (RAGGED) l.clear_outside(v);  // whole chunks outside the row read as zero
+    const float mean = group_sum(sum_all<P>(v), bufs[group][0], group, nt, t) * inv_n;
+    const f32x2 mean2 = splat(mean);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      v[e] -= mean;
-      if (C::valid(e, t, nt, N)) m2 = fmaf(v[e], v[e], m2);
-    }
-    const float var = group_sum(m2, bufs[group][1], group, nt, t) * inv_n;
-    const float rstd = 1.0f / sqrtf(var + eps);
+    for (int k = 0; k < P; ++k) v[k] = sub2(v[k], mean2);
+    l.clear_outside(v);
+    f32x2 m2 = mul2(v[0], v[0]);
+#pragma unroll
+    for (int k = 1; k < P; ++k) m2 = fma2(v[k], v[k], m2);
+    const float rstd = rsqrtf(fmaf(group_sum(both(m2), bufs[group][1], group, nt, t), inv_n, eps));
     if (t == 0) {
       if (mean_out) mean_out[row] = mean;
       if (rstd_out) rstd_out[row] = rstd;
     }
+    const f32x2 rstd2 = splat(rstd);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float h = v[e] * rstd;
-      v[e] = weight ? (bias ? fmaf(h, rw.at(e), rb.at(e)) : h * rw.at(e)) : (bias ? h + rb.at(e) : h);
-    }
-    store_row<T, E, VEC>(y + row * N, v, t, nt, N);
+    for (int k = 0; k < P; ++k) v[k] = fma2(mul2(v[k], rstd2), w[k], b[k]);
+    store_row<T, E, RAGGED>(l, y, in.at, v);
+    if (left == 0) break;
+    s = s + 1 == stages ? 0 : s + 1;
   }
 }
 
-// Any width: three passes of one CTA over its row.
-template <class T, class W, bool RES>
-__global__ void __launch_bounds__(256) fwd_wide_kernel(const T* __restrict__ x, const T* __restrict__ res,
-                                                       const W* __restrict__ weight, const W* __restrict__ bias,
-                                                       float eps, T* __restrict__ y, float* __restrict__ mean_out,
-                                                       float* __restrict__ rstd_out, long long M, long long N) {
+// Any width and alignment: three passes of one CTA over its row.  The types
+// are run-time values; the speed of this path is L2's, not the conversions'.
+__global__ void __launch_bounds__(512) fwd_wide_kernel(const void* __restrict__ x, const void* __restrict__ res, int xf,
+                                                       const void* __restrict__ weight, const void* __restrict__ bias,
+                                                       int wf, float eps, void* __restrict__ y,
+                                                       float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                                                       long long M, long long N) {
   __shared__ float bufs[2][32];
   const int t = threadIdx.x, nt = blockDim.x;
   for (long long row = blockIdx.x; row < M; row += gridDim.x) {
-    const T* xr = x + row * N;
-    const T* rr = RES ? res + row * N : nullptr;
     auto at = [&](long long c) {
-      const float v = Elem<T>::get(__ldg(xr + c));
-      return RES ? __fadd_rn(v, Elem<T>::get(__ldg(rr + c))) : v;
+      const float v = load_io(x, row * N + c, xf);
+      return res ? __fadd_rn(v, load_io(res, row * N + c, xf)) : v;
     };
     float sum = 0.0f;
     for (long long c = t; c < N; c += nt) sum += at(c);
@@ -240,158 +404,187 @@ __global__ void __launch_bounds__(256) fwd_wide_kernel(const T* __restrict__ x, 
       if (mean_out) mean_out[row] = mean;
       if (rstd_out) rstd_out[row] = rstd;
     }
-    for (long long c = t; c < N; c += nt) {
-      const float h = (at(c) - mean) * rstd;
-      const float w = weight ? Elem<W>::get(__ldg(weight + c)) : 1.0f;
-      const float b = bias ? Elem<W>::get(__ldg(bias + c)) : 0.0f;
-      y[row * N + c] = Elem<T>::put(fmaf(h, w, b));
-    }
+    for (long long c = t; c < N; c += nt)
+      store_io(y, row * N + c, xf,
+               fmaf((at(c) - mean) * rstd, weight ? load_io(weight, c, wf) : 1.0f, bias ? load_io(bias, c, wf) : 0.0f));
   }
 }
 
-// dx, and this CTA's column sums: partial[blockIdx.x][0][n] = sum of dy * h,
-// [1][n] = sum of dy over the CTA's rows (PARAMS).  ACC_SMEM: the column sums
-// are kept in dynamic shared memory, two floats per element, each touched by
-// its owner alone.  Dynamic shared memory: [groups][2][E][nt] floats, also the
-// buffer in which the groups of a CTA are added.
-template <class T, class W, int E, bool VEC, bool RES, bool PARAMS, bool ACC_SMEM>
-__global__ void __launch_bounds__((E <= 8 && !ACC_SMEM) ? 512 : kMaxRowThreads, 1)
+// dx, and with `partial` this CTA's column sums: partial[blockIdx.x][0][n] =
+// sum of dy * h, [1][n] = sum of dy over the CTA's rows.  CTAs of more than 512
+// threads have no registers to spare for a ring's bookkeeping and the column
+// sums: they load rows directly and keep the sums in dynamic shared memory,
+// [2][E][nt] floats, each touched by its owner alone.  Otherwise dynamic shared
+// memory is the ring, then (several groups) [2][N] floats for their sums.
+template <class T, int E, bool RAGGED, bool RES, int TMAX>
+__global__ void __launch_bounds__(TMAX, ctas_per_sm(true, E, TMAX))
     bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ res,
-               const W* __restrict__ weight, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
-               T* __restrict__ dx, float* __restrict__ partial, long long M, int N) {
-  using C = Cols<(int)sizeof(T), E, VEC>;
-  __shared__ float bufs[kMaxGroups][2][2][32];
-  extern __shared__ float acc_s[];
+               const void* __restrict__ weight, int wf, const float* __restrict__ mean_in,
+               const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ partial, long long M, int N,
+               int stages) {
+  using L = Layout<T, E, RAGGED>;
+  constexpr int NT = RES ? 3 : 2;
+  constexpr int P = E / 2;  // pairs
+  constexpr bool RING = TMAX <= 512, ACC_SMEM = !RING;
+  __shared__ __align__(16) float bufs[kMaxGroups][2][2][32];
+  extern __shared__ __align__(16) uint8_t ring[];
   const int t = threadIdx.x, nt = blockDim.x, group = threadIdx.y, groups = blockDim.y;
   const long long step = (long long)gridDim.x * groups;
-  long long row = (long long)blockIdx.x * groups + group;
-  float aw[ACC_SMEM ? 1 : E], ab[ACC_SMEM ? 1 : E];
-  float* my = acc_s + (size_t)group * 2 * E * nt + t;  // + (which * E + e) * nt
-  if (PARAMS) {
+  const long long row0 = (long long)blockIdx.x * groups + group;
+  const L l(t, nt, row0, N);  // the same phase in every row of this group
+  Rows<T, E, RAGGED, NT, RING> in;
+  in.p[0] = dy;
+  in.p[1] = x;
+  if (RES) in.p[RES ? 2 : 0] = res;
+  in.at = row0 * N + l.col(0);
+  in.stride = step * N;
+  in.total = M * N;
+  in.pitch = (uint32_t)(nt * groups) * 16;
+  in.smem = (uint32_t)__cvta_generic_to_shared(ring) + (uint32_t)(group * nt + t) * 16;
+  int left = row0 < M ? (int)((M - 1 - row0) / step) : -1;  // rows after the first, -1: no row at all
+  const bool ends = row0 + left * step == M - 1;
+  if (RING) {
+    in.clear(l, stages);
+    for (int s = 0; s < stages - 1; ++s) {
+      if (s <= left) in.issue(l, s, s, ends && s == left);
+      cp_commit();
+    }
+  }
+  for (int k = t; k < 128; k += nt) bufs[group][0][0][k] = 0.0f;
+  group_sync(group, nt);
+  float* acc_s = reinterpret_cast<float*>(ring + (RING ? (size_t)stages * NT * L::NV * in.pitch : 0));
+  f32x2* my = reinterpret_cast<f32x2*>(acc_s) + t;  // ACC_SMEM (one group): + (which * P + k) * nt
+  f32x2 aw[ACC_SMEM ? 1 : P], ab[ACC_SMEM ? 1 : P];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (ACC_SMEM) {
-        my[e * nt] = 0.0f;
-        my[(E + e) * nt] = 0.0f;
-      } else {
-        aw[e] = 0.0f;
-        ab[e] = 0.0f;
-      }
+  for (int k = 0; k < P; ++k) {
+    if (ACC_SMEM) {
+      my[k * nt] = 0ull;
+      my[(P + k) * nt] = 0ull;
+    } else {
+      aw[k] = 0ull;
+      ab[k] = 0ull;
     }
   }
   const float inv_n = 1.0f / (float)N;
-  Raw<W, E> rw;
-  if (weight) load_row<W, sizeof(T), E, VEC, false>(rw, weight, t, nt, N);
-  Raw<T, E> rx, rr, rd;
-  float mean_n = 0.0f, rstd_n = 0.0f;
-  if (row < M) {
-    load_row<T, sizeof(T), E, VEC, true>(rx, x + row * N, t, nt, N);
-    if (RES) load_row<T, sizeof(T), E, VEC, true>(rr, res + row * N, t, nt, N);
-    load_row<T, sizeof(T), E, VEC, true>(rd, dy + row * N, t, nt, N);
-    mean_n = __ldg(mean_in + row);
-    rstd_n = __ldg(rstd_in + row);
-  }
-  for (int parity = 0; row < M; row += step, parity ^= 1) {
-    const float mean = mean_n, rstd = rstd_n;
-    float h[E], g[E];
-    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float v = RES ? __fadd_rn(rx.at(e), rr.at(e)) : rx.at(e);
-      const float d = rd.at(e);  // zero past N: no sum sees those columns
-      h[e] = C::valid(e, t, nt, N) ? (v - mean) * rstd : 0.0f;
-      g[e] = weight ? d * rw.at(e) : d;
-      s1 += g[e];
-      s2 = fmaf(g[e], h[e], s2);
-      if (PARAMS) {
-        if (ACC_SMEM) {
-          my[e * nt] = fmaf(d, h[e], my[e * nt]);
-          my[(E + e) * nt] += d;
-        } else {
-          aw[e] = fmaf(d, h[e], aw[e]);
-          ab[e] += d;
-        }
-      }
+  f32x2 w[P];
+  l.load_vector(weight, wf, 1.0f, w);
+  const float *mean_p = mean_in + row0, *rstd_p = rstd_in + row0;
+  float mean_n = left >= 0 ? __ldg(mean_p) : 0.0f, rstd_n = left >= 0 ? __ldg(rstd_p) : 0.0f;
+  int parity = 0;
+  for (int s = 0; left >= 0; in.at += in.stride, --left, parity ^= 1) {
+    if (RING) {
+      if (stages - 1 <= left) in.issue(l, stages - 1, s == 0 ? stages - 1 : s - 1, ends && stages - 1 == left);
+      cp_commit();
+      cp_wait(stages - 1);
     }
-    if (row + step < M) {
-      load_row<T, sizeof(T), E, VEC, true>(rx, x + (row + step) * N, t, nt, N);
-      if (RES) load_row<T, sizeof(T), E, VEC, true>(rr, res + (row + step) * N, t, nt, N);
-      load_row<T, sizeof(T), E, VEC, true>(rd, dy + (row + step) * N, t, nt, N);
-      mean_n = __ldg(mean_in + row + step);
-      rstd_n = __ldg(rstd_in + row + step);
+    const f32x2 mean = splat(mean_n), rstd = splat(rstd_n);
+    if (left > 0) {
+      mean_p += step;
+      rstd_p += step;
+      mean_n = __ldg(mean_p);
+      rstd_n = __ldg(rstd_p);
+    }
+    f32x2 h[P], g[P];
+    in.get(l, s, 0, g);
+    in.get(l, s, 1, h);
+    if (RES) {
+      f32x2 r[P];
+      in.get(l, s, RES ? 2 : 0, r);
+#pragma unroll
+      for (int k = 0; k < P; ++k) h[k] = add2(h[k], r[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < P; ++k) h[k] = mul2(sub2(h[k], mean), rstd);
+    if (RAGGED) l.clear_outside(g);
+    if (RAGGED) l.clear_outside(h);  // whole chunks outside the row: g is zero there
+    f32x2 s1 = 0ull, s2 = 0ull;
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      if (ACC_SMEM) {
+        my[k * nt] = fma2(g[k], h[k], my[k * nt]);
+        my[(P + k) * nt] = add2(my[(P + k) * nt], g[k]);
+      } else {
+        aw[k] = fma2(g[k], h[k], aw[k]);
+        ab[k] = add2(ab[k], g[k]);
+      }
+      g[k] = mul2(g[k], w[k]);
+      s1 = add2(s1, g[k]);
+      s2 = fma2(g[k], h[k], s2);
     }
     if (dx) {
-      s1 = warp_sum(s1);
-      s2 = warp_sum(s2);
+      float m1 = warp_sum(both(s1)), m2 = warp_sum(both(s2));
       if (nt > 32) {
         float* b1 = bufs[group][parity][0];
         float* b2 = bufs[group][parity][1];
         if ((t & 31) == 0) {
-          b1[t >> 5] = s1;
-          b2[t >> 5] = s2;
+          b1[t >> 5] = m1;
+          b2[t >> 5] = m2;
         }
         group_sync(group, nt);
-        const int lane = t & 31;
-        s1 = warp_sum(lane < (nt >> 5) ? b1[lane] : 0.0f);
-        s2 = warp_sum(lane < (nt >> 5) ? b2[lane] : 0.0f);
+        m1 = m2 = 0.0f;
+        for (int i = 0; i * 128 < nt; ++i) {
+          const float4 q1 = reinterpret_cast<const float4*>(b1)[i], q2 = reinterpret_cast<const float4*>(b2)[i];
+          m1 += (q1.x + q1.y) + (q1.z + q1.w);
+          m2 += (q2.x + q2.y) + (q2.z + q2.w);
+        }
       }
-      const float m1 = s1 * inv_n, m2 = s2 * inv_n;
+      const f32x2 a1 = splat(m1 * inv_n), a2 = splat(m2 * inv_n);
 #pragma unroll
-      for (int e = 0; e < E; ++e) h[e] = rstd * (g[e] - fmaf(h[e], m2, m1));
-      store_row<T, E, VEC>(dx + row * N, h, t, nt, N);
+      for (int k = 0; k < P; ++k) h[k] = mul2(rstd, sub2(g[k], fma2(h[k], a2, a1)));
+      store_row<T, E, RAGGED>(l, dx, in.at, h);
     }
+    s = s + 1 == stages ? 0 : s + 1;
   }
-  if (!PARAMS) return;
-  if (!ACC_SMEM && groups > 1) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      my[e * nt] = aw[e];
-      my[(E + e) * nt] = ab[e];
-    }
-  }
-  if (groups > 1) __syncthreads();
-  if (group != 0) return;
+  if (partial == nullptr) return;
+  // Groups of a CTA have different phases when rows are not whole chunks, so
+  // their sums are added per column: each group in turn into [2][N] floats.
   float* out = partial + (size_t)blockIdx.x * 2 * N;
+  for (int q = 0; q < groups; ++q) {
+    if (groups > 1) __syncthreads();
+    if (group != q) continue;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    float a, b;
-    if (ACC_SMEM || groups > 1) {
-      a = my[e * nt];
-      b = my[(E + e) * nt];
-      for (int q = 1; q < groups; ++q) {
-        a += my[((size_t)q * 2 * E + e) * nt];
-        b += my[((size_t)q * 2 * E + E + e) * nt];
+    for (int k = 0; k < P; ++k) {
+      const f32x2 av = ACC_SMEM ? my[k * nt] : aw[ACC_SMEM ? 0 : k];
+      const f32x2 bv = ACC_SMEM ? my[(P + k) * nt] : ab[ACC_SMEM ? 0 : k];
+      float a[2], b[2];
+      upk2(av, a[0], a[1]);
+      upk2(bv, b[0], b[1]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int c = l.col(2 * k + j);
+        if (!l.inside(2 * k + j)) continue;
+        if (groups == 1) {
+          out[c] = a[j];
+          out[N + c] = b[j];
+        } else {
+          acc_s[c] = q == 0 ? a[j] : acc_s[c] + a[j];
+          acc_s[N + c] = q == 0 ? b[j] : acc_s[N + c] + b[j];
+        }
       }
-    } else {
-      a = aw[e];
-      b = ab[e];
-    }
-    const int c = C::col(e, t, nt);
-    if (c < N) {
-      out[c] = a;
-      out[N + c] = b;
     }
   }
+  if (groups == 1) return;
+  __syncthreads();
+  for (int c = group * nt + t; c < 2 * N; c += nt * groups) out[c] = acc_s[c];
 }
 
-// Any width: dx in two passes of one CTA over its row.
-template <class T, class W, bool RES>
-__global__ void __launch_bounds__(256)
-    bwd_wide_kernel(const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ res,
-                    const W* __restrict__ weight, const float* __restrict__ mean_in,
-                    const float* __restrict__ rstd_in, T* __restrict__ dx, long long M, long long N) {
+// Any width and alignment: dx in two passes of one CTA over its row.
+__global__ void __launch_bounds__(512)
+    bwd_wide_kernel(const void* __restrict__ dy, const void* __restrict__ x, const void* __restrict__ res, int xf,
+                    const void* __restrict__ weight, int wf, const float* __restrict__ mean_in,
+                    const float* __restrict__ rstd_in, void* __restrict__ dx, long long M, long long N) {
   __shared__ float bufs[2][32];
   const int t = threadIdx.x, nt = blockDim.x;
   for (long long row = blockIdx.x; row < M; row += gridDim.x) {
     const float mean = mean_in[row], rstd = rstd_in[row];
     auto hat = [&](long long c) {
-      float v = Elem<T>::get(__ldg(x + row * N + c));
-      if (RES) v = __fadd_rn(v, Elem<T>::get(__ldg(res + row * N + c)));
+      float v = load_io(x, row * N + c, xf);
+      if (res) v = __fadd_rn(v, load_io(res, row * N + c, xf));
       return (v - mean) * rstd;
     };
     auto grad = [&](long long c) {
-      const float d = Elem<T>::get(__ldg(dy + row * N + c));
-      return weight ? d * Elem<W>::get(__ldg(weight + c)) : d;
+      const float d = load_io(dy, row * N + c, xf);
+      return weight ? d * load_io(weight, c, wf) : d;
     };
     float s1 = 0.0f, s2 = 0.0f;
     for (long long c = t; c < N; c += nt) {
@@ -401,24 +594,24 @@ __global__ void __launch_bounds__(256)
     }
     const float m1 = group_sum(s1, bufs[0], 0, nt, t) / (float)N;
     const float m2 = group_sum(s2, bufs[1], 0, nt, t) / (float)N;
-    for (long long c = t; c < N; c += nt)
-      dx[row * N + c] = Elem<T>::put(rstd * (grad(c) - fmaf(hat(c), m2, m1)));
+    for (long long c = t; c < N; c += nt) store_io(dx, row * N + c, xf, rstd * (grad(c) - fmaf(hat(c), m2, m1)));
   }
 }
 
-// Any width: column sums of a slab of rows, one column per thread.
-template <class T, bool RES>
+// Any width and alignment: column sums of every gridDim.y-th row, one column
+// per thread.
 __global__ void __launch_bounds__(256)
-    bwd_wide_cols_kernel(const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ res,
+    bwd_wide_cols_kernel(const void* __restrict__ dy, const void* __restrict__ x, const void* __restrict__ res, int xf,
                          const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
                          float* __restrict__ partial, long long M, long long N) {
   const long long c = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= N) return;
   float a = 0.0f, b = 0.0f;
+#pragma unroll 4
   for (long long row = blockIdx.y; row < M; row += gridDim.y) {
-    float v = Elem<T>::get(__ldg(x + row * N + c));
-    if (RES) v = __fadd_rn(v, Elem<T>::get(__ldg(res + row * N + c)));
-    const float d = Elem<T>::get(__ldg(dy + row * N + c));
+    float v = load_io(x, row * N + c, xf);
+    if (res) v = __fadd_rn(v, load_io(res, row * N + c, xf));
+    const float d = load_io(dy, row * N + c, xf);
     a = fmaf(d, (v - __ldg(mean_in + row)) * __ldg(rstd_in + row), a);
     b += d;
   }
@@ -460,140 +653,151 @@ int reduce_cols(const float* partial, int slabs, int planes, long long N, W* out
   return launch_status();
 }
 
-constexpr int kSlabs = 148 * 2;  // upper bound of the CTAs that leave column sums (workspace)
+constexpr int kWideSlabs = 64;  // row slabs of bwd_wide_cols_kernel
 
 struct Shape {
-  int nt, groups, e;
+  int e, nt, groups, grid, stages;
+  bool ragged;  // rows are not whole 16-byte chunks
+  size_t smem;
 };
-// Threads per row (E = 8 elements each, 16 beyond 8192 columns) and rows per
-// CTA (CTAs of about `target` threads).
-inline Shape shape(long long N, int target) {
+
+// Elements per thread: 8 up to 1024 columns, 16 beyond (fewer threads to
+// reduce over).  Beyond 8192 columns a CTA has more than 512 threads and the
+// backward's column sums move from registers to shared memory.  Rows per CTA: about 256
+// threads.  Grid: as many CTAs as shared memory and threads allow per SM, a
+// whole number of phases when rows are not whole chunks.  Ring: up to 3
+// stages, what fits.
+inline Shape shape(long long M, long long N, int esize, int tensors, bool bwd) {
   Shape s{};
-  s.e = N <= 8LL * kMaxRowThreads ? 8 : 16;
-  s.nt = (int)(((N + s.e - 1) / s.e + 31) / 32 * 32);
-  s.groups = target / s.nt;
+  const int vw = 16 / esize;
+  s.e = N <= 1024 ? 8 : 16;
+  s.ragged = N % vw != 0;
+  const long long span = s.ragged ? N + vw - 1 : N;
+  s.nt = (int)((span + 32LL * s.e - 1) / (32LL * s.e) * 32);
+  s.groups = 256 / s.nt;
   s.groups = s.groups < 1 ? 1 : s.groups > kMaxGroups ? kMaxGroups : s.groups;
+  if (s.groups > M) s.groups = (int)M;
+  const int threads = s.nt * s.groups;
+  // column sums: 1024-thread CTAs keep them here, several groups add them here
+  const size_t acc = !bwd ? 0 : s.nt > 512 ? (size_t)2 * s.e * s.nt * 4 : s.groups > 1 ? (size_t)2 * N * 4 : 0;
+  const size_t stage = (size_t)tensors * s.e * esize * threads;  // at most 96 KB up to 512 threads
+  s.stages = s.nt > 512 ? 0 : (int)((kMaxSmem - acc) / stage);
+  if (s.stages > 3) s.stages = 3;
+  s.smem = acc + stage * s.stages;
+  int per_sm = ctas_per_sm(bwd, s.e, threads <= 256 ? 256 : 1024);
+  if (s.smem > 0 && per_sm > (int)(kMaxSmem / s.smem)) per_sm = (int)(kMaxSmem / s.smem);
+  if (per_sm < 1) per_sm = 1;
+  const long long want = (M + s.groups - 1) / s.groups;
+  long long cap = (long long)sm_count() * per_sm;
+  if (s.ragged && want > cap) cap = cap / vw * vw;
+  s.grid = (int)(want < cap ? want : cap);
   return s;
 }
+// Rows this wide have no register path (a ragged row spans up to 7 more columns).
+inline bool wide(long long N) { return N > kMaxRegN || (N > kMaxRegN - 8 && N % 8 != 0); }
 
-inline int grid_rows(long long M, int groups, int per_sm) {
-  const long long want = (M + groups - 1) / groups;
-  const long long cap = (long long)sm_count() * per_sm;
-  return (int)(want < cap ? want : cap);
+// CTAs of the backward, each leaving one slab of column sums.
+inline int bwd_slabs(long long M, long long N, int esize, bool res, bool vec) {
+  if (!vec || wide(N)) return (int)(M < kWideSlabs ? M : kWideSlabs);
+  return shape(M, N, esize, res ? 3 : 2, true).grid;
 }
 
-template <class T, class W, int E, bool VEC, bool RES>
-int launch_fwd(const Shape& s, const void* x, const void* res, const void* w, const void* b, float eps, void* y,
-               float* mean, float* rstd, long long M, long long N, cudaStream_t st) {
-  const int threads = s.nt * s.groups;
-  const int grid = grid_rows(M, s.groups, 2048 / threads > 0 ? 2048 / threads : 1);
-  fwd_kernel<T, W, E, VEC, RES><<<grid, dim3(s.nt, s.groups), 0, st>>>(
-      static_cast<const T*>(x), static_cast<const T*>(res), static_cast<const W*>(w), static_cast<const W*>(b), eps,
-      static_cast<T*>(y), mean, rstd, M, (int)N);
-  return launch_status();
-}
-
-template <class T, class W>
-int forward(const void* x, const void* res, const void* w, const void* b, float eps, void* y, float* mean, float* rstd,
-            long long M, long long N, cudaStream_t st) {
-  if (N > kMaxRegN) {
-    const int grid = grid_rows(M, 1, 8);
-    if (res)
-      fwd_wide_kernel<T, W, true><<<grid, 256, 0, st>>>(static_cast<const T*>(x), static_cast<const T*>(res),
-                                                        static_cast<const W*>(w), static_cast<const W*>(b), eps,
-                                                        static_cast<T*>(y), mean, rstd, M, N);
-    else
-      fwd_wide_kernel<T, W, false><<<grid, 256, 0, st>>>(static_cast<const T*>(x), nullptr,
-                                                         static_cast<const W*>(w), static_cast<const W*>(b), eps,
-                                                         static_cast<T*>(y), mean, rstd, M, N);
-    return launch_status();
-  }
-  const bool vec = N % (16 / (int)sizeof(T)) == 0 && aligned(x, 16) && aligned(res, 16) && aligned(y, 16) &&
-                   aligned(w, 16) && aligned(b, 16);
-  const Shape s = shape(N, 256);
-#define PACKR_NORM_FWD(E, V, R) \
-  return launch_fwd<T, W, E, V, R>(s, x, res, w, b, eps, y, mean, rstd, M, N, st)
-  if (s.e == 8) {
-    if (vec) { if (res) PACKR_NORM_FWD(8, true, true); else PACKR_NORM_FWD(8, true, false); }
-    if (res) PACKR_NORM_FWD(8, false, true); else PACKR_NORM_FWD(8, false, false);
-  }
-  if (vec) { if (res) PACKR_NORM_FWD(16, true, true); else PACKR_NORM_FWD(16, true, false); }
-  if (res) PACKR_NORM_FWD(16, false, true); else PACKR_NORM_FWD(16, false, false);
-#undef PACKR_NORM_FWD
-}
-
-template <class T, class W, int E, bool VEC, bool RES, bool PARAMS, bool ACC_SMEM>
-int launch_bwd(const Shape& s, const void* dy, const void* x, const void* res, const void* w, const float* mean,
-               const float* rstd, void* dx, float* partial, int slabs, long long M, long long N, cudaStream_t st) {
-  auto kern = bwd_kernel<T, W, E, VEC, RES, PARAMS, ACC_SMEM>;
-  const size_t smem = PARAMS && (ACC_SMEM || s.groups > 1) ? (size_t)s.groups * 2 * E * s.nt * sizeof(float) : 0;
-  if (smem > 48 * 1024 &&
+template <class K>
+int allow_smem(K kern, size_t smem) {
+  if (smem > 40 * 1024 &&  // the default limit less the static buffers
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
     cudaGetLastError();
     return PACKR_ERR_CUDA;
   }
-  kern<<<slabs, dim3(s.nt, s.groups), smem, st>>>(static_cast<const T*>(dy), static_cast<const T*>(x),
-                                                  static_cast<const T*>(res), static_cast<const W*>(w), mean, rstd,
-                                                  static_cast<T*>(dx), partial, M, (int)N);
+  return PACKR_OK;
+}
+
+template <class T, int E, bool RES, int TMAX>
+int launch_fwd(const Shape& s, const void* x, const void* res, const void* w, const void* b, int wf, float eps, void* y,
+               float* mean, float* rstd, long long M, long long N, cudaStream_t st) {
+  auto kern = s.ragged ? fwd_kernel<T, E, true, RES, TMAX> : fwd_kernel<T, E, false, RES, TMAX>;
+  const int rc = allow_smem(kern, s.smem);
+  if (rc != PACKR_OK) return rc;
+  kern<<<s.grid, dim3(s.nt, s.groups), s.smem, st>>>(static_cast<const T*>(x), static_cast<const T*>(res), w, b, wf, eps,
+                                                     static_cast<T*>(y), mean, rstd, M, (int)N, s.stages);
   return launch_status();
 }
 
-// CTAs of the backward, each leaving one slab of column sums.
-inline int bwd_slabs(long long M, long long N) {
-  if (N > kMaxRegN) return (int)(M < 64 ? M : 64);
-  const Shape s = shape(N, 512);
-  const int n = grid_rows(M, s.groups, s.nt * s.groups <= 512 ? 2 : 1);
-  return n < kSlabs ? n : kSlabs;
+template <class T>
+int forward(const void* x, const void* res, const void* w, const void* b, int wf, float eps, void* y, float* mean,
+            float* rstd, long long M, long long N, cudaStream_t st) {
+  const bool vec = aligned(x, 16) && aligned(res, 16) && aligned(y, 16);
+  if (!vec || wide(N)) {
+    const long long cap = 4LL * sm_count();
+    fwd_wide_kernel<<<(int)(M < cap ? M : cap), N >= 4096 ? 512 : 128, 0, st>>>(x, res, sizeof(T) == 4, w, b, wf, eps, y,
+                                                                               mean, rstd, M, N);
+    return launch_status();
+  }
+  const Shape s = shape(M, N, sizeof(T), res ? 2 : 1, false);
+#define PACKR_NORM_FWD(E, TMAX)                                                              \
+  return res ? launch_fwd<T, E, true, TMAX>(s, x, res, w, b, wf, eps, y, mean, rstd, M, N, st) \
+             : launch_fwd<T, E, false, TMAX>(s, x, res, w, b, wf, eps, y, mean, rstd, M, N, st)
+  if (s.e == 8) PACKR_NORM_FWD(8, 256);
+  if (s.nt <= 256) PACKR_NORM_FWD(16, 256);
+  if (s.nt <= 512) PACKR_NORM_FWD(16, 512);
+  PACKR_NORM_FWD(16, 1024);
+#undef PACKR_NORM_FWD
 }
 
-template <class T, class W, bool RES>
-int backward_res(const void* dy, const void* x, const void* res, const void* w, const float* mean, const float* rstd,
-                 void* dx, void* dw, void* db, float* partial, long long M, long long N, cudaStream_t st) {
+template <class T, int E, bool RES, int TMAX>
+int launch_bwd(const Shape& s, const void* dy, const void* x, const void* res, const void* w, int wf, const float* mean,
+               const float* rstd, void* dx, float* partial, long long M, long long N, cudaStream_t st) {
+  auto kern = s.ragged ? bwd_kernel<T, E, true, RES, TMAX> : bwd_kernel<T, E, false, RES, TMAX>;
+  const int rc = allow_smem(kern, s.smem);
+  if (rc != PACKR_OK) return rc;
+  kern<<<s.grid, dim3(s.nt, s.groups), s.smem, st>>>(static_cast<const T*>(dy), static_cast<const T*>(x),
+                                                     static_cast<const T*>(res), w, wf, mean, rstd,
+                                                     static_cast<T*>(dx), partial, M, (int)N, s.stages);
+  return launch_status();
+}
+
+template <class T>
+int backward(const void* dy, const void* x, const void* res, const void* w, int wf, const float* mean,
+             const float* rstd, void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes, long long M,
+             long long N, cudaStream_t st) {
   const bool params = dw != nullptr || db != nullptr;
-  const int slabs = bwd_slabs(M, N);
+  const bool vec = aligned(dy, 16) && aligned(x, 16) && aligned(res, 16) && aligned(dx, 16);
+  const int slabs = bwd_slabs(M, N, sizeof(T), res != nullptr, vec);
+  float* partial = params ? static_cast<float*>(workspace) : nullptr;
+  if (params && (workspace == nullptr || workspace_bytes < (size_t)slabs * 2 * N * sizeof(float) || !aligned(workspace, 16)))
+    return PACKR_ERR_WORKSPACE;
   int rc = PACKR_OK;
-  if (N > kMaxRegN) {
+  if (!vec || wide(N)) {
+    const int xf = sizeof(T) == 4;
     if (dx) {
-      bwd_wide_kernel<T, W, RES><<<grid_rows(M, 1, 8), 256, 0, st>>>(
-          static_cast<const T*>(dy), static_cast<const T*>(x), static_cast<const T*>(res), static_cast<const W*>(w),
-          mean, rstd, static_cast<T*>(dx), M, N);
+      const long long cap = 4LL * sm_count();
+      bwd_wide_kernel<<<(int)(M < cap ? M : cap), N >= 4096 ? 512 : 128, 0, st>>>(dy, x, res, xf, w, wf, mean, rstd, dx, M,
+                                                                                  N);
       if ((rc = launch_status()) != PACKR_OK) return rc;
     }
     if (params) {
-      bwd_wide_cols_kernel<T, RES><<<dim3((unsigned)((N + 255) / 256), (unsigned)slabs), 256, 0, st>>>(
-          static_cast<const T*>(dy), static_cast<const T*>(x), static_cast<const T*>(res), mean, rstd, partial, M, N);
-      if ((rc = launch_status()) != PACKR_OK) return rc;
+      bwd_wide_cols_kernel<<<dim3((unsigned)((N + 255) / 256), (unsigned)slabs), 256, 0, st>>>(dy, x, res, xf, mean, rstd,
+                                                                                               partial, M, N);
+      rc = launch_status();
     }
   } else {
-    const bool vec = N % (16 / (int)sizeof(T)) == 0 && aligned(dy, 16) && aligned(x, 16) && aligned(res, 16) &&
-                     aligned(dx, 16) && aligned(w, 16);
-    const Shape s = shape(N, 512);
-#define PACKR_NORM_BWD(E, V, P, A) \
-  rc = launch_bwd<T, W, E, V, RES, P, A>(s, dy, x, res, w, mean, rstd, dx, partial, slabs, M, N, st)
-#define PACKR_NORM_BWD_P(E, V, A)                                            \
-  do {                                                                       \
-    if (params) PACKR_NORM_BWD(E, V, true, A); else PACKR_NORM_BWD(E, V, false, A); \
-  } while (0)
-    if (s.nt <= 512 && s.e == 8) {
-      if (vec) PACKR_NORM_BWD_P(8, true, false); else PACKR_NORM_BWD_P(8, false, false);
-    } else if (s.e == 8) {
-      if (vec) PACKR_NORM_BWD_P(8, true, true); else PACKR_NORM_BWD_P(8, false, true);
-    } else {
-      if (vec) PACKR_NORM_BWD_P(16, true, true); else PACKR_NORM_BWD_P(16, false, true);
-    }
-#undef PACKR_NORM_BWD_P
+    const Shape s = shape(M, N, sizeof(T), res ? 3 : 2, true);
+#define PACKR_NORM_BWD(E, TMAX)                                                                  \
+  rc = res ? launch_bwd<T, E, true, TMAX>(s, dy, x, res, w, wf, mean, rstd, dx, partial, M, N, st) \
+           : launch_bwd<T, E, false, TMAX>(s, dy, x, res, w, wf, mean, rstd, dx, partial, M, N, st)
+    if (s.e == 8)
+      PACKR_NORM_BWD(8, 256);
+    else if (s.nt <= 256)
+      PACKR_NORM_BWD(16, 256);
+    else if (s.nt <= 512)
+      PACKR_NORM_BWD(16, 512);
+    else
+      PACKR_NORM_BWD(16, 1024);
 #undef PACKR_NORM_BWD
-    if (rc != PACKR_OK) return rc;
   }
-  if (!params) return PACKR_OK;
-  return reduce_cols(partial, slabs, 2, N, static_cast<W*>(dw), static_cast<W*>(db), st);
-}
-
-template <class T, class W>
-int backward(const void* dy, const void* x, const void* res, const void* w, const float* mean, const float* rstd,
-             void* dx, void* dw, void* db, float* partial, long long M, long long N, cudaStream_t st) {
-  return res ? backward_res<T, W, true>(dy, x, res, w, mean, rstd, dx, dw, db, partial, M, N, st)
-             : backward_res<T, W, false>(dy, x, res, w, mean, rstd, dx, dw, db, partial, M, N, st);
+  if (rc != PACKR_OK || !params) return rc;
+  return wf ? reduce_cols(partial, slabs, 2, N, static_cast<float*>(dw), static_cast<float*>(db), st)
+            : reduce_cols(partial, slabs, 2, N, static_cast<uint16_t*>(dw), static_cast<uint16_t*>(db), st);
 }
 
 inline int check(long long M, long long N, int x_dtype, int w_dtype, const void* const* xs, int nx,
@@ -627,15 +831,19 @@ extern "C" int packr_layer_norm_forward(const void* x, const void* residual, int
   if (M == 0) return PACKR_OK;
   cudaStream_t s = as_stream(stream);
   const bool xf = x_dtype == PACKR_DTYPE_F32, wf = w_dtype == PACKR_DTYPE_F32;
-  if (xf && wf) return norm::forward<float, float>(x, residual, weight, bias, eps, y, mean, rstd, M, N, s);
-  if (xf) return norm::forward<float, uint16_t>(x, residual, weight, bias, eps, y, mean, rstd, M, N, s);
-  if (wf) return norm::forward<uint16_t, float>(x, residual, weight, bias, eps, y, mean, rstd, M, N, s);
-  return norm::forward<uint16_t, uint16_t>(x, residual, weight, bias, eps, y, mean, rstd, M, N, s);
+  return xf ? norm::forward<float>(x, residual, weight, bias, wf, eps, y, mean, rstd, M, N, s)
+            : norm::forward<uint16_t>(x, residual, weight, bias, wf, eps, y, mean, rstd, M, N, s);
 }
 
 extern "C" size_t packr_layer_norm_backward_workspace_bytes(int64_t M, int64_t N) {
   if (M <= 0 || N <= 0 || M > 0x7FFFFFFFll || N > 0x7FFFFFFFll) return 0;
-  return (size_t)packr::norm::bwd_slabs(M, N) * 2 * (size_t)N * sizeof(float);
+  // the most of any type, residual and alignment
+  int slabs = 0;
+  for (int i = 0; i < 5; ++i) {
+    const int n = packr::norm::bwd_slabs(M, N, i & 1 ? 2 : 4, (i & 2) != 0, i != 4);
+    slabs = n > slabs ? n : slabs;
+  }
+  return (size_t)slabs * 2 * (size_t)N * sizeof(float);
 }
 
 extern "C" int packr_layer_norm_backward(const void* dy, const void* x, const void* residual, int x_dtype,
@@ -659,18 +867,8 @@ extern "C" int packr_layer_norm_backward(const void* dy, const void* x, const vo
     return PACKR_OK;
   }
   if (dx == nullptr && dweight == nullptr && dbias == nullptr) return PACKR_OK;
-  if (dweight != nullptr || dbias != nullptr) {
-    if (workspace == nullptr || workspace_bytes < packr_layer_norm_backward_workspace_bytes(M, N) ||
-        !aligned(workspace, 16))
-      return PACKR_ERR_WORKSPACE;
-  }
-  float* partial = static_cast<float*>(workspace);
-  if (xf && wf)
-    return norm::backward<float, float>(dy, x, residual, weight, mean, rstd, dx, dweight, dbias, partial, M, N, s);
-  if (xf)
-    return norm::backward<float, uint16_t>(dy, x, residual, weight, mean, rstd, dx, dweight, dbias, partial, M, N, s);
-  if (wf)
-    return norm::backward<uint16_t, float>(dy, x, residual, weight, mean, rstd, dx, dweight, dbias, partial, M, N, s);
-  return norm::backward<uint16_t, uint16_t>(dy, x, residual, weight, mean, rstd, dx, dweight, dbias, partial, M, N,
-                                            s);
+  return xf ? norm::backward<float>(dy, x, residual, weight, wf, mean, rstd, dx, dweight, dbias, workspace,
+                                    workspace_bytes, M, N, s)
+            : norm::backward<uint16_t>(dy, x, residual, weight, wf, mean, rstd, dx, dweight, dbias, workspace,
+                                       workspace_bytes, M, N, s);
 }
