@@ -640,29 +640,30 @@ struct EpiBlock {
       const int w = lane & 15;
       const bool col_in = w < nval;
       const float b = P.bias != nullptr && col_in ? load_io(P.bias, gn0 + w, P.bias_f32) : 0.0f;
+      const int row2 = r0 + (lane >> 4);  // and + 2, + 4, ...
+      const long long o0 = (long long)row2 * P.ld_out + gn0 + w;
 #pragma unroll 1
-      for (int i = 0; i < 16; i += 4) {
-        float f[4], r4[4];
+      for (int i = 0; i < 16; i += 8) {
+        float f[8], r8[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 8; ++k)
+          r8[k] = E.residual != nullptr && col_in && row2 + 2 * (i + k) < P.Mg
+                      ? load_io(E.residual, o0 + 2 * (i + k) * P.ld_out, F32) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
           const int r = (i + k) * 2 + (lane >> 4);
-          const long long o = (long long)(r0 + r) * P.ld_out + gn0 + w;
-          const bool in = col_in && r0 + r < P.Mg;
-          r4[k] = E.residual != nullptr && in ? load_io(E.residual, o, F32) : 0.0f;
           asm volatile("ld.shared.f32 %0, [%1];"
                        : "=f"(f[k])
                        : "r"(stg + (uint32_t)(r * 64 + (((w >> 2) ^ ((r >> 1) & 3)) << 4) + (w & 3) * 4))
                        : "memory");
           f[k] = __fadd_rn(f[k], b);
-          if (E.z != nullptr && in) store_io(E.z, o, F32, f[k]);
+          if (E.z != nullptr && col_in && row2 + 2 * (i + k) < P.Mg) store_io(E.z, o0 + 2 * (i + k) * P.ld_out, F32, f[k]);
         }
-        act::apply_all<4>(E.act, f);
+        act::apply_all<8>(E.act, f);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = (i + k) * 2 + (lane >> 4);
-          if (col_in && r0 + r < P.Mg)
-            store_io(E.out, (long long)(r0 + r) * P.ld_out + gn0 + w, F32, __fadd_rn(f[k], r4[k]));
-        }
+        for (int k = 0; k < 8; ++k)
+          if (col_in && row2 + 2 * (i + k) < P.Mg)
+            store_io(E.out, o0 + 2 * (i + k) * P.ld_out, F32, __fadd_rn(f[k], r8[k]));
       }
     }
     __syncwarp();  // the buffer is free for the next half

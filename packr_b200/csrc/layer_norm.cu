@@ -123,7 +123,7 @@ template <class T, int E, bool RAGGED>
 struct Layout {
   static constexpr int VW = 16 / (int)sizeof(T);
   static constexpr int NV = E / VW;
-  static constexpr uint32_t kFull = (1u << E) - 1u;
+  static constexpr uint32_t kFull = E == 32 ? 0xFFFFFFFFu : (1u << (E & 31)) - 1u;
   int t, nt, phase, N;
   uint32_t mask;  // elements inside the row
   bool full;
@@ -151,6 +151,25 @@ struct Layout {
   }
   // the thread's values of a [N] vector, `absent` where there is none
   __device__ __forceinline__ void load_vector(const void* p, int f32, float absent, f32x2* x) const {
+    if (!RAGGED && p != nullptr && aligned(p, 16)) {  // whole chunks: 8- or 16-byte loads
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+#pragma unroll
+        for (int k = 0; k < VW; k += 4) {
+          f32x2* d = x + (v * VW + k) / 2;
+          d[0] = d[1] = splat(absent);
+          if (!any(v)) continue;
+          if (f32) {
+            unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(p) + col(v * VW) + k)), d, float());
+          } else {
+            const uint2 q = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + col(v * VW) + k));
+            d[0] = pk2(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xFFFF0000u));
+            d[1] = pk2(__uint_as_float(q.y << 16), __uint_as_float(q.y & 0xFFFF0000u));
+          }
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
       float a = absent, b = absent;
@@ -210,6 +229,7 @@ struct Rows {
         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(smem + (k * L::NV + v) * pitch), "r"(0) : "memory");
     }
   }
+  template <bool ADD>  // ADD: onto x
   __device__ __forceinline__ void get(const L& l, int stage, int a, f32x2* x) const {
 #pragma unroll
     for (int v = 0; v < L::NV; ++v) {
@@ -232,7 +252,14 @@ struct Rows {
           q = pack(f, T());
         }
       }
-      unpack(q, x + v * (L::VW / 2), T());
+      if (ADD) {
+        f32x2 r[L::VW / 2];
+        unpack(q, r, T());
+#pragma unroll
+        for (int j = 0; j < L::VW / 2; ++j) x[v * (L::VW / 2) + j] = add2(x[v * (L::VW / 2) + j], r[j]);
+      } else {
+        unpack(q, x + v * (L::VW / 2), T());
+      }
     }
   }
 };
@@ -295,11 +322,11 @@ __device__ __forceinline__ float group_sum(float v, float* buf, int group, int n
   return s;
 }
 
-// CTAs per SM that the register bounds are set for: TMAX is the most threads of
-// a CTA (256; 512 beyond 4096 columns, 1024 beyond 8192).  Two or three small
-// CTAs hide one another's reductions.
+// CTAs of TMAX threads per SM that the register bounds are set for: 80 registers
+// a thread, 128 where more values are held, 64 with 1024 threads.  Two or three
+// small CTAs hide one another's reductions.
 __host__ __device__ constexpr int ctas_per_sm(bool bwd, int e, int tmax) {
-  return tmax > 256 ? 1 : bwd && e == 16 ? 2 : 3;
+  return tmax > 256 ? 1 : e == 8 || (e == 16 && !bwd) ? 3 : 2;
 }
 
 template <class T, int E, bool RAGGED, bool RES, int TMAX>
@@ -308,7 +335,7 @@ __global__ void __launch_bounds__(TMAX, ctas_per_sm(false, E, TMAX))
                const void* __restrict__ bias, int wf, float eps, T* __restrict__ y, float* __restrict__ mean_out,
                float* __restrict__ rstd_out, long long M, int N, int stages) {
   using L = Layout<T, E, RAGGED>;
-  constexpr bool RING = TMAX <= 512;
+  constexpr bool RING = true;
   constexpr int P = E / 2;  // pairs
   __shared__ __align__(16) float bufs[kMaxGroups][2][32];
   extern __shared__ __align__(16) uint8_t ring[];
@@ -347,13 +374,8 @@ __global__ void __launch_bounds__(TMAX, ctas_per_sm(false, E, TMAX))
       cp_wait(stages - 1);
     }
     f32x2 v[P];
-    in.get(l, s, 0, v);
-    if (RES) {
-      f32x2 r[P];
-      in.get(l, s, RES ? 1 : 0, r);
-#pragma unroll
-      for (int k = 0; k < P; ++k) v[k] = add2(v[k], r[k]);
-    }
+    in.template get<false>(l, s, 0, v);
+    if (RES) in.template get<true>(l, s, RES ? 1 : 0, v);
     if (RAGGED) l.clear_outside(v);  // whole chunks outside the row read as zero
     const float mean = group_sum(sum_all<P>(v), bufs[group][0], group, nt, t) * inv_n;
     const f32x2 mean2 = splat(mean);
@@ -485,14 +507,9 @@ __global__ void __launch_bounds__(TMAX, ctas_per_sm(true, E, TMAX))
       rstd_n = __ldg(rstd_p);
     }
     f32x2 h[P], g[P];
-    in.get(l, s, 0, g);
-    in.get(l, s, 1, h);
-    if (RES) {
-      f32x2 r[P];
-      in.get(l, s, RES ? 2 : 0, r);
-#pragma unroll
-      for (int k = 0; k < P; ++k) h[k] = add2(h[k], r[k]);
-    }
+    in.template get<false>(l, s, 0, g);
+    in.template get<false>(l, s, 1, h);
+    if (RES) in.template get<true>(l, s, RES ? 2 : 0, h);
 #pragma unroll
     for (int k = 0; k < P; ++k) h[k] = mul2(sub2(h[k], mean), rstd);
     if (RAGGED) l.clear_outside(g);
@@ -661,16 +678,17 @@ struct Shape {
   size_t smem;
 };
 
-// Elements per thread: 8 up to 1024 columns, 16 beyond (fewer threads to
-// reduce over).  Beyond 8192 columns a CTA has more than 512 threads and the
-// backward's column sums move from registers to shared memory.  Rows per CTA: about 256
-// threads.  Grid: as many CTAs as shared memory and threads allow per SM, a
-// whole number of phases when rows are not whole chunks.  Ring: up to 3
-// stages, what fits.
+// Elements per thread: 8 up to 1024 columns, 16 beyond (fewer threads to reduce
+// over), in the forward 32 beyond 4096 (CTAs of at most 512 threads).  The
+// backward's column sums leave registers for 16 elements only: beyond 4096
+// columns it has one CTA of up to 1024 threads per SM, and beyond 8192 the sums
+// move to shared memory.  Rows per CTA: about 256 threads.  Grid: as many CTAs
+// as registers and shared memory hold, a whole number of phases when rows are
+// not whole chunks.  Ring: up to 3 stages, what fits.
 inline Shape shape(long long M, long long N, int esize, int tensors, bool bwd) {
   Shape s{};
   const int vw = 16 / esize;
-  s.e = N <= 1024 ? 8 : 16;
+  s.e = N <= 1024 ? 8 : N <= 4096 || bwd ? 16 : 32;
   s.ragged = N % vw != 0;
   const long long span = s.ragged ? N + vw - 1 : N;
   s.nt = (int)((span + 32LL * s.e - 1) / (32LL * s.e) * 32);
@@ -680,11 +698,13 @@ inline Shape shape(long long M, long long N, int esize, int tensors, bool bwd) {
   const int threads = s.nt * s.groups;
   // column sums: 1024-thread CTAs keep them here, several groups add them here
   const size_t acc = !bwd ? 0 : s.nt > 512 ? (size_t)2 * s.e * s.nt * 4 : s.groups > 1 ? (size_t)2 * N * 4 : 0;
-  const size_t stage = (size_t)tensors * s.e * esize * threads;  // at most 96 KB up to 512 threads
-  s.stages = s.nt > 512 ? 0 : (int)((kMaxSmem - acc) / stage);
+  const size_t stage = (size_t)tensors * s.e * esize * threads;  // at most 128 KB, with a ring
+  s.stages = bwd && s.nt > 512 ? 0 : (int)((kMaxSmem - acc) / stage);
   if (s.stages > 3) s.stages = 3;
   s.smem = acc + stage * s.stages;
-  int per_sm = ctas_per_sm(bwd, s.e, threads <= 256 ? 256 : 1024);
+  const int regs = ctas_per_sm(bwd, s.e, 256) == 3 ? 80 : threads > 512 ? 64 : 128;
+  int per_sm = 65536 / (regs * threads);
+  if (per_sm > 4) per_sm = 4;
   if (s.smem > 0 && per_sm > (int)(kMaxSmem / s.smem)) per_sm = (int)(kMaxSmem / s.smem);
   if (per_sm < 1) per_sm = 1;
   const long long want = (M + s.groups - 1) / s.groups;
@@ -738,9 +758,9 @@ int forward(const void* x, const void* res, const void* w, const void* b, int wf
   return res ? launch_fwd<T, E, true, TMAX>(s, x, res, w, b, wf, eps, y, mean, rstd, M, N, st) \
              : launch_fwd<T, E, false, TMAX>(s, x, res, w, b, wf, eps, y, mean, rstd, M, N, st)
   if (s.e == 8) PACKR_NORM_FWD(8, 256);
-  if (s.nt <= 256) PACKR_NORM_FWD(16, 256);
-  if (s.nt <= 512) PACKR_NORM_FWD(16, 512);
-  PACKR_NORM_FWD(16, 1024);
+  if (s.e == 16) PACKR_NORM_FWD(16, 256);
+  if (s.nt <= 256) PACKR_NORM_FWD(32, 256);
+  PACKR_NORM_FWD(32, 512);
 #undef PACKR_NORM_FWD
 }
 

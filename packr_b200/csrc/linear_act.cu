@@ -74,11 +74,49 @@ int decode(const uint8_t* W_p, const uint16_t* W_f, const float* lut, uint16_t* 
 // dz = dout * act'(z) for a slab of rows:
 //   hi[r, c] = bf16(dz), lo[r, c] = bf16(dz - hi) (optional; the difference is
 //   exact in f32), colsum[slab][c] = sum over the slab's rows of dz (optional).
-// A thread owns 8 columns and walks its slab's rows, two rows' loads in
-// flight; sums of different slabs are added in order by a second launch.
+// A thread owns 8 columns and walks its slab's rows; sums of different slabs
+// are added in order by a second launch.
 // hi == nullptr: only the column sums (a bf16 dout without activation is the
 // GEMMs' operand as it stands).
-constexpr int kDzUnroll = 2;
+// Bound by HBM (2 + 2 bytes in, 2 out per element with bf16): raw loads of
+// kDzUnroll rows are issued before the first is used.
+constexpr int kDzUnroll = 4;
+template <bool F32>
+struct DzRow {  // 8 elements as loaded
+  uint4 q[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* src, long long off, bool vec, int nc) {
+    if (vec) {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(src) + off * (F32 ? 4 : 2));
+#pragma unroll
+      for (int k = 0; k < (F32 ? 2 : 1); ++k) q[k] = __ldcs(p + k);
+    } else {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = j < nc ? __float_as_uint(load_io(src, off + j, F32)) : 0u;
+      if (F32) {
+        q[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        q[F32 ? 1 : 0] = make_uint4(w[4], w[5], w[6], w[7]);
+      } else {
+        q[0] = make_uint4(w[0] >> 16 | w[1], w[2] >> 16 | w[3], w[4] >> 16 | w[5], w[6] >> 16 | w[7]);
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float* v) const {
+    if (F32) {
+      const uint4 a = q[0], b = q[F32 ? 1 : 0];
+      v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+      v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+    } else {
+      const uint32_t w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      }
+    }
+  }
+};
+
 template <bool F32, int ACT>
 __global__ void __launch_bounds__(256) dz_kernel(const void* __restrict__ dout, const void* __restrict__ z, int M,
                                                  int N, int rows_per_slab, uint16_t* __restrict__ hi,
@@ -91,47 +129,41 @@ __global__ void __launch_bounds__(256) dz_kernel(const void* __restrict__ dout, 
   const int nc = (int)min(8ll, (long long)N - c0);
   const bool v8 = vec && nc == 8;
   float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  auto load = [&](const void* src, int r, float* v) {
-    const long long off = (long long)r * N + c0;
-    if (v8) {
-      prep::load8<F32>(src, off, v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < nc ? load_io(src, off + j, F32) : 0.0f;
-    }
-  };
-  auto emit = [&](int r, float* d) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] += d[j];
-    if (hi == nullptr) return;
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      h[j] = pack_bf16x2_rne(d[2 * j], d[2 * j + 1]);
-      l[j] = pack_bf16x2_rne(__fsub_rn(d[2 * j], __uint_as_float(h[j] << 16)),
-                             __fsub_rn(d[2 * j + 1], __uint_as_float(h[j] & 0xFFFF0000u)));
-    }
-    // ld is a multiple of 8: the padding of a ragged row is written as zero
-    *reinterpret_cast<uint4*>(hi + (long long)r * ld + c0) = make_uint4(h[0], h[1], h[2], h[3]);
-    if (lo != nullptr) *reinterpret_cast<uint4*>(lo + (long long)r * ld + c0) = make_uint4(l[0], l[1], l[2], l[3]);
-  };
   for (int r = r0; r < r1; r += kDzUnroll) {
-    float d[kDzUnroll][8], zz[kDzUnroll][8];
+    DzRow<F32> rd[kDzUnroll], rz[kDzUnroll];
 #pragma unroll
     for (int u = 0; u < kDzUnroll; ++u) {
       if (r + u < r1) {
-        load(dout, r + u, d[u]);
-        if (ACT != PACKR_ACT_NONE) load(z, r + u, zz[u]);
+        rd[u].load(dout, (long long)(r + u) * N + c0, v8, nc);
+        if (ACT != PACKR_ACT_NONE) rz[u].load(z, (long long)(r + u) * N + c0, v8, nc);
       }
     }
 #pragma unroll
     for (int u = 0; u < kDzUnroll; ++u) {
-      if (r + u < r1) {
-        if (ACT != PACKR_ACT_NONE) {
+      if (r + u >= r1) break;
+      float d[8];
+      rd[u].get(d);
+      if (ACT != PACKR_ACT_NONE) {
+        float zz[8];
+        rz[u].get(zz);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d[u][j] *= act::slope<ACT>(zz[u][j]);
-        }
-        emit(r + u, d[u]);
+        for (int j = 0; j < 8; ++j) d[j] *= act::slope<ACT>(zz[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] += d[j];
+      if (hi == nullptr) continue;
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = pack_bf16x2_rne(d[2 * j], d[2 * j + 1]);
+      // ld is a multiple of 8: the padding of a ragged row is written as zero
+      const long long o = (long long)(r + u) * ld + c0;
+      *reinterpret_cast<uint4*>(hi + o) = make_uint4(h[0], h[1], h[2], h[3]);
+      if (lo != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          l[j] = pack_bf16x2_rne(__fsub_rn(d[2 * j], __uint_as_float(h[j] << 16)),
+                                 __fsub_rn(d[2 * j + 1], __uint_as_float(h[j] & 0xFFFF0000u)));
+        *reinterpret_cast<uint4*>(lo + o) = make_uint4(l[0], l[1], l[2], l[3]);
       }
     }
   }

@@ -33,8 +33,9 @@ def _stream(device) -> ctypes.c_void_p:
 
 
 def _raw_stream(device) -> int:
-    """Handle of torch's current stream on `device`."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of torch's current stream on `device`, without building a
+    torch.cuda.Stream (several microseconds a call)."""
+    return _current_raw_stream(device.index)
 
 
 def _on_device(device):
@@ -45,6 +46,8 @@ def _on_device(device):
 
 
 _NO_SWITCH = contextlib.nullcontext()
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -57,6 +60,11 @@ def _dtype_code(t: torch.Tensor) -> int:
 
 def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def _addr(t) -> int | None:
+    """The tensor's address as a plain number (ctypes converts it), or None."""
+    return None if t is None else t.data_ptr()
 
 
 def _workspace(nbytes: int, device) -> torch.Tensor | None:
@@ -325,10 +333,10 @@ def linear_act_forward(x: torch.Tensor, W_p: torch.Tensor, W_f: torch.Tensor, lu
         nbytes = lib.packr_linear_act_workspace_bytes(M, K, N, xd, wp, wf)
         ws = _workspace(nbytes, dev)
         code = lib.packr_linear_act_forward(
-            x.data_ptr(), xd, wp, wf, lut.data_ptr(), None if bias is None else bias.data_ptr(),
-            _dtype_code(bias) if bias is not None else 0, activation, None if residual is None else residual.data_ptr(),
-            out.data_ptr(), None if z is None else z.data_ptr(), _dtype_code(out), M, K, N,
-            None if ws is None else ws.data_ptr(), nbytes, _raw_stream(dev))
+            x.data_ptr(), xd, wp, wf, lut.data_ptr(), _addr(bias),
+            _dtype_code(bias) if bias is not None else 0, activation, _addr(residual),
+            out.data_ptr(), _addr(z), _dtype_code(out), M, K, N,
+            _addr(ws), nbytes, _raw_stream(dev))
     _lib.check("packr_linear_act_forward", code)
     return out, z
 
@@ -359,12 +367,13 @@ def linear_act_backward(dout: torch.Tensor, z: torch.Tensor | None, activation: 
     xd = _dtype_code(x)
     flags = _lib.PACKR_BWD_DW_SPLIT if dw_split_for(x.dtype) else 0
     with _on_device(dev):
-        nbytes = lib.packr_linear_act_backward_workspace_bytes(M, K, N, xd, flags, _ptr(W_p), _ptr(W_f))
+        wp, wf = W_p.data_ptr(), W_f.data_ptr()
+        nbytes = lib.packr_linear_act_backward_workspace_bytes(M, K, N, xd, flags, wp, wf)
         ws = _workspace(nbytes, dev)
         code = lib.packr_linear_act_backward(
-            _ptr(dout), _ptr(z), _dtype_code(dout), activation, _ptr(x), xd, _ptr(W_p), _ptr(W_f), _ptr(lut),
-            _ptr(counts), _ptr(dX), _ptr(dW), _ptr(dlut), _ptr(dbias),
-            _dtype_code(dbias) if dbias is not None else 0, M, K, N, flags, _ptr(ws), nbytes, _stream(dev))
+            dout.data_ptr(), _addr(z), _dtype_code(dout), activation, x.data_ptr(), xd, wp, wf, lut.data_ptr(),
+            _addr(counts), _addr(dX), _addr(dW), _addr(dlut), _addr(dbias),
+            _dtype_code(dbias) if dbias is not None else 0, M, K, N, flags, _addr(ws), nbytes, _raw_stream(dev))
     _lib.check("packr_linear_act_backward", code)
     return dX, dW, dlut, dbias
 

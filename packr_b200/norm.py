@@ -18,37 +18,33 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernel import _on_device, _raw_stream
+from .kernel import _addr, _on_device, _raw_stream
 
 _F32, _BF16 = torch.float32, torch.bfloat16
 _CODE = {_F32: _lib.PACKR_DTYPE_F32, _BF16: _lib.PACKR_DTYPE_BF16}
 
 
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
 def layer_norm_forward(x, weight, bias, eps, residual=None, stats=False):
-    """(y, mean, rstd) of a contiguous [..., N] x; mean and rstd are f32 [M]
-    with `stats`, else None.  Arguments as packr_layer_norm checks them."""
+    """(y, s) of a contiguous [..., N] x; with `stats` s is f32 [2, M], the rows'
+    means and reciprocal standard deviations, else None.  Arguments as
+    packr_layer_norm checks them."""
     lib = _lib.load()
     n = x.shape[-1]
     m = x.numel() // n
     y = torch.empty_like(x)
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty(2, m, dtype=_F32, device=x.device).unbind(0)
+    s = torch.empty((2, m), dtype=_F32, device=x.device) if stats else None
+    mean = _addr(s)
     w = weight if weight is not None else bias
     with _on_device(x.device):
         code = lib.packr_layer_norm_forward(
             x.data_ptr(), _addr(residual), _CODE[x.dtype], _addr(weight), _addr(bias),
-            _CODE[w.dtype] if w is not None else 0, eps, y.data_ptr(), _addr(mean), _addr(rstd), m, n,
+            _CODE[w.dtype] if w is not None else 0, eps, y.data_ptr(), mean, None if s is None else mean + 4 * m, m, n,
             _raw_stream(x.device))
     _lib.check("packr_layer_norm_forward", code)
-    return y, mean, rstd
+    return y, s
 
 
-def layer_norm_backward(dy, x, weight, mean, rstd, residual=None, w_dtype=_F32, need_dx=True, need_dweight=True,
+def layer_norm_backward(dy, x, weight, stats, residual=None, w_dtype=_F32, need_dx=True, need_dweight=True,
                         need_dbias=True):
     """(dx, dweight, dbias); entries not requested are None.  dx is also the
     residual's gradient."""
@@ -64,7 +60,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd, residual=None, w_dtype=_F32, 
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         code = lib.packr_layer_norm_backward(
             dy.data_ptr(), x.data_ptr(), _addr(residual), _CODE[x.dtype], _addr(weight), _CODE[w_dtype],
-            mean.data_ptr(), rstd.data_ptr(), _addr(dx), _addr(dw), _addr(db), m, n, _addr(ws), nbytes,
+            stats.data_ptr(), stats.data_ptr() + 4 * m, _addr(dx), _addr(dw), _addr(db), m, n, _addr(ws), nbytes,
             _raw_stream(dev))
     _lib.check("packr_layer_norm_backward", code)
     return dx, dw, db
@@ -73,20 +69,19 @@ def layer_norm_backward(dy, x, weight, mean, rstd, residual=None, w_dtype=_F32, 
 class PackRLayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, residual):
-        y, mean, rstd = layer_norm_forward(x, weight, bias, eps, residual, stats=True)
-        ctx.save_for_backward(x, weight, residual, mean, rstd)
+        y, stats = layer_norm_forward(x, weight, bias, eps, residual, stats=True)
+        ctx.save_for_backward(x, weight, residual, stats)
         ctx.w_dtype = (weight if weight is not None else bias).dtype if weight is not None or bias is not None else _F32
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, residual, mean, rstd = ctx.saved_tensors
+        x, weight, residual, stats = ctx.saved_tensors
         nx, nw, nb, _, nr = ctx.needs_input_grad
         if dy.dtype != x.dtype:
             dy = dy.to(x.dtype)
-        dx, dw, db = layer_norm_backward(dy.contiguous(), x, weight, mean, rstd, residual, ctx.w_dtype, nx or nr, nw,
-                                         nb)
+        dx, dw, db = layer_norm_backward(dy.contiguous(), x, weight, stats, residual, ctx.w_dtype, nx or nr, nw, nb)
         return dx if nx else None, dw, db, None, dx if nr else None
 
 
