@@ -142,15 +142,15 @@ enum BSrc { B_RING = 0, B_WTMA = 1, B_PLAIN = 2 };
 // B stage feeds two pair MMAs (two 256-row subtiles), halving the decode and
 // lut traffic per FLOP; the two subtiles' accumulators then fill TMEM (no
 // double buffering across tiles, but each subtile is released separately).
-// EPI: the forward with bias, activation and residual in its epilogue, io type
-// bf16 (1) or f32 (2); 0: the others.
+// EPI (0: none).  FWD: bias, activation and residual in the epilogue, io type
+// bf16 (1) or f32 (2).  DW: no lut gradient, so no histogram (1).
 template <int MODE, int BSRC, int MSUB, int EPI = 0>
 struct Cfg {
   static constexpr bool kDecode = MODE != DW && BSRC != B_PLAIN;
   static constexpr bool kWtma = kDecode && BSRC == B_WTMA;
   static constexpr bool kPlainB = MODE != DW && BSRC == B_PLAIN;  // FWD / DX with B by TMA
   static constexpr int kMSub = MSUB;
-  static constexpr int kStages = kWtma ? (MSUB == 2 ? 3 : 4) : (kPlainB && MSUB == 2 ? 4 : (MODE == DW ? 4 : 6));
+  static constexpr int kStages = kWtma ? (MSUB == 2 ? 3 : 4) : ((kPlainB || EPI) && MSUB == 2 ? 4 : (MODE == DW && !EPI ? 4 : 6));
   static constexpr int kABytes = MSUB * A_BYTES;            // A subtiles per stage
   static constexpr int kWpBytes = kWtma ? BN_CTA * BK : 0;  // u8 W_p tile per stage
   static constexpr int kStageBytes = kABytes + B_BYTES + kWpBytes;
@@ -169,6 +169,8 @@ struct Cfg {
   // GEMMs only (for DW the split-tile fix-up measured slower than the wave
   // quantisation it removes)
   static constexpr bool kStreamK = kPlainB;
+  // whole tiles from a launch-wide counter
+  static constexpr bool kDyn = kPlainB || EPI;
   static constexpr int kStgBytes = kStageOut ? kEpiWarps * (EPI ? 2048 : 4096) : 0;
   static constexpr int kChunksPerEpiWarp = (BN / 32) / (kEpiWarps / 4);
   static constexpr int kDecWarp0 = 2 + kEpiWarps;             // first decode warp
@@ -178,7 +180,7 @@ struct Cfg {
   static constexpr int kThreads = kWarps * 32;
   static constexpr bool kAmn = MODE == DW;   // A stored MN-major in smem
   static constexpr bool kBmn = MODE != DX;   // B stored MN-major in smem
-  static constexpr int kHistBytes = HIST_COPIES * HIST_COPY_BYTES + HIST_SUM_BYTES + HIST_XCHG_BYTES;
+  static constexpr int kHistBytes = EPI ? 0 : HIST_COPIES * HIST_COPY_BYTES + HIST_SUM_BYTES + HIST_XCHG_BYTES;
   static constexpr int kLutBytes = kDecode ? LUT_BYTES : 0;
   static constexpr int kStgOff = MODE == DW ? kHistBytes : kLutBytes;  // staging buffers in the aux region
   static constexpr int kAuxBytes = kStgOff + kStgBytes;
@@ -547,6 +549,35 @@ __device__ __forceinline__ void store_rows_staged(uint32_t stg, const float* v, 
   __syncwarp();
 }
 
+// As store_rows_staged<2> for rows that are not whole 16-byte chunks: two rows
+// per step, a lane writes two neighbouring elements of its row.
+__device__ __forceinline__ void store_rows_ragged(uint32_t stg, const uint32_t* h, uint16_t* out, int r0, int m_limit,
+                                                  long long ld, int gn0, int nval) {
+  const int lane = threadIdx.x & 31, sw = (lane >> 1) & 3;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stg + (uint32_t)(lane * 64 + ((j ^ sw) << 4))),
+                 "r"(h[4 * j]), "r"(h[4 * j + 1]), "r"(h[4 * j + 2]), "r"(h[4 * j + 3])
+                 : "memory");
+  __syncwarp();
+  const int w = lane & 15;
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const int r = 2 * i + (lane >> 4);
+    uint32_t d;
+    asm volatile("ld.shared.b32 %0, [%1];"
+                 : "=r"(d)
+                 : "r"(stg + (uint32_t)(r * 64 + (((w >> 2) ^ ((r >> 1) & 3)) << 4) + (w & 3) * 4))
+                 : "memory");
+    if (r0 + r < m_limit) {
+      uint16_t* o = out + (long long)(r0 + r) * ld + gn0 + 2 * w;
+      if (2 * w < nval) o[0] = (uint16_t)d;
+      if (2 * w + 1 < nval) o[1] = (uint16_t)(d >> 16);
+    }
+  }
+  __syncwarp();
+}
+
 // The fused epilogue of one warp's 32 x 16 block.  The accumulator (lane l:
 // row l) goes through the warp's 2 KB staging buffer and comes back with 4 consecutive columns per lane, 8 rows per
 // step, so that the lane's bias stays in registers over the rows and the
@@ -707,11 +738,11 @@ template <int MODE, int BSRC, int MSUB, int EPI = 0>
 __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
     packr_gemm_kernel(const Params P, const __grid_constant__ Maps maps) {
   using C = Cfg<MODE, BSRC, MSUB, EPI>;
-  static_assert(EPI == 0 || (MODE == FWD && C::kPlainB), "the fused epilogue belongs to the plain forward");
+  static_assert(EPI == 0 || MODE == DW || (MODE == FWD && C::kPlainB), "the fused epilogue belongs to the plain forward");
   static_assert(EPI == 0 || C::kEpiWarps == 16, "four warps per TMEM quarter, 64 columns each");
   constexpr int STAGES = C::kStages;
   static_assert(C::kSmemBytes <= 227 * 1024, "shared memory per CTA");
-  static_assert(MODE != DW || MSUB == 1, "the DW epilogue's histogram runs per 256-row tile");
+  static_assert(MODE != DW || MSUB == 1 || EPI != 0, "the DW epilogue's histogram runs per 256-row tile");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // 1024-byte aligned base for the 128-byte-swizzled tiles; offsetting the
   // __shared__ array keeps the compiler emitting shared-memory accesses.
@@ -760,7 +791,7 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
       prefetch_tmap(&maps.wp);
     }
   }
-  if (MODE == DW && warp >= 2 && warp < C::kDecWarp0) {
+  if (MODE == DW && EPI == 0 && warp >= 2 && warp < C::kDecWarp0) {
     uint32_t* hist = reinterpret_cast<uint32_t*>(sAux);
     for (int i = threadIdx.x - 64; i < C::kHistBytes / 4; i += C::kEpiWarps * 32) hist[i] = 0u;
   }
@@ -782,7 +813,7 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
 
   // Dynamic tiles (one thread per role).  Entry i of the pair's sequence sits
   // in queue slot i % TILE_Q, phase (i / TILE_Q) & 1.
-  const bool dyn = C::kPlainB && P.dyn != 0;
+  const bool dyn = C::kDyn && P.dyn != 0;
   // the even CTA's producer: takes the next tile (-1 past the last) and
   // publishes it to both CTAs; -2 if the kernel aborted
   auto q_push = [&](int i) -> int {
@@ -890,8 +921,11 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
           const uint32_t fbar = mapa(smem_u32(&bars->full[s]), 0);
           uint8_t* a_dst = sA + s * C::kABytes;
           if (MODE == DW) {
-            tma_load_2d_pair(a_dst, &maps.a[seg], fbar, m0, k0);
-            tma_load_2d_pair(a_dst + 8192, &maps.a[seg], fbar, m0 + 64, k0);
+#pragma unroll
+            for (int sub = 0; sub < MSUB; ++sub) {
+              tma_load_2d_pair(a_dst + sub * A_BYTES, &maps.a[seg], fbar, m0 + sub * 2 * BM, k0);
+              tma_load_2d_pair(a_dst + sub * A_BYTES + 8192, &maps.a[seg], fbar, m0 + sub * 2 * BM + 64, k0);
+            }
             uint8_t* b_dst = sB + s * B_BYTES;
             tma_load_2d_pair(b_dst, &maps.b[seg], fbar, n0, k0);
             tma_load_2d_pair(b_dst + 8192, &maps.b[seg], fbar, n0 + 64, k0);
@@ -1021,14 +1055,14 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
           const uint32_t aph = MSUB == 1 ? ((uint32_t)(t_local >> 1) & 1u) : ((uint32_t)t_local & 1u);
           // this warp's 32 rows of the subtile
           const int r0 = (u.tile % P.m_tiles) * (2 * BM * MSUB) + sub * 2 * BM + (int)rank * BM + q * 32;
-          if (P.epi.residual != nullptr && r0 + lane < P.Mg && n0 < P.Ng)  // towards L2 while the MMAs run
+          if (MODE == FWD && P.epi.residual != nullptr && r0 + lane < P.Mg && n0 < P.Ng)  // towards L2 while the MMAs run
             asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(P.epi.residual) +
                                                           ((long long)(r0 + lane) * P.ld_out + n0) * (EPI == 2 ? 4 : 2)));
           if (!mbar_wait_warp(&bars->tfull[acc], aph, abort_flag, kEpilogueSleepNs)) {
             alive = false;
             break;
           }
-          if (u.kind == 2 && sub == 0) {  // stream-K tail: wait for every following pair's head partial
+          if (C::kStreamK && u.kind == 2 && sub == 0) {  // stream-K tail: wait for every following pair's head partial
             const long long tile_end = (long long)(u.tile + 1) * kb_total;
             for (int q2 = pair + 1; alive && q2 < npairs && sk_start(P, q2, npairs) < tile_end; ++q2) {
               alive = wait_flag(P.sk_flags + (q2 * 2 + (int)rank) * C::kEpiWarps + ew, abort_flag);
@@ -1046,6 +1080,22 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(acc ? tempty1 : tempty0);
+          if constexpr (MODE == DW) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int gn0 = n0 + c * 32, nval = min(32, P.Ng - gn0);
+              if (nval <= 0 || r0 >= P.Mg) continue;
+              uint32_t h[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                h[j] = pack_bf16x2_rne(__uint_as_float(v[32 * c + 2 * j]), __uint_as_float(v[32 * c + 2 * j + 1]));
+              if (nval == 32 && (P.ld_out & 7) == 0 && P.out_vec)
+                store_rows_staged<2>(stg, reinterpret_cast<const float*>(h), P.out, r0, P.Mg, P.ld_out, gn0);
+              else
+                store_rows_ragged(stg, h, static_cast<uint16_t*>(P.out), r0, P.Mg, P.ld_out, gn0, nval);
+            }
+            continue;
+          }
           // stream-K partials [col][row], coalesced along rows
           const long long slot0 = (((long long)pair * MSUB + sub) * 2 + rank) * (BN * BM) + (ew >> 2) * 64 * BM + row;
           if (u.kind == 1) {
@@ -1539,6 +1589,17 @@ int make_map_u8(CUtensorMap* m, const void* base, long long inner, long long row
   return r == CUDA_SUCCESS ? PACKR_OK : PACKR_ERR_INVALID_ARGUMENT;
 }
 
+// Whether splitting the last, partly filled wave of `rem` tiles over all pairs
+// pays for the fused linear layer: it saves the idle pairs' share of a tile's
+// k-blocks (0.38 us each per 256-row subtile) and costs the flags' clearing,
+// the partials' way through L2 and the waits, together about 20 us.  Measured
+// (forward, decode included): 777 x 1000 -> 1111 40 us split, 28 whole; 300 x
+// 1024 -> 4096 36 and 26; 130 x 4096 -> 4096 54 and 52; 257 x 11008 -> 4096 100
+// and 118.
+inline bool split_pays(int rem, int pairs, long long kblocks, int msub) {
+  return kblocks * msub * (pairs - rem) >= 64LL * pairs;
+}
+
 template <int MODE, int BSRC, int MSUB = 1, int EPI = 0>
 int launch_impl(Params P, const Maps& maps, cudaStream_t stream) {
   using C = Cfg<MODE, BSRC, MSUB, EPI>;
@@ -1583,8 +1644,8 @@ int launch_impl(Params P, const Maps& maps, cudaStream_t stream) {
   // tile's share spanning several pairs whose partials its first pair adds
   // (measured: the plain forward and dX at 256 rows, 16-43 tiles of the
   // Llama FFN layers, otherwise leave most SMs idle).
-  const bool sk_all = C::kStreamK && PACKR_STREAM_K && P.sk_partial != nullptr && P.sk_flags != nullptr &&
-                      tiles < max_pairs && max_pairs > 1 && max_pairs <= P.sk_slots && kbt >= 2 &&
+  const bool sk_all = C::kStreamK && PACKR_STREAM_K && (EPI == 0 || split_pays(tiles % max_pairs, max_pairs, kbt, MSUB)) &&
+                      P.sk_partial != nullptr && P.sk_flags != nullptr && tiles < max_pairs && max_pairs > 1 && max_pairs <= P.sk_slots && kbt >= 2 &&
                       (long long)tiles * kbt >= max_pairs;  // every pair a non-empty range (it publishes a flag)
   const int pairs = sk_all ? max_pairs : (tiles < max_pairs ? tiles : max_pairs);
   cfg.gridDim = dim3(2 * pairs, 1, 1);
@@ -1605,7 +1666,8 @@ int launch_impl(Params P, const Maps& maps, cudaStream_t stream) {
     // pair.
     const int waves = tiles / pairs, rem = tiles % pairs;
     P.sk_dp_tiles = waves >= 2 ? (waves - 1) * pairs : 0;
-    if (waves >= 1 && rem != 0 && rem * 100 <= pairs * PACKR_SK_LAST_WAVE_PCT &&
+    if (waves >= 1 && rem != 0 && (EPI == 0 || split_pays(rem, pairs, kbt, MSUB)) &&
+        rem * 100 <= pairs * PACKR_SK_LAST_WAVE_PCT &&
         (long long)(tiles - P.sk_dp_tiles) * kbt / pairs >= kbt) {
       P.sk = 1;
       if (cudaMemsetAsync(P.sk_flags, 0, (size_t)pairs * 2 * C::kEpiWarps * sizeof(int), stream) != cudaSuccess)
@@ -1616,7 +1678,7 @@ int launch_impl(Params P, const Maps& maps, cudaStream_t stream) {
   // is the first word of the stream-K flags, unused then)
   P.dyn = 0;
   P.tile_counter = nullptr;
-  if (C::kPlainB && PACKR_DYN_TILES && !P.sk && P.sk_flags != nullptr && tiles > pairs) {
+  if (C::kDyn && PACKR_DYN_TILES && !P.sk && P.sk_flags != nullptr && tiles > pairs) {
     P.dyn = 1;
     P.tile_counter = P.sk_flags;
     if (cudaMemsetAsync(P.tile_counter, 0, sizeof(int), stream) != cudaSuccess) return PACKR_ERR_CUDA;
@@ -1671,6 +1733,17 @@ int launch_plain(Params P, const Maps& maps, cudaStream_t stream) {
   P.k_blocks = (P.Kg + BK - 1) / BK;
   if (P.Mg >= PACKR_PLAIN_MSUB2_MIN_M) return launch_impl<MODE, B_PLAIN, 2>(P, maps, stream);
   return launch_impl<MODE, B_PLAIN, 1>(P, maps, stream);
+}
+
+// dW without the lut gradient: P.sk_flags (nullable) one word for the tile
+// counter.  512-row tiles when there are waves of them and a long reduction.
+int launch_dw_plain(Params P, const Maps& maps, cudaStream_t stream) {
+  P.out_vec = aligned(P.out, 16);
+  P.n_tiles = (P.Ng + BN - 1) / BN;
+  P.k_blocks = (P.Kg + BK - 1) / BK;
+  if ((long long)((P.Mg + 511) / 512) * P.n_tiles >= sm_count() && P.Kg >= PACKR_PLAIN_MSUB2_MIN_M)
+    return launch_impl<DW, B_RING, 2, 1>(P, maps, stream);
+  return launch_impl<DW, B_RING, 1, 1>(P, maps, stream);
 }
 
 // Subtiles of the fused forward's tiles.

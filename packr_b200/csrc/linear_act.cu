@@ -245,7 +245,7 @@ size_t plan_forward(Carve& c, Fwd& p, Route r, long long M, long long K, long lo
 struct Bwd {
   uint16_t *dh, *dl, *xh, *xl, *wd;
   float *part, *skp, *colsum, *dlut_sum;
-  int* skf;
+  int *skf, *tiles;
   int32_t* counts;
 };
 
@@ -268,12 +268,45 @@ size_t plan_backward(Carve& c, Bwd& p, long long M, long long K, long long N, in
   p.colsum = dbias ? c.take<float>((size_t)dz_plan(M, N).slabs * N) : nullptr;
   p.dlut_sum = dlut ? c.take<float>(256) : nullptr;
   p.counts = dlut && !have_counts ? c.take<int32_t>(256) : nullptr;
+  p.tiles = dw ? c.take<int>(1) : nullptr;
   return c.off;
 }
 
 inline bool act_ok(int a) { return a >= PACKR_ACT_NONE && a <= PACKR_ACT_SILU; }
 inline bool io_ok(int d) { return d == PACKR_DTYPE_F32 || d == PACKR_DTYPE_BF16; }
 inline size_t io_size(int d) { return d == PACKR_DTYPE_F32 ? 4 : 2; }
+
+// x [M, K] -> hi = bf16(x) and, for the split dW, lo = bf16(x - hi), rows padded
+// to a multiple of 8 with zeros.  One thread per 8 consecutive elements of a
+// row, any row length and alignment.
+__global__ void __launch_bounds__(256) operand_kernel(const void* __restrict__ x, int f32, long long M, int K,
+                                                      int chunks_per_row, int vec, uint4* __restrict__ hi,
+                                                      uint4* __restrict__ lo) {
+  const long long total = M * chunks_per_row;
+  for (long long c = (long long)blockIdx.x * 256 + threadIdx.x; c < total; c += (long long)gridDim.x * 256) {
+    const long long r = c / chunks_per_row;
+    const int k0 = (int)(c - r * chunks_per_row) * 8;
+    const long long off = r * K + k0;
+    float v[8];
+    if (vec) {  // f32 rows of whole chunks
+      const float4 a = __ldcs(reinterpret_cast<const float4*>(static_cast<const float*>(x) + off));
+      const float4 b = __ldcs(reinterpret_cast<const float4*>(static_cast<const float*>(x) + off) + 1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = k0 + j < K ? load_io(x, off + j, f32) : 0.0f;
+    }
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      h[j] = pack_bf16x2_rne(v[2 * j], v[2 * j + 1]);
+      l[j] = pack_bf16x2_rne(__fsub_rn(v[2 * j], __uint_as_float(h[j] << 16)),
+                             __fsub_rn(v[2 * j + 1], __uint_as_float(h[j] & 0xFFFF0000u)));
+    }
+    hi[c] = make_uint4(h[0], h[1], h[2], h[3]);
+    if (lo != nullptr) lo[c] = make_uint4(l[0], l[1], l[2], l[3]);
+  }
+}
 
 // x as the GEMMs' bf16 operand (a copy in xh, with its residual part in xl,
 // when its type or row length needs one).
@@ -284,15 +317,12 @@ int operand_x(const void* x, int x_dtype, long long M, long long K, uint16_t* xh
   if (xh == nullptr) return PACKR_OK;
   *a = xh;
   *lda = round8(K);
-  // grid.y of the copy holds 65535 blocks of 32 rows
-  for (long long r = 0; r < M; r += 65535LL * prep::kRowsPerCta) {
-    const long long n = M - r < 65535LL * prep::kRowsPerCta ? M - r : 65535LL * prep::kRowsPerCta;
-    const char* src = static_cast<const char*>(x) + (size_t)(r * K) * io_size(x_dtype);
-    int st = prep::split_rows(src, x_dtype == PACKR_DTYPE_F32, K, n, K, xh + r * round8(K),
-                              xl ? xl + r * round8(K) : nullptr, round8(K), nullptr, s);
-    if (st != PACKR_OK) return st;
-  }
-  return PACKR_OK;
+  const int cpr = (int)(round8(K) / 8), f32 = x_dtype == PACKR_DTYPE_F32;
+  const long long blocks = (M * cpr + 255) / 256, cap = 16LL * sm_count();
+  operand_kernel<<<(int)(blocks < cap ? blocks : cap), 256, 0, s>>>(x, f32, M, (int)K, cpr, f32 && (K & 7) == 0 && aligned(x, 16),
+                                                                   reinterpret_cast<uint4*>(xh),
+                                                                   reinterpret_cast<uint4*>(xl));
+  return launch_status();
 }
 
 }  // namespace linear_act
@@ -447,7 +477,10 @@ extern "C" int packr_linear_act_backward(const void* dout, const void* z, int ou
     P.out_f32 = x_dtype == PACKR_DTYPE_F32;
     P.sk_partial = p.skp;
     P.sk_flags = p.skf;
-    P.sk_slots = linear::sk_pairs();
+    // no split of a short reduction (gemm::split_pays)
+    const int msub = linear::plain_msub(M), pairs = linear::sk_pairs();
+    const long long tiles = ((M + 256LL * msub - 1) / (256 * msub)) * ((K + 255) / 256);
+    P.sk_slots = gemm::split_pays((int)(tiles % pairs), pairs, (N + 63) / 64, msub) ? pairs : 0;
     if ((st = gemm::launch_plain<gemm::DX>(P, maps, s)) != PACKR_OK) return st;
   }
   if (dw || dl) {
@@ -476,7 +509,13 @@ extern "C" int packr_linear_act_backward(const void* dout, const void* z, int ou
     P.ld_out = N;
     P.hist_idx = dl ? W_p : nullptr;
     P.dlut_sum = p.dlut_sum;
-    if ((st = gemm::launch<gemm::DW>(P, maps, s)) != PACKR_OK) return st;
+    if (!dl) {
+      P.sk_flags = p.tiles;
+      st = gemm::launch_dw_plain(P, maps, s);
+    } else {
+      st = gemm::launch<gemm::DW>(P, maps, s);
+    }
+    if (st != PACKR_OK) return st;
   }
   if (dl) {
     const int32_t* counts = lut_counts;
