@@ -531,7 +531,7 @@ def bench_bert(args, world, rank, peaks, peak_kind):
     from packr_b200.cuda_adam import CUDA8BitAdam
     from packr_b200.dp import ShardedAdam8
     dev = torch.device("cuda", torch.cuda.current_device())
-    model = wl.bert_classifier(dev, seed=0)
+    model = wl.bert_classifier(dev, seed=0, fused=args.fused)
     model.train()
     params = [p for p in model.parameters() if p.requires_grad]
     n_params = sum(p.numel() for p in params)
@@ -570,7 +570,8 @@ def bench_bert(args, world, rank, peaks, peak_kind):
         "ms_per_step": round(ms_step, 4), "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
         "dtype": "fp32 model, bf16 W_f operands", "data": "synthetic (random ids, 2-class labels)",
         "config": {"workload": "bert: BERT-base (12 x 768, FFN 3072, 12 heads, vocab 30522), FFN layers as "
-                               "PackRLinear (compress_model, layer_scope='ffn'), batch 32 x seq 128 per GPU",
+                               "PackRLinear (compress_model, layer_scope='ffn'), batch 32 x seq 128 per GPU"
+                               + (", fused epilogues and norms" if args.fused else ""),
                    "params": n_params, "packr_layers": len(layers),
                    "optimizer": "CUDA8BitAdam" if world == 1 else "ShardedAdam8 (ZeRO-1, overlapped reduce-scatter)",
                    "parallelism": f"dp{world}"},
@@ -1158,6 +1159,8 @@ def main():
     ap.add_argument("--timeline", default=None,
                     help="ffn: after the timed steps, write rank 0's CUPTI timeline of 3 more steps "
                          "(every kernel and copy: start, duration, stream) to this JSON file")
+    ap.add_argument("--fused", action="store_true",
+                    help="bert: activations in the packed layers' epilogues, residual sums in the norms' kernels")
     ap.add_argument("--profile-once", action="store_true",
                     help="ffn: run each kernel of one gate-layer step once (for ncu captures), print nothing")
     args = ap.parse_args()

@@ -14,7 +14,7 @@ from .kernel import packr_matmul
 from .autograd import PackRMatmulFunction, PackRLinearFunction, PackRLinearActFunction, packr_linear_act
 from .norm import PackRLayerNorm, PackRLayerNormFunction, packr_layer_norm
 from .layer import PackRLinear
-from .layer_patcher import compress_model
+from .layer_patcher import PackRAddNorm, compress_model, fuse_epilogues
 from .config import PackRConfig, SchemeType
 from .optim import FusedQuantizedAdam
 from .cuda_adam import CUDA8BitAdam
@@ -31,6 +31,7 @@ CV2LRTController = VelvetController
 __all__ = [
     "PackRConfig", "PackRLinear", "PackRMatmulFunction", "PackRLinearFunction", "packr_matmul", "compress_model",
     "PackRLinearActFunction", "packr_linear_act", "PackRLayerNorm", "PackRLayerNormFunction", "packr_layer_norm",
+    "PackRAddNorm", "fuse_epilogues",
     "SchemeType", "FusedQuantizedAdam", "CUDA8BitAdam", "VelvetController", "OffloadManager",
     "PHRConfig", "PHRLinear", "PHRMatmulFunction", "phr_matmul", "CV2LRTController",
 ]

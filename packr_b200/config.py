@@ -4,7 +4,8 @@ Same fields and defaults.  In this build `offload` and mode "zpackr" are not
 available (host offload is unnecessary at B200 memory sizes and the zpackr
 modules are not part of the reference tree); `compress_model` reports them.
 `use_8bit_optimizer` / `optimizer_type` are advisory, as in the reference:
-the caller constructs the optimizer.
+the caller constructs the optimizer.  `fuse_epilogues` is this build's own:
+compress_model then also runs fuse_epilogues (layer_patcher.py).
 """
 from dataclasses import dataclass
 from typing import Literal
@@ -28,6 +29,7 @@ class PackRConfig:
     optimizer_type: Literal["triton8", "cuda8", "adamw"] = "triton8"
     gradient_mix: float = 0.5
     grad_ema_beta: float = 0.9967
+    fuse_epilogues: bool = False
 
 
 # Legacy alias

@@ -9,13 +9,19 @@ and `from_linear`.  forward() flattens 3-D input as the reference does
 (layer.py:79-81, 99-100); the bias add of layer.py:96-97 is fused into the
 GEMM epilogue, and the lut bin counts used by the lut gradient are cached per
 layer (W_p is frozen) instead of recounted every backward.
+
+Beyond the reference, `layer.activation`, `layer.out_dtype` and
+forward(x, residual=...) put an activation, a residual sum and the output's
+rounding into the same GEMM epilogue (packr_linear_act); at their defaults the
+layer is the reference's.
 """
 from __future__ import annotations
 
 import torch
 import torch.nn as nn
 
-from .autograd import PackRLinearFunction
+from . import _lib
+from .autograd import PackRLinearFunction, packr_linear_act
 from . import kernel as _k
 
 
@@ -30,10 +36,23 @@ def _build_codebook() -> torch.Tensor:
 
 
 class PackRLinear(nn.Module):
-    """PackR linear layer with learnable LUT: out = x @ (W_f + lut[W_p]) + bias."""
+    """PackR linear layer with learnable LUT: out = act(x @ (W_f + lut[W_p]) + bias) + residual.
 
-    def __init__(self, in_features, out_features, bias=True):
+    activation: None, "relu", "gelu", "gelu_tanh" or "silu"; out_dtype: float32
+    (the reference's) or bfloat16.  Both may be set at any time."""
+
+    activation = None
+    out_dtype = torch.float32
+
+    def __init__(self, in_features, out_features, bias=True, activation=None, out_dtype=torch.float32):
         super().__init__()
+        if activation is not None and activation not in _lib.ACTIVATIONS:
+            raise ValueError(f"PackRLinear: activation must be None or one of {sorted(_lib.ACTIVATIONS)}, "
+                             f"not {activation!r}")
+        if activation is not None:
+            self.activation = activation
+        if out_dtype != torch.float32:
+            self.out_dtype = out_dtype
         self.in_features = in_features
         self.out_features = out_features
         self.W_p = nn.Parameter(torch.randint(0, 256, (in_features, out_features), dtype=torch.uint8),
@@ -61,9 +80,14 @@ class PackRLinear(nn.Module):
             self._counts_key = key
         return self._counts
 
-    def forward(self, x):
+    def forward(self, x, residual=None):
         if not (x.is_cuda and self.W_p.is_cuda):
             raise RuntimeError("PackRLinear runs on CUDA tensors only (no CPU path in the B200 build)")
+        if residual is not None or self.activation not in (None, "none") or self.out_dtype != torch.float32:
+            if x.dtype not in (torch.bfloat16, torch.float32):
+                x = x.float()
+            return packr_linear_act(x, self.W_p, self.W_f, self.lut, self.bias_f, self.activation, residual,
+                                    self.out_dtype, self.lut_counts() if self.lut.requires_grad else None)
         orig_shape = x.shape
         if x.dim() == 3:
             x = x.reshape(-1, x.shape[-1])
@@ -74,7 +98,9 @@ class PackRLinear(nn.Module):
         return out
 
     def extra_repr(self):
-        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias_f is not None}"
+        return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias_f is not None}"
+                + (f", activation={self.activation}" if self.activation is not None else "")
+                + (f", out_dtype={self.out_dtype}" if self.out_dtype != torch.float32 else ""))
 
     @classmethod
     def from_linear(cls, module: nn.Linear):

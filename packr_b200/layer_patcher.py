@@ -1,13 +1,18 @@
 """compress_model — replace nn.Linear layers by PackRLinear
-(reference packr/layer_patcher.py:9-130, same name-based scope rules)."""
+(reference packr/layer_patcher.py:9-130, same name-based scope rules) — and
+fuse_epilogues, which moves what a model computes around its packed layers
+(activation, residual sum, layer norm) into their kernels."""
 from __future__ import annotations
 
 import warnings
 
+import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from .config import PackRConfig
 from .layer import PackRLinear
+from .norm import PackRLayerNorm
 
 
 def compress_model(model: nn.Module, config: PackRConfig = None):
@@ -29,6 +34,8 @@ def compress_model(model: nn.Module, config: PackRConfig = None):
         else:
             _replace_module(model, name, packr)
         packr_layers.append((name, packr))
+    if config.fuse_epilogues:
+        fuse_epilogues(model)
     if config.gradient_checkpointing:
         _enable_gradient_checkpointing(model)
     if config.offload and packr_layers:
@@ -77,3 +84,75 @@ def _enable_gradient_checkpointing(model: nn.Module):
         model.gradient_checkpointing_enable()
     except AttributeError:
         pass
+
+
+# (layer, activation) attribute pairs of transformer feed-forward blocks whose
+# forward applies the activation to the layer's output and to nothing else
+_ACTIVATED = [("dense", "intermediate_act_fn"), ("gate_proj", "act_fn"), ("fc1", "activation_fn"),
+              ("dense_h_to_4h", "act")]
+_ACTIVATION_CLASSES = {"ReLU": "relu", "SiLU": "silu", "SiLUActivation": "silu", "GELUActivation": "gelu",
+                       "NewGELUActivation": "gelu_tanh", "GELUTanh": "gelu_tanh", "PytorchGELUTanh": "gelu_tanh"}
+_ACTIVATION_FUNCTIONS = {F.relu: "relu", torch.relu: "relu", F.gelu: "gelu", F.silu: "silu"}
+
+
+# blocks whose forward is LayerNorm(dropout(dense(hidden_states)) + input_tensor)
+_ADD_NORM_CLASSES = {a + b for a in ("Bert", "Roberta", "Electra") for b in ("Output", "SelfOutput")}
+
+
+def _activation_name(fn):
+    """packr_linear_act's name of an activation module or function, or None."""
+    if isinstance(fn, nn.GELU):
+        return {"none": "gelu", "tanh": "gelu_tanh"}.get(fn.approximate)
+    if isinstance(fn, nn.Module):
+        return _ACTIVATION_CLASSES.get(type(fn).__name__)
+    try:
+        return _ACTIVATION_FUNCTIONS.get(fn)
+    except TypeError:  # not hashable
+        return None
+
+
+class PackRAddNorm(nn.Module):
+    """LayerNorm(dropout(dense(x)) + residual), the close of a post-norm block,
+    with the sum taken inside the norm's kernel.  Takes over the submodules of
+    the block it replaces under their names, so state dicts keep their keys."""
+
+    def __init__(self, dense, LayerNorm, dropout=None):
+        super().__init__()
+        self.dense = dense
+        self.LayerNorm = PackRLayerNorm.from_layer_norm(LayerNorm)
+        self.dropout = dropout if dropout is not None else nn.Identity()
+
+    def forward(self, hidden_states, input_tensor):
+        h = self.dropout(self.dense(hidden_states))
+        return self.LayerNorm(h, residual=input_tensor.to(h.dtype))
+
+
+def fuse_epilogues(model: nn.Module):
+    """Fuses what surrounds the packed layers of `model`, in place:
+
+    * an activation that follows a PackRLinear (BERT's dense +
+      intermediate_act_fn, a gated MLP's gate_proj + act_fn, fc1 +
+      activation_fn, dense_h_to_4h + act) becomes the layer's `activation`;
+    * blocks that add their input before a layer norm (BERT's BertOutput and
+      BertSelfOutput, and their Roberta and Electra twins) become PackRAddNorm.
+
+    Activations other than relu, gelu (either form) and silu stay as they are.
+    Parameters, their names and the model's results (up to rounding) do not
+    change.  Returns the model."""
+    for name, module in list(model.named_modules()):
+        for layer, act in _ACTIVATED:
+            lin = getattr(module, layer, None)
+            known = _activation_name(getattr(module, act, None))
+            if isinstance(lin, PackRLinear) and lin.activation is None and known is not None:
+                lin.activation = known
+                if act in module._modules:
+                    module._modules[act] = nn.Identity()
+                else:
+                    setattr(module, act, nn.Identity())
+        if type(module).__name__ in _ADD_NORM_CLASSES and name:
+            norm = getattr(module, "LayerNorm", None)
+            if type(norm) is nn.LayerNorm and len(norm.normalized_shape) == 1:
+                fused = PackRAddNorm(module.dense, norm, module.dropout)
+                fused.train(module.training)
+                _replace_module(model, name, fused)
+    return model

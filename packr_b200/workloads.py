@@ -11,7 +11,7 @@ import torch.nn as nn
 
 from .config import PackRConfig
 from .layer import PackRLinear
-from .layer_patcher import compress_model
+from .layer_patcher import compress_model, fuse_epilogues
 
 BERT_BASE = dict(vocab_size=30522, hidden_size=768, num_hidden_layers=12, num_attention_heads=12,
                  intermediate_size=3072)
@@ -19,14 +19,16 @@ LLAMA3_8B = dict(vocab_size=128256, hidden_size=4096, intermediate_size=14336, n
                  num_attention_heads=32, num_key_value_heads=8)
 
 
-def bert_classifier(device, layers: int = 12, seed: int = 0, **overrides):
+def bert_classifier(device, layers: int = 12, seed: int = 0, fused: bool = False, **overrides):
     """BertForSequenceClassification (2 labels, fp32) with its FFN Linear
-    layers compressed by compress_model(layer_scope="ffn") (from_linear)."""
+    layers compressed by compress_model(layer_scope="ffn") (from_linear).
+    fused: gelu in the packed layers' epilogue, residual sums in the norms'
+    kernels (PackRConfig.fuse_epilogues)."""
     from transformers import BertConfig, BertForSequenceClassification
     torch.manual_seed(seed)
     cfg = BertConfig(**{**BERT_BASE, "num_hidden_layers": layers, **overrides}, num_labels=2)
     model = BertForSequenceClassification(cfg).to(device)
-    compress_model(model, PackRConfig(layer_scope="ffn"))
+    compress_model(model, PackRConfig(layer_scope="ffn", fuse_epilogues=fused))
     return model
 
 
@@ -50,11 +52,12 @@ class _Cast(nn.Module):
         return self.inner(x).to(self.dtype)
 
 
-def llama_decoder(device, layers: int = 32, seed: int = 0, dtype=torch.bfloat16, **overrides):
+def llama_decoder(device, layers: int = 32, seed: int = 0, dtype=torch.bfloat16, fused: bool = False, **overrides):
     """LlamaForCausalLM (Llama-3-8B shapes by default) in bf16 with every
     Linear, lm_head included, replaced by a synthetic-init PackRLinear (W_p
     uniform, sorted N(0, 0.02 sqrt(768/K)) lut, N(0, 0.002 sqrt(768/K)) W_f)
-    whose output is cast back to bf16."""
+    whose output is cast back to bf16.  fused: the packed layers write bf16
+    themselves, and the gate projections apply the silu."""
     from transformers import LlamaConfig, LlamaForCausalLM
     torch.manual_seed(seed)
     cfg = LlamaConfig(**{**LLAMA3_8B, "num_hidden_layers": layers, **overrides})
@@ -74,8 +77,12 @@ def llama_decoder(device, layers: int = 32, seed: int = 0, dtype=torch.bfloat16,
                                    lut_std=0.02 * (768 / lin.in_features) ** 0.5,
                                    wf_std=0.002 * (768 / lin.in_features) ** 0.5)
         parent, _, leaf = name.rpartition(".")
-        setattr(model.get_submodule(parent) if parent else model, leaf, _Cast(pk, dtype))
+        if fused:
+            pk.out_dtype = dtype
+        setattr(model.get_submodule(parent) if parent else model, leaf, pk if fused else _Cast(pk, dtype))
         del lin
+    if fused:
+        fuse_epilogues(model)
     if device != "cpu":
         torch.cuda.empty_cache()
     return model

@@ -1,0 +1,129 @@
+"""The fused operators as a model runs them: a feed-forward block of two packed
+layers and a norm against its 64-bit form, transformers' BERT and Llama with
+fused epilogues against the same models without."""
+import pytest
+import torch
+
+import packr_b200 as packr
+from fused_reference import act64, weights64
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def rel(a, b):
+    return float((a.detach().double() - b.double()).norm() / b.double().norm())
+
+
+@pytest.mark.parametrize("M", [1, 3, 40, 300])
+@pytest.mark.parametrize("prenorm", [False, True])
+def test_feed_forward_block(cuda, M, prenorm):
+    """h = down(gelu(up(x))); post-norm: norm(h + x); pre-norm: norm first, then
+    h + x in the down projection's epilogue.  bf16 throughout.
+
+    Every stored bf16 tensor on the way costs at most 2^-8 / sqrt(3) = 2.3e-3 of
+    its 2-norm; the longest path (forward to the upstream gradient's way back:
+    up, down, norm, dz twice, dx twice) has eight, and a factor 2 covers the
+    norm's and the activation's slopes: 2 * sqrt(8) * 2.3e-3 = 1.3e-2."""
+    K, H = 192, 512
+    up = packr.PackRLinear.synthetic(K, H, seed=1, lut_std=0.05, wf_std=0.005)
+    down = packr.PackRLinear.synthetic(H, K, seed=2, lut_std=0.05, wf_std=0.005)
+    for lin in (up, down):
+        lin.out_dtype = BF16
+        lin.lut.requires_grad_(False)
+        torch.nn.init.normal_(lin.bias_f, std=0.2)
+    up.activation = "gelu"
+    norm = packr.PackRLayerNorm(K, dtype=BF16, device="cuda")
+    torch.nn.init.normal_(norm.weight, 1.0, 0.1)
+    torch.nn.init.normal_(norm.bias, 0.0, 0.1)
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = torch.randn(M, K, generator=g, device="cuda").bfloat16().requires_grad_(True)
+    dy = torch.randn(M, K, generator=g, device="cuda").bfloat16()
+    params = [up.W_f, up.bias_f, down.W_f, down.bias_f, norm.weight, norm.bias]
+    y = down(up(norm(x)), residual=x) if prenorm else norm(down(up(x)), residual=x)
+    got = torch.autograd.grad(y, [x] + params, dy)
+
+    d = lambda t: t.detach().double().requires_grad_(True)  # noqa: E731
+    x64, b1, b2, nw, nb = d(x), d(up.bias_f), d(down.bias_f), d(norm.weight), d(norm.bias)
+    w1 = weights64(up.W_p, up.W_f, up.lut).requires_grad_(True)
+    w2 = weights64(down.W_p, down.W_f, down.lut).requires_grad_(True)
+
+    def ln(s):
+        c = s - s.mean(1, keepdim=True)
+        return c / torch.sqrt((c * c).mean(1, keepdim=True) + 1e-5) * nw + nb
+
+    ffn = lambda t: act64(t @ w1 + b1, "gelu") @ w2 + b2  # noqa: E731
+    ref = ffn(ln(x64)) + x64 if prenorm else ln(ffn(x64) + x64)
+    want = torch.autograd.grad(ref, [x64, w1, b1, w2, b2, nw, nb], dy.double())
+    assert rel(y, ref.detach()) < 1.3e-2
+    for name, a, b in zip(("x", "W_f up", "bias up", "W_f down", "bias down", "norm weight", "norm bias"), got, want):
+        assert rel(a, b) < 1.3e-2, name
+
+
+def test_bert_with_fused_epilogues(cuda):
+    """Same logits and gradients as the unfused model up to rounding: f32
+    activations, bf16 operands in both (a rounding that falls the other way
+    moves an operand by 2^-8 of itself)."""
+    from packr_b200 import workloads as wl
+    models = [wl.bert_classifier(cuda, layers=2, seed=0, fused=f).eval() for f in (False, True)]
+    assert sum(isinstance(m, packr.PackRAddNorm) for m in models[1].modules()) == 4
+    models[1].load_state_dict(models[0].state_dict())
+    ids, labels = wl.bert_batch(cuda, batch=4, seq=32)
+    outs = []
+    for m in models:
+        out = m(input_ids=ids, labels=labels)
+        out.loss.backward()
+        outs.append(out)
+    assert rel(outs[1].logits, outs[0].logits.detach()) < 2e-2
+    grads = [dict(m.named_parameters()) for m in models]
+    for name, p in grads[0].items():
+        if p.grad is not None and float(p.grad.norm()) > 1e-6:
+            assert rel(grads[1][name].grad, p.grad) < 5e-2, name
+    models[1].train()  # dropout between the layer and the norm
+    models[1](input_ids=ids, labels=labels).loss.backward()
+
+
+def test_llama_with_fused_epilogues(cuda):
+    from packr_b200 import workloads as wl
+    sizes = dict(hidden_size=256, intermediate_size=512, num_attention_heads=4, num_key_value_heads=2, vocab_size=1024)
+    models = [wl.llama_decoder("cuda", layers=2, seed=0, fused=f, **sizes).eval() for f in (False, True)]
+    gates = [m for n, m in models[1].named_modules() if n.endswith("gate_proj")]
+    assert gates and all(g.activation == "silu" and g.out_dtype == BF16 for g in gates)
+    ids = wl.llama_batch("cuda", seq=64, vocab=1024)
+    outs = [m(input_ids=ids, labels=ids) for m in models]
+    for o in outs:
+        o.loss.backward()
+    assert rel(outs[1].logits, outs[0].logits.detach()) < 2e-2
+    for (n, p), (_, q) in zip(models[0].named_parameters(), ((n.replace(".inner", ""), p) for n, p in models[1].named_parameters())):
+        if p.grad is not None and float(p.grad.float().norm()) > 1e-6:
+            assert rel(q.grad, p.grad) < 6e-2, n
+
+
+def test_training_step_with_the_8_bit_optimizer(cuda):
+    """The gradients of fused layers reach CUDA8BitAdam as the plain ones do."""
+    from packr_b200.cuda_adam import CUDA8BitAdam
+    up = packr.PackRLinear.synthetic(128, 256, seed=1)
+    up.activation = "silu"
+    norm = packr.PackRLayerNorm(256, device="cuda")
+    params = [p for m in (up, norm) for p in m.parameters() if p.requires_grad]
+    opt = CUDA8BitAdam(params, lr=1e-3)
+    x = torch.randn(64, 128, device="cuda")
+    before = [p.detach().clone() for p in params]
+    norm(up(x)).square().mul(torch.randn(64, 256, device="cuda")).sum().backward()
+    opt.step()
+    assert all(torch.isfinite(p).all() and not torch.equal(p, b) for p, b in zip(params, before))
+
+
+def test_layer_attributes_change_the_route_only(cuda):
+    lin = packr.PackRLinear.synthetic(96, 160, seed=3)
+    x = torch.randn(2, 9, 96, device="cuda").bfloat16()
+    plain = lin(x)
+    assert plain.dtype == F32 and plain.shape == (2, 9, 160)
+    r = torch.randn(2, 9, 160, device="cuda")
+    assert torch.allclose(lin(x, residual=r), plain + r, rtol=1e-5, atol=1e-5)
+    lin.activation = "relu"
+    assert torch.allclose(lin(x), plain.clamp_min(0), rtol=1e-5, atol=1e-5)
+    lin.activation, lin.out_dtype = None, BF16
+    assert torch.allclose(lin(x).float(), plain, rtol=2.0 ** -8, atol=1e-5)
+    assert torch.equal(lin(x.half()), lin(x.half().float()))

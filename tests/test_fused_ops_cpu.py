@@ -131,3 +131,70 @@ def test_reference_norm_and_linear_follow_torch():
     got = linear64(xb, W_p, W_f, lut, bias, "gelu", None, torch.float32, dout)
     for k, v in (("out", out), ("dx", dx), ("dW_f", dw)):
         assert torch.allclose(got[k][0], v, rtol=1e-10, atol=1e-12), k
+
+
+def _bert_block():
+    from transformers import BertConfig
+    from transformers.models.bert.modeling_bert import BertLayer
+    cfg = BertConfig(hidden_size=32, num_attention_heads=2, intermediate_size=64, hidden_act="gelu")
+    cfg._attn_implementation = "eager"
+    block = torch.nn.ModuleDict({"layer": BertLayer(cfg)})
+    layer = block["layer"]
+    for parent, name in ((layer.intermediate, "dense"), (layer.output, "dense")):
+        lin = getattr(parent, name)
+        setattr(parent, name, packr.PackRLinear(lin.in_features, lin.out_features))
+    return block
+
+
+def test_fuse_epilogues_rewires_a_bert_layer():
+    block = _bert_block().eval()
+    keys = list(block.state_dict())
+    norms = {n: p for n, p in block.named_parameters()}
+    assert packr.fuse_epilogues(block) is block
+    layer = block["layer"]
+    assert layer.intermediate.dense.activation == "gelu"
+    assert isinstance(layer.intermediate.intermediate_act_fn, torch.nn.Identity)
+    for m in (layer.output, layer.attention.output):
+        assert isinstance(m, packr.PackRAddNorm) and isinstance(m.LayerNorm, packr.PackRLayerNorm) and not m.training
+    assert list(block.state_dict()) == keys
+    assert all(p is norms[n] for n, p in block.named_parameters())
+    packr.fuse_epilogues(block)  # a second run changes nothing
+    assert layer.intermediate.dense.activation == "gelu"
+
+
+@pytest.mark.parametrize("fn,name", [
+    (torch.nn.GELU(), "gelu"), (torch.nn.GELU(approximate="tanh"), "gelu_tanh"), (torch.nn.ReLU(), "relu"),
+    (torch.nn.SiLU(), "silu"), (torch.nn.functional.gelu, "gelu"), (torch.relu, "relu"), (torch.nn.Tanh(), None),
+    (torch.nn.ReLU6(), None), (lambda z: z, None), (None, None)])
+def test_which_activations_are_fused(fn, name):
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.gate_proj = packr.PackRLinear(8, 16, bias=False)
+            self.act_fn = fn
+
+    b = Block()
+    packr.fuse_epilogues(b)
+    assert b.gate_proj.activation == name
+    assert isinstance(b.act_fn, torch.nn.Identity) == (name is not None)
+
+
+def test_plain_linears_keep_their_activation():
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.fc1 = torch.nn.Linear(8, 16)
+            self.activation_fn = torch.nn.ReLU()
+
+    b = Block()
+    packr.fuse_epilogues(b)
+    assert isinstance(b.activation_fn, torch.nn.ReLU)
+
+
+def test_layer_takes_known_activations():
+    assert packr.PackRLinear(4, 8).activation is None
+    assert packr.PackRLinear(4, 8, activation="silu", out_dtype=torch.bfloat16).extra_repr().endswith(
+        "activation=silu, out_dtype=torch.bfloat16")
+    with pytest.raises(ValueError):
+        packr.PackRLinear(4, 8, activation="tanh")
+    assert packr.PackRConfig().fuse_epilogues is False

@@ -243,3 +243,33 @@ def test_gradient_against_differences(cuda):
             num = (f(1e-5) - f(-1e-5)) / 2e-5
             terms = got["d" + k].double() * v
             assert abs(float(terms.sum()) - num) <= 2.0 ** -7 * float(terms.norm()) * 4 + 1e-5 * (1 + abs(num)), (act, k)
+
+
+@pytest.mark.parametrize("K,N", [(4096, 4864), (4100, 4720), (4104, 4723)])
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_weight_gradient_of_large_layers(cuda, K, N, act):
+    """Enough 512 x 256 tiles and tokens for the held-accumulator dW kernels,
+    with the lut gradient (act none) and without; edges inside a tile."""
+    c = case(1030, K, N, BF16, BF16, seed=K, residual=False, bias=None)
+    need = ("x", "W_f", "lut") if act == "none" else ("W_f",)
+    got = grads(c, act, BF16, need=need)
+    compare(c, got, act, BF16)
+    if act == "none":
+        only = grads(c, act, BF16, need=("lut",))["dlut"]
+        assert torch.allclose(only, got["dlut"], rtol=1e-4, atol=1e-6 * float(got["dlut"].abs().max()))
+
+
+def test_weight_gradient_with_non_finite_and_zero_tiles(cuda):
+    """The integer histogram's fallbacks: a tile of zeros adds nothing, a tile
+    with an infinity adds its values as they are."""
+    c = case(1024, 4096, 4864, BF16, BF16, seed=1, residual=False, bias=None)
+    c["dout"][:, :256] = 0
+    got = grads(c, "none", BF16, need=("W_f", "lut"))
+    assert not got["dW_f"][:, :256].any()
+    compare(c, got, "none", BF16)
+    c["W_p"].fill_(7)
+    c["W_p"][5, 300] = 200
+    c["x"][3, 5] = float("inf")
+    got = grads(c, "none", BF16, need=("W_f", "lut"))
+    assert not torch.isfinite(got["dlut"][7]) and not torch.isfinite(got["dlut"][200])
+    assert not got["dlut"][:7].any() and not got["dlut"][8:200].any() and not got["dlut"][201:].any()
