@@ -228,8 +228,8 @@ int packr_predecode_route(int64_t M, int64_t K, int64_t N, const uint8_t* W_p, c
  * the query's size.  The reference runs packr_matmul, then torch kernels for
  * the bias, activation and residual (packr/layer.py:96-97 and the host
  * model's own). */
-size_t packr_linear_act_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, const uint8_t* W_p,
-                                        const uint16_t* W_f);
+size_t packr_linear_act_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, int out_dtype,
+                                        const uint8_t* W_p, const uint16_t* W_f);
 int packr_linear_act_forward(const void* x, int x_dtype, const uint8_t* W_p, const uint16_t* W_f, const float* lut,
                              const void* bias, int bias_dtype, int activation, const void* residual, void* out,
                              void* z, int out_dtype, int64_t M, int64_t K, int64_t N, void* workspace,

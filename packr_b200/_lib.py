@@ -71,7 +71,7 @@ SIGNATURES = {
     "packr_backward_decoded": (_I32, [_VP, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64,
                                       _I64, _I32, _VP, _SZ, _VP]),
     "packr_predecode_route": (_I32, [_I64, _I64, _I64, _VP, _VP]),
-    "packr_linear_act_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32, _VP, _VP]),
+    "packr_linear_act_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32, _I32, _VP, _VP]),
     "packr_linear_act_forward": (_I32, [_VP, _I32, _VP, _VP, _VP, _VP, _I32, _I32, _VP, _VP, _VP, _I32, _I64, _I64,
                                         _I64, _VP, _SZ, _VP]),
     "packr_linear_act_backward_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32, _I32, _VP, _VP]),

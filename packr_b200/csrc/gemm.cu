@@ -71,6 +71,8 @@ constexpr int BN_CTA = 128;      // B columns held by each CTA
 constexpr int BK = 64, UK = 16;
 constexpr int MAX_STAGES = 6;
 constexpr int TILE_Q = 4;        // dynamic-tile queue slots
+constexpr int kSegBlocks = 32;   // k-blocks of one accumulator of an f32 output (2048 elements)
+constexpr int kMore = 4;         // Unit::kind flag
 constexpr int BARS_BYTES = 512;  // shared memory reserved for struct Bars
 constexpr int A_BYTES = BM * BK * 2;      // 16 KB
 constexpr int B_BYTES = BN_CTA * BK * 2;  // 16 KB
@@ -842,16 +844,33 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
   // schedules too: the even CTA's producer alone walks the schedule, so that
   // the epilogue warps, which hold accumulators in registers, carry none of its
   // state.  False past the last unit or on an abort.
+  // An f32 output takes its reduction in segments of kSegBlocks k-blocks: the
+  // tensor cores truncate each f32 accumulation, which adds up to 1e-9 of the
+  // result per reduction element, one way (measured 4.2e-6 at 4096, 1.1e-5 at
+  // 11008), so the segments' accumulators are added by the epilogue instead,
+  // rounded to nearest.  kMore marks a unit whose sum goes on in the next.
+  Unit rest{-1, 0, 0, 0};  // (producer) what is left of a segmented unit
   auto unit_push = [&](int i, Sched& sc, Unit& x) -> bool {
     const int slot = i % TILE_Q;
     const uint32_t ph = (uint32_t)(i / TILE_Q) & 1u;
     if (!mbar_wait_cluster(&bars->qempty[slot], ph ^ 1u, abort_flag)) return false;
     bool more;
-    if (dyn) {
+    if (EPI == 2 && rest.k0 < rest.k1) {
+      x = rest;
+      more = true;
+    } else if (dyn) {
       x = Unit{atomicAdd(P.tile_counter, 1), 0, kb_total, 0};
       more = x.tile < num_tiles;
     } else {
       more = next_unit(sc, x);
+    }
+    if (EPI == 2 && more) {
+      rest = x;
+      rest.k0 = x.k1;
+      if (x.k1 - x.k0 > kSegBlocks) {
+        x.k1 = rest.k0 = x.k0 + kSegBlocks;
+        x.kind |= kMore;
+      }
     }
     if (!more) x.tile = -1;
     bars->qtile[slot] = x.tile;
@@ -1039,7 +1058,8 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
       const uint32_t stg = smem_u32(sAux) + (uint32_t)(C::kStgOff + ew * 2048);
       const uint32_t tempty0 = mapa(smem_u32(&bars->tempty[0]), 0);
       const uint32_t tempty1 = mapa(smem_u32(&bars->tempty[1]), 0);
-      bool alive = true;
+      bool alive = true, carried = false;
+      uint32_t v[64];  // the warp's accumulator, with what earlier segments left (carried)
       for (int t_local = 0; alive; ++t_local) {
         // lane 0 reads the queue, every lane gets the same answer
         Unit u{-1, 0, 0, 0};
@@ -1047,6 +1067,8 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
         u.tile = __shfl_sync(0xFFFFFFFFu, u.tile, 0);
         u.kind = __shfl_sync(0xFFFFFFFFu, u.kind, 0);
         if (u.tile < 0) break;
+        const bool more = EPI == 2 && MODE == FWD && (u.kind & kMore) != 0;
+        u.kind &= ~kMore;
         const int n0 = (u.tile / P.m_tiles) * BN + (ew >> 2) * 64;
         int n_heads = 0;
 #pragma unroll 1
@@ -1062,7 +1084,7 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
             alive = false;
             break;
           }
-          if (C::kStreamK && u.kind == 2 && sub == 0) {  // stream-K tail: wait for every following pair's head partial
+          if (C::kStreamK && u.kind == 2 && !more && sub == 0) {  // stream-K tail: wait for every following pair's head partial
             const long long tile_end = (long long)(u.tile + 1) * kb_total;
             for (int q2 = pair + 1; alive && q2 < npairs && sk_start(P, q2, npairs) < tile_end; ++q2) {
               alive = wait_flag(P.sk_flags + (q2 * 2 + (int)rank) * C::kEpiWarps + ew, abort_flag);
@@ -1071,15 +1093,27 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
             if (!alive) break;
           }
           tc_fence_after();
-          uint32_t v[64];
+          const uint32_t t_acc = tmem_base + (uint32_t)(acc * ACC_COLS + (ew >> 2) * 64) + ((uint32_t)(q * 32) << 16);
+          if (EPI == 2 && MODE == FWD && carried) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-            tmem_ld_32x32b_x32(tmem_base + (uint32_t)(acc * ACC_COLS + (ew >> 2) * 64 + c * 32) + ((uint32_t)(q * 32) << 16),
-                               *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
-          tmem_ld_wait();
+            for (int c = 0; c < 4; ++c) {
+              uint32_t w[16];
+              tmem_ld_32x32b_x16(t_acc + c * 16, w);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                v[16 * c + j] = __float_as_uint(__fadd_rn(__uint_as_float(v[16 * c + j]), __uint_as_float(w[j])));
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_acc + c * 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
+            tmem_ld_wait();
+          }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(acc ? tempty1 : tempty0);
+          carried = more;
+          if (more) continue;
           if constexpr (MODE == DW) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -1119,7 +1153,7 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
             for (int j = 0; j < 48; ++j) v[j] = v[j + 16];
           }
         }
-        if (alive && u.kind == 1) {  // publish this warp's part of the head partial
+        if (alive && u.kind == 1 && !more) {  // publish this warp's part of the head partial
           __threadfence();
           __syncwarp();
           if (lane == 0) {
@@ -1553,6 +1587,22 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+// Runs a tensor-map encoding.  It is a driver call and needs a context current
+// on this thread, which the runtime binds at a thread's first runtime call: a
+// host thread whose first CUDA work is this call (the autograd engine's, when
+// no copy or memset comes before the GEMM) has none yet, so a failed encoding
+// is repeated once after cudaSetDevice has bound it.
+template <class F>
+int encode_bound(F encode) {
+  if (encode() == CUDA_SUCCESS) return PACKR_OK;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) {
+    cudaGetLastError();
+    return PACKR_ERR_CUDA;
+  }
+  return encode() == CUDA_SUCCESS ? PACKR_OK : PACKR_ERR_INVALID_ARGUMENT;
+}
+
 // bf16 2-D map over [rows, inner] with the given row stride, 128-byte swizzle,
 // box {64, box_rows}.  Out-of-range elements read as zero.
 int make_map(CUtensorMap* m, const void* base, long long inner, long long rows, long long row_stride_bytes,
@@ -1565,10 +1615,11 @@ int make_map(CUtensorMap* m, const void* base, long long inner, long long rows, 
   cuuint64_t strides[1] = {(cuuint64_t)row_stride_bytes};
   cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1u, 1u};
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? PACKR_OK : PACKR_ERR_INVALID_ARGUMENT;
+  return encode_bound([&] {
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 // u8 2-D map over [rows, inner] (row stride in bytes), no swizzle, box
@@ -1583,10 +1634,11 @@ int make_map_u8(CUtensorMap* m, const void* base, long long inner, long long row
   cuuint64_t strides[1] = {(cuuint64_t)row_stride_bytes};
   cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1u, 1u};
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? PACKR_OK : PACKR_ERR_INVALID_ARGUMENT;
+  return encode_bound([&] {
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 // Whether splitting the last, partly filled wave of `rem` tiles over all pairs
@@ -1746,23 +1798,25 @@ int launch_dw_plain(Params P, const Maps& maps, cudaStream_t stream) {
   return launch_impl<DW, B_RING, 1, 1>(P, maps, stream);
 }
 
-// Subtiles of the fused forward's tiles.
+// Subtiles of the fused forward's tiles: 512 rows (half the traffic of W's tiles)
+// for a bf16 output with a long reduction, otherwise 256, whose second
+// accumulator takes the next tile or, for an f32 output, the next segment.
+// Measured at 4096 rows: 4096 -> 11008 311 us with 512, 339 with 256; 768 -> 2048
+// 66 and 46.
 #ifndef PACKR_EPI_MSUB2_MIN_K
 #define PACKR_EPI_MSUB2_MIN_K 2048
 #endif
-inline int epi_msub(long long M, long long K) {
-  return M >= PACKR_PLAIN_MSUB2_MIN_M && K >= PACKR_EPI_MSUB2_MIN_K ? 2 : 1;
+inline int epi_msub(long long M, long long K, int io_f32) {
+  return !io_f32 && M >= PACKR_PLAIN_MSUB2_MIN_M && K >= PACKR_EPI_MSUB2_MIN_K ? 2 : 1;
 }
 
 // The plain forward with the fused epilogue P.epi.
 int launch_plain_epi(Params P, const Maps& maps, cudaStream_t stream) {
   P.n_tiles = (P.Ng + BN - 1) / BN;
   P.k_blocks = (P.Kg + BK - 1) / BK;
-  if (epi_msub(P.Mg, P.Kg) == 2)
-    return P.epi.io_f32 ? launch_impl<FWD, B_PLAIN, 2, 2>(P, maps, stream)
-                        : launch_impl<FWD, B_PLAIN, 2, 1>(P, maps, stream);
-  return P.epi.io_f32 ? launch_impl<FWD, B_PLAIN, 1, 2>(P, maps, stream)
-                      : launch_impl<FWD, B_PLAIN, 1, 1>(P, maps, stream);
+  if (P.epi.io_f32) return launch_impl<FWD, B_PLAIN, 1, 2>(P, maps, stream);
+  if (epi_msub(P.Mg, P.Kg, 0) == 2) return launch_impl<FWD, B_PLAIN, 2, 1>(P, maps, stream);
+  return launch_impl<FWD, B_PLAIN, 1, 1>(P, maps, stream);
 }
 
 }  // namespace gemm

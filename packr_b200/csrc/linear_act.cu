@@ -228,15 +228,15 @@ struct Fwd {
   int* skf;
 };
 
-size_t plan_forward(Carve& c, Fwd& p, Route r, long long M, long long K, long long N, int x_dtype) {
+size_t plan_forward(Carve& c, Fwd& p, Route r, long long M, long long K, long long N, int x_dtype, int io_f32) {
   p = Fwd{};
   if (r == GEMV) return 0;
   p.xh = linear::x_needs_copy(x_dtype, K) ? c.take<uint16_t>((size_t)M * round8(K)) : nullptr;
   if (r == SKINNY) {
-    p.part = c.take<float>(gemm::skinny_partial_bytes(M, K, N) / sizeof(float));
+    p.part = c.take<float>(gemm::skinny_partial_bytes(M, K, N, io_f32 ? gemm::kSegBlocks : 0) / sizeof(float));
   } else {
     p.wd = c.take<uint16_t>((size_t)K * round8(N));
-    p.skp = c.take<float>(gemm::sk_partial_bytes(linear::sk_pairs(), gemm::epi_msub(M, K)) / sizeof(float));
+    p.skp = c.take<float>(gemm::sk_partial_bytes(linear::sk_pairs(), gemm::epi_msub(M, K, io_f32)) / sizeof(float));
     p.skf = c.take<int>(gemm::sk_flag_bytes(linear::sk_pairs(), 16) / sizeof(int));
   }
   return c.off;
@@ -328,13 +328,14 @@ int operand_x(const void* x, int x_dtype, long long M, long long K, uint16_t* xh
 }  // namespace linear_act
 }  // namespace packr
 
-extern "C" size_t packr_linear_act_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, const uint8_t* W_p,
-                                                   const uint16_t* W_f) {
+extern "C" size_t packr_linear_act_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, int out_dtype,
+                                                   const uint8_t* W_p, const uint16_t* W_f) {
   using namespace packr;
   if (M <= 0 || K <= 0 || N <= 0) return 0;
   linear::Carve c{nullptr};
   linear_act::Fwd p;
-  return linear_act::plan_forward(c, p, linear_act::route(M, K, N, W_p, W_f), M, K, N, x_dtype);
+  return linear_act::plan_forward(c, p, linear_act::route(M, K, N, W_p, W_f), M, K, N, x_dtype,
+                                  out_dtype == PACKR_DTYPE_F32);
 }
 
 extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_t* W_p, const uint16_t* W_f,
@@ -358,7 +359,7 @@ extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_
   const Route r = route(M, K, N, W_p, W_f);
   Carve c{static_cast<uint8_t*>(workspace)};
   Fwd p;
-  const size_t need = linear_act::plan_forward(c, p, r, M, K, N, x_dtype);
+  const size_t need = linear_act::plan_forward(c, p, r, M, K, N, x_dtype, out_dtype == PACKR_DTYPE_F32);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, linear::kAlign)))
     return PACKR_ERR_WORKSPACE;
   Epilogue e{};

@@ -265,8 +265,9 @@ struct SkPlan {
 
 // Reduction splits (R = reduction length, Out = output features): the fewest
 // waves of units over the resident CTAs (one per SM), each unit at least 4
-// k-blocks, the partial sums at most 1/8 of W's bytes.
-inline SkPlan skinny_plan(long long M, long long R, long long Out) {
+// k-blocks, the partial sums at most 1/8 of W's bytes.  max_per > 0: at most so
+// many k-blocks per split (kSegBlocks for an f32 output, see there).
+inline SkPlan skinny_plan(long long M, long long R, long long Out, int max_per = 0) {
   SkPlan p{};
   p.npad = skinny_npad(M);
   p.n_tiles = (int)((Out + BN_CTA - 1) / BN_CTA);
@@ -276,9 +277,11 @@ inline SkPlan skinny_plan(long long M, long long R, long long Out) {
   const long long cap_k = p.k_blocks / 4 > 0 ? p.k_blocks / 4 : 1;
   if (cap > cap_k) cap = cap_k;
   if (cap < 1) cap = 1;
+  const long long least = max_per > 0 ? (p.k_blocks + max_per - 1) / max_per : 1;
+  if (cap < least) cap = least;
   double best = 1e30;
   p.splits = 1;
-  for (long long s = 1; s <= cap; ++s) {
+  for (long long s = least; s <= cap; ++s) {
     const long long per = (p.k_blocks + s - 1) / s;
     const long long units = (long long)p.n_tiles * s;
     const long long waves = (units + sms - 1) / sms;
@@ -295,8 +298,8 @@ inline SkPlan skinny_plan(long long M, long long R, long long Out) {
   return p;
 }
 
-inline size_t skinny_partial_bytes(long long M, long long R, long long Out) {
-  const SkPlan p = skinny_plan(M, R, Out);
+inline size_t skinny_partial_bytes(long long M, long long R, long long Out, int max_per = 0) {
+  const SkPlan p = skinny_plan(M, R, Out, max_per);
   return (size_t)p.splits * M * Out * sizeof(float);
 }
 
@@ -321,10 +324,10 @@ int skinny_launch(const SkParams& P, const SkMaps& maps, int grid, cudaStream_t 
 // partial [splits][M][Out].
 template <int MODE>
 int skinny_run(const uint16_t* act_bf16, long long ld_act, const uint8_t* W_p, const uint16_t* W_f, const float* lut,
-               long long M, long long K, long long N, float* partial, SkPlan& pl, cudaStream_t st) {
+               long long M, long long K, long long N, float* partial, SkPlan& pl, cudaStream_t st, int max_per = 0) {
   const long long R = MODE == FWD ? K : N, Out = MODE == FWD ? N : K;
   if (M < 1 || M > 128) return PACKR_ERR_SHAPE;
-  pl = skinny_plan(M, R, Out);
+  pl = skinny_plan(M, R, Out, max_per);
   SkMaps maps;
   int rc = MODE == FWD ? make_map(&maps.wf, W_f, N, K, N * 2, BK) : make_map(&maps.wf, W_f, N, K, N * 2, BN_CTA);
   if (rc == PACKR_OK)
@@ -472,7 +475,7 @@ int skinny_forward_epi(const uint16_t* x_bf16, long long ldx, const uint8_t* W_p
                        const float* lut, const void* bias, int bias_f32, const Epilogue& epi, long long M, long long K,
                        long long N, float* partial, cudaStream_t st) {
   SkPlan pl;
-  int rc = skinny_run<FWD>(x_bf16, ldx, W_p, W_f, lut, M, K, N, partial, pl, st);
+  int rc = skinny_run<FWD>(x_bf16, ldx, W_p, W_f, lut, M, K, N, partial, pl, st, epi.io_f32 ? kSegBlocks : 0);
   if (rc != PACKR_OK) return rc;
   skinny_reduce_epi_kernel<<<gemv::reduce_blocks(M, N), 256, 0, st>>>(partial, pl.splits, (int)M, (int)N, bias,
                                                                       bias_f32, epi);

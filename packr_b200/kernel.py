@@ -330,12 +330,13 @@ def linear_act_forward(x: torch.Tensor, W_p: torch.Tensor, W_f: torch.Tensor, lu
     xd = _dtype_code(x)
     wp, wf = W_p.data_ptr(), W_f.data_ptr()
     with _on_device(dev):
-        nbytes = lib.packr_linear_act_workspace_bytes(M, K, N, xd, wp, wf)
+        od = _dtype_code(out)
+        nbytes = lib.packr_linear_act_workspace_bytes(M, K, N, xd, od, wp, wf)
         ws = _workspace(nbytes, dev)
         code = lib.packr_linear_act_forward(
             x.data_ptr(), xd, wp, wf, lut.data_ptr(), _addr(bias),
             _dtype_code(bias) if bias is not None else 0, activation, _addr(residual),
-            out.data_ptr(), _addr(z), _dtype_code(out), M, K, N,
+            out.data_ptr(), _addr(z), od, M, K, N,
             _addr(ws), nbytes, _raw_stream(dev))
     _lib.check("packr_linear_act_forward", code)
     return out, z

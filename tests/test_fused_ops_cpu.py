@@ -76,7 +76,7 @@ def test_workspace_queries_of_empty_problems():
     lib = _lib.load()
     assert lib.packr_layer_norm_backward_workspace_bytes(0, 8) == 0
     assert lib.packr_layer_norm_backward_workspace_bytes(-3, 8) == 0
-    assert lib.packr_linear_act_workspace_bytes(0, 8, 8, 1, None, None) == 0
+    assert lib.packr_linear_act_workspace_bytes(0, 8, 8, 1, 1, None, None) == 0
     assert lib.packr_linear_act_backward_workspace_bytes(4, 0, 8, 1, 0, None, None) == 0
 
 

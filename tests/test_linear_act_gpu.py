@@ -273,3 +273,42 @@ def test_weight_gradient_with_non_finite_and_zero_tiles(cuda):
     got = grads(c, "none", BF16, need=("W_f", "lut"))
     assert not torch.isfinite(got["dlut"][7]) and not torch.isfinite(got["dlut"][200])
     assert not got["dlut"][:7].any() and not got["dlut"][8:200].any() and not got["dlut"][201:].any()
+
+
+@pytest.mark.parametrize("need", ["x", "W_f", "lut"])
+def test_first_cuda_work_of_a_thread(cuda, need):
+    """A backward whose first driver call is a tensor-map encoding, on a host
+    thread that has made no runtime call (the autograd engine's threads)."""
+    import threading
+    from packr_b200 import kernel as K
+    c = case(160, 128, 144, BF16, BF16, seed=2, residual=False, bias=None)
+    args = (c["dout"], None, 0, c["x"], c["W_p"], c["W_f"], c["lut"], None, need == "x", need == "W_f", need == "lut", None)
+    want = [t for t in K.linear_act_backward(*args) if t is not None]
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        try:
+            got.append(K.linear_act_backward(*args))
+        except Exception as e:  # noqa: BLE001
+            got.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert not isinstance(got[0], Exception), got[0]
+    torch.cuda.synchronize()
+    for a, b in zip((t for t in got[0] if t is not None), want):
+        assert torch.allclose(a.float(), b.float(), rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize("M,K,N", [(300, 11008, 520), (2100, 9000, 1040), (64, 11008, 272)])
+def test_f32_output_of_a_long_reduction(cuda, M, K, N):
+    """The tensor cores truncate every accumulation; an f32 output sums at most
+    2048 elements in one accumulator (128 accumulations of up to 2^-23 of a sum
+    that grows as its square root: 128 * 2^-23 / 2 * 2/3 = 5e-6 of the result at
+    worst, one way), where 11008 in one gave 1.1e-5."""
+    c = case(M, K, N, BF16, F32, seed=1, residual=False)
+    want = linear64(c["x"], c["W_p"], c["W_f"], c["lut"], c["bias"], "none", None, F32)["out"][0]
+    got = call(c, "none", F32).double()
+    assert float((got - want).norm() / want.norm()) < 6e-6
