@@ -1622,10 +1622,11 @@ int make_map(CUtensorMap* m, const void* base, long long inner, long long rows, 
   });
 }
 
-// u8 2-D map over [rows, inner] (row stride in bytes), no swizzle, box
-// {box_inner, box_rows}; out-of-range elements read as zero.
+// u8 2-D map over [rows, inner] (row stride in bytes), no swizzle (or, for a
+// 128-byte box, the 128-byte one), box {box_inner, box_rows}; out-of-range
+// elements read as zero.
 int make_map_u8(CUtensorMap* m, const void* base, long long inner, long long rows, long long row_stride_bytes,
-                int box_inner, int box_rows) {
+                int box_inner, int box_rows, bool swizzle = false) {
   auto fn = encode_fn();
   if (fn == nullptr) return PACKR_ERR_CUDA;
   if (!aligned(base, 16) || (row_stride_bytes & 15) != 0) return PACKR_ERR_ALIGNMENT;
@@ -1636,7 +1637,8 @@ int make_map_u8(CUtensorMap* m, const void* base, long long inner, long long row
   cuuint32_t estr[2] = {1u, 1u};
   return encode_bound([&] {
     return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   });
 }

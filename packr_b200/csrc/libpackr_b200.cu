@@ -11,6 +11,7 @@
 #include "linear.cu"
 #include "static_scratch.cu"
 #include "layer_norm.cu"
+#include "skinny_mma.cu"
 #include "linear_act.cu"
 #include "velvet.cu"
 #include "compress.cu"

@@ -7,8 +7,8 @@
 // is stored in that type: its rounding moves act'(z) by at most the half step
 // of the type, which is what a bf16 layer followed by a bf16 activation keeps.
 //
-// Routes (forward): up to 4 rows the CUDA-core GEMV; 5..128 rows the skinny
-// tcgen05 GEMM and its reduction; from 129 rows, and wherever W's rows do not
+// Routes (forward): 1 and 2 rows the CUDA-core GEMV; 3..16 the mma.sync kernel
+// and 17..128 the skinny tcgen05 GEMM, each with its reduction; from 129 rows, and wherever W's rows do not
 // allow TMA (N % 16 != 0 or a misaligned base), W is decoded once into the
 // workspace, with rows padded to a multiple of 8, and read by TMA, so that odd
 // widths take the same tensor-core GEMM as even ones.  The backward takes dz
@@ -214,9 +214,16 @@ int dz_launch(int a, const void* dout, const void* z, long long M, long long N, 
 }
 
 // ------------------------------------------------------------------ plans
-enum Route { GEMV, SKINNY, PLAIN };
+enum Route { GEMV, SKINNY_MMA, SKINNY, PLAIN };
+// Rows of the mma.sync route, where W's layout allows its TMA.  Measured (us; 11008
+// -> 4096 / 4096 -> 11008 / 1024 -> 4096): 2 rows 29.5 / 29.5 / 8.6 with it, 34.2 /
+// 27.6 / 7.4 with the GEMV; 3 and 4 rows 29.8 / 29.3 / 8.8 and 40.7 / 32.3 / 9.4; 16
+// rows 31.8 / 30.9 / 9.9 with it, 42.2 / 41.6 / 13.1 with the tcgen05 skinny GEMM.
+// (24 rows in a four-group instance: 46.9 against 42.3.)
+constexpr long long kSkinnyMmaMinM = 3, kSkinnyMmaMaxM = 16;
 
 inline Route route(long long M, long long K, long long N, const uint8_t* W_p, const uint16_t* W_f) {
+  if (M >= kSkinnyMmaMinM && M <= kSkinnyMmaMaxM && gemm::wtma_ok(W_p, W_f, N)) return SKINNY_MMA;
   if (linear::skinny_eligible(M, N) && gemm::wtma_ok(W_p, W_f, N)) return SKINNY;
   if (gemv::eligible(M, K, N, W_p, W_f)) return GEMV;
   return PLAIN;
@@ -232,7 +239,9 @@ size_t plan_forward(Carve& c, Fwd& p, Route r, long long M, long long K, long lo
   p = Fwd{};
   if (r == GEMV) return 0;
   p.xh = linear::x_needs_copy(x_dtype, K) ? c.take<uint16_t>((size_t)M * round8(K)) : nullptr;
-  if (r == SKINNY) {
+  if (r == SKINNY_MMA) {
+    p.part = c.take<float>(gemm::sm_partial_bytes(M, K, N) / sizeof(float));
+  } else if (r == SKINNY) {
     p.part = c.take<float>(gemm::skinny_partial_bytes(M, K, N, io_f32 ? gemm::kSegBlocks : 0) / sizeof(float));
   } else {
     p.wd = c.take<uint16_t>((size_t)K * round8(N));
@@ -375,6 +384,9 @@ extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_
   const void* a;
   long long lda;
   if ((st = operand_x(x, x_dtype, M, K, p.xh, nullptr, &a, &lda, s)) != PACKR_OK) return st;
+  if (r == SKINNY_MMA)
+    return gemm::skinny_mma_forward(static_cast<const uint16_t*>(a), lda, W_p, W_f, lut, bias, bias_f32, e, M, K, N,
+                                    p.part, s);
   if (r == SKINNY)
     return gemm::skinny_forward_epi(static_cast<const uint16_t*>(a), lda, W_p, W_f, lut, bias, bias_f32, e, M, K, N,
                                     p.part, s);

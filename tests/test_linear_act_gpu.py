@@ -48,7 +48,7 @@ def compare(c, got, act, out):
 
 
 # up to 4 rows, 5..128, above; widths that TMA reads and that it does not
-SIZES = [(1, 64, 64), (1, 1000, 1001), (2, 256, 130), (4, 130, 96), (3, 33, 20), (5, 128, 64), (7, 100, 33),
+SIZES = [(6, 72, 144), (13, 700, 1040), (17, 520, 256), (31, 96, 128), (32, 4104, 144), (1, 64, 64), (1, 1000, 1001), (2, 256, 130), (4, 130, 96), (3, 33, 20), (5, 128, 64), (7, 100, 33),
          (16, 64, 1000), (100, 768, 1001), (128, 200, 256), (129, 64, 512), (200, 1000, 520), (257, 72, 1111),
          (300, 40, 50), (1, 1, 1), (130, 1, 3), (1030, 128, 272)]
 
@@ -200,7 +200,7 @@ def test_weight_gradient_lands_in_the_optimizer_buffer(cuda):
 
 
 def test_other_stream_and_captured_graph(cuda):
-    for M in (2, 40, 200):
+    for M in (2, 8, 40, 200):
         c = case(M, 128, 256, BF16, BF16, seed=M)
         want = call(c, "gelu", BF16)
         s = torch.cuda.Stream()
