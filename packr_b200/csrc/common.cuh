@@ -22,6 +22,30 @@ int check_device();
 // Maps the last CUDA launch error to a status code (and clears it).
 int launch_status();
 
+// Launches a kernel that may be set up while the previous kernel of the stream
+// still runs; it waits for that kernel's end itself (griddepcontrol.wait) before
+// it touches memory.  Saves the launch latency between two kernels of one
+// operator, about 2 us.
+template <class... P, class... A>
+int launch_overlapped(void (*kern)(P...), dim3 grid, dim3 block, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...) != cudaSuccess) {
+    cudaGetLastError();
+    return PACKR_ERR_LAUNCH;
+  }
+  return launch_status();
+}
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 __host__ __device__ inline bool aligned(const void* p, uintptr_t a) {

@@ -30,6 +30,8 @@
 //   a fixed order, so results do not depend on timing.
 // Rows wider than 16384, and tensors that do not start on a 16-byte boundary,
 // are walked by one CTA per row in passes over L2-resident data.
+#include <atomic>
+
 #include "activation.cuh"
 #include "common.cuh"
 
@@ -453,6 +455,7 @@ __global__ void __launch_bounds__(TMAX, ctas_per_sm(true, E, TMAX))
   const int t = threadIdx.x, nt = blockDim.x, group = threadIdx.y, groups = blockDim.y;
   const long long step = (long long)gridDim.x * groups;
   const long long row0 = (long long)blockIdx.x * groups + group;
+  let_next_kernel_start();
   const L l(t, nt, row0, N);  // the same phase in every row of this group
   Rows<T, E, RAGGED, NT, RING> in;
   in.p[0] = dy;
@@ -650,6 +653,7 @@ __global__ void __launch_bounds__(512) reduce_cols_kernel(const float* __restric
   W* out = which ? out1 : out0;
   if (out == nullptr) return;
   float a = 0.0f;
+  wait_previous_kernel();
   if (c < N)
     for (int q = warp; q < slabs; q += 16) a += __ldcg(partial + ((size_t)q * planes + which) * N + c);
   s[warp][lane] = a;
@@ -665,9 +669,8 @@ __global__ void __launch_bounds__(512) reduce_cols_kernel(const float* __restric
 // ------------------------------------------------------------------ host
 template <class W>
 int reduce_cols(const float* partial, int slabs, int planes, long long N, W* out0, W* out1, cudaStream_t st) {
-  reduce_cols_kernel<W><<<dim3((unsigned)((N + 31) / 32), (unsigned)planes), 512, 0, st>>>(partial, slabs, planes, N,
-                                                                                           out0, out1);
-  return launch_status();
+  return launch_overlapped(reduce_cols_kernel<W>, dim3((unsigned)((N + 31) / 32), (unsigned)planes), dim3(512), st,
+                           partial, slabs, planes, N, out0, out1);
 }
 
 constexpr int kWideSlabs = 64;  // row slabs of bwd_wide_cols_kernel
@@ -722,13 +725,20 @@ inline int bwd_slabs(long long M, long long N, int esize, bool res, bool vec) {
   return shape(M, N, esize, res ? 3 : 2, true).grid;
 }
 
+// Raises a kernel's dynamic shared-memory limit to kMaxSmem, once per device
+// (`done`: the kernel's own flags; relaxed: concurrent first calls set the same
+// attribute).
 template <class K>
-int allow_smem(K kern, size_t smem) {
-  if (smem > 40 * 1024 &&  // the default limit less the static buffers
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+int allow_smem(K kern, size_t smem, std::atomic<int>* done) {
+  if (smem <= 40 * 1024) return PACKR_OK;  // the default limit less the static buffers
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (done[dev & 63].load(std::memory_order_relaxed)) return PACKR_OK;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess) {
     cudaGetLastError();
     return PACKR_ERR_CUDA;
   }
+  done[dev & 63].store(1, std::memory_order_relaxed);
   return PACKR_OK;
 }
 
@@ -736,7 +746,8 @@ template <class T, int E, bool RES, int TMAX>
 int launch_fwd(const Shape& s, const void* x, const void* res, const void* w, const void* b, int wf, float eps, void* y,
                float* mean, float* rstd, long long M, long long N, cudaStream_t st) {
   auto kern = s.ragged ? fwd_kernel<T, E, true, RES, TMAX> : fwd_kernel<T, E, false, RES, TMAX>;
-  const int rc = allow_smem(kern, s.smem);
+  static std::atomic<int> done[2][64];
+  const int rc = allow_smem(kern, s.smem, done[s.ragged]);
   if (rc != PACKR_OK) return rc;
   kern<<<s.grid, dim3(s.nt, s.groups), s.smem, st>>>(static_cast<const T*>(x), static_cast<const T*>(res), w, b, wf, eps,
                                                      static_cast<T*>(y), mean, rstd, M, (int)N, s.stages);
@@ -768,7 +779,8 @@ template <class T, int E, bool RES, int TMAX>
 int launch_bwd(const Shape& s, const void* dy, const void* x, const void* res, const void* w, int wf, const float* mean,
                const float* rstd, void* dx, float* partial, long long M, long long N, cudaStream_t st) {
   auto kern = s.ragged ? bwd_kernel<T, E, true, RES, TMAX> : bwd_kernel<T, E, false, RES, TMAX>;
-  const int rc = allow_smem(kern, s.smem);
+  static std::atomic<int> done[2][64];
+  const int rc = allow_smem(kern, s.smem, done[s.ragged]);
   if (rc != PACKR_OK) return rc;
   kern<<<s.grid, dim3(s.nt, s.groups), s.smem, st>>>(static_cast<const T*>(dy), static_cast<const T*>(x),
                                                      static_cast<const T*>(res), w, wf, mean, rstd,

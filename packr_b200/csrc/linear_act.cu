@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const void* __restrict__ dout, 
                                                  int N, int rows_per_slab, uint16_t* __restrict__ hi,
                                                  uint16_t* __restrict__ lo, long long ld, int vec,
                                                  float* __restrict__ colsum) {
+  let_next_kernel_start();
   const long long c0 = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8;
   if (c0 >= N) return;
   const int r0 = blockIdx.y * rows_per_slab;
