@@ -117,6 +117,20 @@ class PackRMatmulFunction(torch.autograd.Function):
         return dX, None, dW, dlut, None, None, None
 
 
+def _linear_act_backward(ctx, grad_out):
+    x, W_p, W_f, lut, z, counts = ctx.saved_tensors
+    nx, _, nwf, nlut, nb, nr = ctx.needs_input_grad[:6]
+    g = grad_out if grad_out.dtype == ctx.out_dtype else grad_out.to(ctx.out_dtype)
+    g = _aligned16(g.contiguous())
+    dX, dW, dlut, dbias = _k.linear_act_backward(g, z, ctx.activation, x, W_p, W_f, lut, counts, nx, nwf, nlut,
+                                                 ctx.bias_dtype if nb else None,
+                                                 dW_out=grad_sink(ctx.wf_param) if nwf else None)
+    return dX, None, dW, dlut, dbias, grad_out if nr else None, None, None, None
+
+
+_linear_act_backward_once = once_differentiable(_linear_act_backward)
+
+
 class PackRLinearActFunction(torch.autograd.Function):
     """out = act(x @ W + bias) + residual on contiguous 2-D operands; keeps x
     and, for an activation, z = x @ W + bias in out's dtype."""
@@ -124,7 +138,7 @@ class PackRLinearActFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W_p, W_f, lut, bias, residual, activation, out_dtype, counts):
         out, z = _k.linear_act_forward(x, W_p, W_f, lut, bias, activation, residual, out_dtype,
-                                       keep_z=activation != _lib.ACTIVATIONS["none"])
+                                       keep_z=activation != _NO_ACTIVATION)
         ctx.save_for_backward(x, W_p, W_f, lut, z, counts)
         ctx.activation, ctx.out_dtype = activation, out_dtype
         ctx.bias_dtype = None if bias is None else bias.dtype
@@ -132,18 +146,13 @@ class PackRLinearActFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
-        x, W_p, W_f, lut, z, counts = ctx.saved_tensors
-        nx, _, nwf, nlut, nb, nr = ctx.needs_input_grad[:6]
-        g = grad_out if grad_out.dtype == ctx.out_dtype else grad_out.to(ctx.out_dtype)
-        g = g.contiguous()
-        if g.data_ptr() % 16:
-            g = g.clone()
-        dX, dW, dlut, dbias = _k.linear_act_backward(g, z, ctx.activation, x, W_p, W_f, lut, counts, nx, nwf, nlut,
-                                                     ctx.bias_dtype if nb else None,
-                                                     dW_out=grad_sink(ctx.wf_param) if nwf else None)
-        return dX, None, dW, dlut, dbias, grad_out if nr else None, None, None, None
+        # a backward that records (create_graph) must refuse a second derivative
+        return (_linear_act_backward_once if torch.is_grad_enabled() else _linear_act_backward)(ctx, grad_out)
+
+
+_NO_ACTIVATION = _lib.ACTIVATIONS["none"]
+_FLOATS = (torch.bfloat16, torch.float32)
 
 
 def _aligned16(t):
@@ -171,44 +180,58 @@ def packr_linear_act(x, W_p, W_f, lut, bias=None, activation=None, residual=None
     gradient of the pre-activation enters the weight and lut gradients rounded
     to bf16, as in PackRLinear; with f32 x as bf16 hi + lo parts
     (PACKR_DW_PRECISION)."""
-    if not (x.is_cuda and W_p.is_cuda and W_f.is_cuda and lut.is_cuda):
+    if not x.is_cuda:
         raise RuntimeError("packr_linear_act runs on CUDA tensors only (no CPU path in the B200 build)")
     act = _lib.ACTIVATIONS.get("none" if activation is None else activation)
     if act is None:
         raise ValueError(f"packr_linear_act: activation must be one of {sorted(_lib.ACTIVATIONS)}, not {activation!r}")
-    if x.dtype not in (torch.bfloat16, torch.float32):
+    if x.dtype not in _FLOATS:
         raise TypeError(f"packr_linear_act: unsupported dtype {x.dtype}")
-    if out_dtype not in (torch.bfloat16, torch.float32):
+    if out_dtype not in _FLOATS:
         raise TypeError(f"packr_linear_act: out_dtype must be float32 or bfloat16, not {out_dtype}")
     if W_p.dtype != torch.uint8 or W_f.dtype != torch.bfloat16 or lut.dtype != torch.float32:
         raise TypeError("packr_linear_act: W_p must be uint8, W_f bfloat16 and lut float32")
-    if W_p.dim() != 2 or W_p.shape != W_f.shape or tuple(lut.shape) != (256,) or min(W_p.shape) < 1:
+    if W_p.dim() != 2 or W_p.shape != W_f.shape or lut.shape != _LUT_SHAPE or W_p.numel() == 0:
         raise ValueError("packr_linear_act: W_p and W_f must be [K, N] (K, N >= 1) and lut [256]")
     K, N = W_p.shape
     if x.dim() < 1 or x.shape[-1] != K:
         raise ValueError(f"packr_linear_act: x's last dimension must be {K}, got {tuple(x.shape)}")
-    lead = x.shape[:-1]
     if not W_p.is_contiguous():
         raise ValueError("packr_linear_act: W_p must be contiguous")
-    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype not in (torch.bfloat16, torch.float32)):
-        raise ValueError(f"packr_linear_act: bias must be bf16 or f32 [{N}]")
-    if residual is not None and (residual.shape != lead + (N,) or residual.dtype != out_dtype):
-        raise ValueError(f"packr_linear_act: residual must be {tuple(lead) + (N,)} of {out_dtype}")
-    if counts is not None and (counts.dtype != torch.int32 or tuple(counts.shape) != (256,)
-                               or not counts.is_contiguous()):
-        raise ValueError("packr_linear_act: counts must be contiguous int32 [256]")
-    for t in (W_p, W_f, lut, bias, residual, counts):
-        if t is not None and t.device != x.device:
-            raise ValueError("packr_linear_act: every tensor must be on x's device")
-    x2 = _aligned16(x.reshape(-1, K).contiguous())
-    r2 = None if residual is None else residual.reshape(-1, N).contiguous()
+    dev = x.device
+    if W_p.device != dev or W_f.device != dev or lut.device != dev:
+        raise ValueError("packr_linear_act: every tensor must be on x's device")
+    grad = x.requires_grad or W_f.requires_grad or lut.requires_grad
+    flat = x.dim() == 2
+    x2 = _aligned16((x if flat else x.reshape(-1, K)).contiguous())
     W_f, lut = W_f.contiguous(), lut.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, W_f, lut, bias, r2)):
-        out = PackRLinearActFunction.apply(x2, W_p, W_f, lut, bias, r2, act, out_dtype, counts)
+    if bias is not None:
+        if bias.dim() != 1 or bias.shape[0] != N or bias.dtype not in _FLOATS:
+            raise ValueError(f"packr_linear_act: bias must be bf16 or f32 [{N}]")
+        if bias.device != dev:
+            raise ValueError("packr_linear_act: every tensor must be on x's device")
+        grad = grad or bias.requires_grad
+        bias = bias.contiguous()
+    if residual is not None:
+        if residual.shape != x.shape[:-1] + (N,) or residual.dtype != out_dtype:
+            raise ValueError(f"packr_linear_act: residual must be {tuple(x.shape[:-1]) + (N,)} of {out_dtype}")
+        if residual.device != dev:
+            raise ValueError("packr_linear_act: every tensor must be on x's device")
+        grad = grad or residual.requires_grad
+        residual = (residual if flat else residual.reshape(-1, N)).contiguous()
+    if counts is not None:
+        if counts.dtype != torch.int32 or counts.shape != _LUT_SHAPE or not counts.is_contiguous():
+            raise ValueError("packr_linear_act: counts must be contiguous int32 [256]")
+        if counts.device != dev:
+            raise ValueError("packr_linear_act: every tensor must be on x's device")
+    if grad and torch.is_grad_enabled():
+        out = PackRLinearActFunction.apply(x2, W_p, W_f, lut, bias, residual, act, out_dtype, counts)
     else:
-        out = _k.linear_act_forward(x2, W_p, W_f, lut, bias, act, r2, out_dtype)[0]
-    return out if x.dim() == 2 else out.reshape(lead + (N,))
+        out = _k.linear_act_forward(x2, W_p, W_f, lut, bias, act, residual, out_dtype)[0]
+    return out if flat else out.reshape(x.shape[:-1] + (N,))
+
+
+_LUT_SHAPE = torch.Size([256])
 
 
 # Legacy alias (reference packr/__init__.py:32)

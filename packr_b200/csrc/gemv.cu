@@ -426,14 +426,21 @@ int launch(const Plan& p, const void* x, int x_f32, int Mr, const uint8_t* W_p, 
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    int clusters = 0;
-    if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess) {
-      cudaGetLastError();
-      clusters = 0;
-    }
-    if (clusters < 1 && q.cluster > 1) {  // a cluster this large does not fit: shrink it
-      q.cluster -= 1;
-      continue;
+    // whether a cluster this large fits: asked once per cluster and shared-memory
+    // size and device (relaxed atomics: concurrent calls ask the same)
+    static std::atomic<long long> fits[64];
+    const long long key = (long long)q.cluster << 32 | (long long)q.smem;
+    if (fits[dev & 63].load(std::memory_order_relaxed) != key) {
+      int clusters = 0;
+      if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        clusters = 0;
+      }
+      if (clusters < 1 && q.cluster > 1) {  // it does not: shrink it
+        q.cluster -= 1;
+        continue;
+      }
+      fits[dev & 63].store(key, std::memory_order_relaxed);
     }
     if (cudaLaunchKernelEx(&cfg, kern, x, x_f32, Mr, W_p, W_f, lut, bias, bias_f32, out, (int)K, (int)N,
                            q.rows_per_cta, q.rows_per_warp, epi) != cudaSuccess)

@@ -353,15 +353,15 @@ def linear_act_backward(dout: torch.Tensor, z: torch.Tensor | None, activation: 
     M, K = x.shape
     N = W_p.shape[1]
     dev = x.device
-    dX = torch.empty(M, K, dtype=x.dtype, device=dev) if need_dx else None
+    dX = torch.empty_like(x) if need_dx else None
     if need_dw and dW_out is not None:
         if (dW_out.dtype != torch.bfloat16 or tuple(dW_out.shape) != (K, N) or not dW_out.is_contiguous()
                 or dW_out.device != dev):
             raise ValueError("dW_out must be a contiguous bf16 [K, N] tensor on x's device")
         dW = dW_out
     else:
-        dW = torch.empty(K, N, dtype=torch.bfloat16, device=dev) if need_dw else None
-    dlut = torch.empty(256, dtype=torch.float32, device=dev) if need_dlut else None
+        dW = torch.empty_like(W_f) if need_dw else None
+    dlut = torch.empty_like(lut) if need_dlut else None
     dbias = torch.empty(N, dtype=dbias_dtype, device=dev) if dbias_dtype is not None else None
     if not (need_dx or need_dw or need_dlut or dbias is not None):
         return None, None, None, None

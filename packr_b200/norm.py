@@ -66,23 +66,31 @@ def layer_norm_backward(dy, x, weight, stats, residual=None, w_dtype=_F32, need_
     return dx, dw, db
 
 
+def _norm_backward(ctx, dy):
+    x, weight, residual, stats = ctx.saved_tensors
+    nx, nw, nb, _, nr = ctx.needs_input_grad
+    if dy.dtype != x.dtype:
+        dy = dy.to(x.dtype)
+    dx, dw, db = layer_norm_backward(dy.contiguous(), x, weight, stats, residual, ctx.w_dtype, nx or nr, nw, nb)
+    return dx if nx else None, dw, db, None, dx if nr else None
+
+
+_norm_backward_once = once_differentiable(_norm_backward)
+
+
 class PackRLayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, residual):
         y, stats = layer_norm_forward(x, weight, bias, eps, residual, stats=True)
         ctx.save_for_backward(x, weight, residual, stats)
-        ctx.w_dtype = (weight if weight is not None else bias).dtype if weight is not None or bias is not None else _F32
+        w = weight if weight is not None else bias
+        ctx.w_dtype = _F32 if w is None else w.dtype
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, residual, stats = ctx.saved_tensors
-        nx, nw, nb, _, nr = ctx.needs_input_grad
-        if dy.dtype != x.dtype:
-            dy = dy.to(x.dtype)
-        dx, dw, db = layer_norm_backward(dy.contiguous(), x, weight, stats, residual, ctx.w_dtype, nx or nr, nw, nb)
-        return dx if nx else None, dw, db, None, dx if nr else None
+        # a backward that records (create_graph) must refuse a second derivative
+        return _norm_backward_once(ctx, dy) if torch.is_grad_enabled() else _norm_backward(ctx, dy)
 
 
 def packr_layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
@@ -102,25 +110,34 @@ def packr_layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
         raise TypeError(f"packr_layer_norm: unsupported dtype {x.dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("packr_layer_norm: x needs a last dimension of at least 1")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if t.device != x.device or t.dtype not in _CODE or tuple(t.shape) != (x.shape[-1],):
-            raise ValueError(f"packr_layer_norm: {name} must be f32 or bf16 [{x.shape[-1]}] on x's device")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError("packr_layer_norm: weight and bias must have one dtype")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
-        raise ValueError("packr_layer_norm: residual must have x's shape, dtype and device")
+    grad = x.requires_grad
+    x = x.contiguous()
+    if weight is not None:
+        _check_vector("weight", weight, x)
+        grad = grad or weight.requires_grad
+        weight = weight.contiguous()
+    if bias is not None:
+        _check_vector("bias", bias, x)
+        if weight is not None and weight.dtype != bias.dtype:
+            raise TypeError("packr_layer_norm: weight and bias must have one dtype")
+        grad = grad or bias.requires_grad
+        bias = bias.contiguous()
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+            raise ValueError("packr_layer_norm: residual must have x's shape, dtype and device")
+        grad = grad or residual.requires_grad
+        residual = residual.contiguous()
     eps = float(eps)
     if not eps >= 0.0:
         raise ValueError(f"packr_layer_norm: eps must be >= 0, got {eps}")
-    x = x.contiguous()
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    residual = None if residual is None else residual.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if grad and torch.is_grad_enabled():
         return PackRLayerNormFunction.apply(x, weight, bias, eps, residual)
     return layer_norm_forward(x, weight, bias, eps, residual)[0]
+
+
+def _check_vector(name, t, x):
+    if t.dim() != 1 or t.shape[0] != x.shape[-1] or t.dtype not in _CODE or t.device != x.device:
+        raise ValueError(f"packr_layer_norm: {name} must be f32 or bf16 [{x.shape[-1]}] on x's device")
 
 
 class PackRLayerNorm(nn.LayerNorm):
