@@ -230,6 +230,7 @@ struct Params {
   float* sk_partial;         // [pairs][MSUB][2 ranks][256 cols][128 rows]
   int* sk_flags;             // [pairs][2 ranks][epilogue warps], zeroed before the launch
   int sk_slots;              // pairs the two buffers above have room for (0: no stream-K)
+  int sk_max_split;          // fewer tiles than pairs: at most so many shares of a tile (0: all pairs)
   int sk_dp_tiles;           // with sk: tiles [0, sk_dp_tiles) go round-robin first (whole tiles)
   // dynamic tiles (plain FWD / DX without stream-K): each pair takes its next
   // whole tile from this counter (zeroed before the launch), so that pairs
@@ -1643,15 +1644,40 @@ int make_map_u8(CUtensorMap* m, const void* base, long long inner, long long row
   });
 }
 
+// Stream-K for the fused linear layer, where it pays.  A 256-row tile's k-block
+// takes 0.38 us; splitting costs about 12 us (the flags' clearing, the partials'
+// way through L2, the waits) and 3 us for each share after a tile's first, which
+// the tile's owner adds in turn.  Measured (forward, decode included): 777 x 1000
+// -> 1111 40 us split, 28 whole; 300 x 1024 -> 4096 36 and 26; 130 x 4096 -> 4096
+// 54 and 52; 257 x 11008 -> 4096 100 and 118; 24 x 4835 -> 175, one tile in 74
+// shares, 219 us.
+//
+// Fewer tiles than pairs: the shares to cut each tile's reduction into (1: none).
+inline int tile_split(long long tiles, int pairs, long long kblocks, int msub) {
+  const double whole = 0.38 * kblocks * msub;
+  int best = 1;
+  double best_t = whole;
+  for (int s = 2; s * tiles <= pairs; ++s) {
+    const double t = whole / s + 12.0 + 3.0 * msub * (s - 1);
+    if (t < best_t) {
+      best_t = t;
+      best = s;
+    }
+  }
+  return best;
+}
 // Whether splitting the last, partly filled wave of `rem` tiles over all pairs
-// pays for the fused linear layer: it saves the idle pairs' share of a tile's
-// k-blocks (0.38 us each per 256-row subtile) and costs the flags' clearing,
-// the partials' way through L2 and the waits, together about 20 us.  Measured
-// (forward, decode included): 777 x 1000 -> 1111 40 us split, 28 whole; 300 x
-// 1024 -> 4096 36 and 26; 130 x 4096 -> 4096 54 and 52; 257 x 11008 -> 4096 100
-// and 118.
-inline bool split_pays(int rem, int pairs, long long kblocks, int msub) {
+// pays.
+inline bool split_pays(long long rem, int pairs, long long kblocks, int msub) {
   return kblocks * msub * (pairs - rem) >= 64LL * pairs;
+}
+// Sets Params' stream-K fields by these rules.
+inline void set_split(Params& P, float* partial, int* flags, int slots, long long tiles, int msub) {
+  const long long kb = (P.Kg + BK - 1) / BK;
+  P.sk_partial = partial;
+  P.sk_flags = flags;
+  P.sk_max_split = tiles < slots ? tile_split(tiles, slots, kb, msub) : 0;
+  P.sk_slots = tiles < slots ? (P.sk_max_split > 1 ? slots : 0) : (split_pays(tiles % slots, slots, kb, msub) ? slots : 0);
 }
 
 template <int MODE, int BSRC, int MSUB = 1, int EPI = 0>
@@ -1698,10 +1724,12 @@ int launch_impl(Params P, const Maps& maps, cudaStream_t stream) {
   // tile's share spanning several pairs whose partials its first pair adds
   // (measured: the plain forward and dX at 256 rows, 16-43 tiles of the
   // Llama FFN layers, otherwise leave most SMs idle).
-  const bool sk_all = C::kStreamK && PACKR_STREAM_K && (EPI == 0 || split_pays(tiles % max_pairs, max_pairs, kbt, MSUB)) &&
-                      P.sk_partial != nullptr && P.sk_flags != nullptr && tiles < max_pairs && max_pairs > 1 && max_pairs <= P.sk_slots && kbt >= 2 &&
-                      (long long)tiles * kbt >= max_pairs;  // every pair a non-empty range (it publishes a flag)
-  const int pairs = sk_all ? max_pairs : (tiles < max_pairs ? tiles : max_pairs);
+  const long long sk_pairs = P.sk_max_split > 0 && (long long)tiles * P.sk_max_split < max_pairs
+                                 ? (long long)tiles * P.sk_max_split : max_pairs;
+  const bool sk_all = C::kStreamK && PACKR_STREAM_K && P.sk_partial != nullptr && P.sk_flags != nullptr &&
+                      tiles < sk_pairs && sk_pairs > 1 && sk_pairs <= P.sk_slots && kbt >= 2 &&
+                      (long long)tiles * kbt >= sk_pairs;  // every pair a non-empty range (it publishes a flag)
+  const int pairs = sk_all ? (int)sk_pairs : (tiles < max_pairs ? tiles : max_pairs);
   cfg.gridDim = dim3(2 * pairs, 1, 1);
   // stream-K when every pair gets at least one tile's worth of k-blocks (so a
   // tile is split between two pairs at most) and the workspace has the slots
@@ -1720,8 +1748,7 @@ int launch_impl(Params P, const Maps& maps, cudaStream_t stream) {
     // pair.
     const int waves = tiles / pairs, rem = tiles % pairs;
     P.sk_dp_tiles = waves >= 2 ? (waves - 1) * pairs : 0;
-    if (waves >= 1 && rem != 0 && (EPI == 0 || split_pays(rem, pairs, kbt, MSUB)) &&
-        rem * 100 <= pairs * PACKR_SK_LAST_WAVE_PCT &&
+    if (waves >= 1 && rem != 0 && rem * 100 <= pairs * PACKR_SK_LAST_WAVE_PCT &&
         (long long)(tiles - P.sk_dp_tiles) * kbt / pairs >= kbt) {
       P.sk = 1;
       if (cudaMemsetAsync(P.sk_flags, 0, (size_t)pairs * 2 * C::kEpiWarps * sizeof(int), stream) != cudaSuccess)

@@ -282,6 +282,11 @@ size_t plan_backward(Carve& c, Bwd& p, long long M, long long K, long long N, in
   return c.off;
 }
 
+// Output tiles (256 * msub rows, 256 columns) of a GEMM.
+inline long long tiles_of(long long rows, long long cols, int msub) {
+  return (rows + 256LL * msub - 1) / (256 * msub) * ((cols + 255) / 256);
+}
+
 inline bool act_ok(int a) { return a >= PACKR_ACT_NONE && a <= PACKR_ACT_SILU; }
 inline bool io_ok(int d) { return d == PACKR_DTYPE_F32 || d == PACKR_DTYPE_BF16; }
 inline size_t io_size(int d) { return d == PACKR_DTYPE_F32 ? 4 : 2; }
@@ -404,9 +409,8 @@ extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_
   P.bias = bias;
   P.bias_f32 = bias_f32;
   P.epi = e;
-  P.sk_partial = p.skp;
-  P.sk_flags = p.skf;
-  P.sk_slots = linear::sk_pairs();
+  const int msub = gemm::epi_msub(M, K, e.io_f32);
+  gemm::set_split(P, p.skp, p.skf, linear::sk_pairs(), tiles_of(M, N, msub), msub);
   return gemm::launch_plain_epi(P, maps, s);
 }
 
@@ -489,12 +493,8 @@ extern "C" int packr_linear_act_backward(const void* dout, const void* z, int ou
     P.out = dX;
     P.ld_out = K;
     P.out_f32 = x_dtype == PACKR_DTYPE_F32;
-    P.sk_partial = p.skp;
-    P.sk_flags = p.skf;
-    // no split of a short reduction (gemm::split_pays)
-    const int msub = linear::plain_msub(M), pairs = linear::sk_pairs();
-    const long long tiles = ((M + 256LL * msub - 1) / (256 * msub)) * ((K + 255) / 256);
-    P.sk_slots = gemm::split_pays((int)(tiles % pairs), pairs, (N + 63) / 64, msub) ? pairs : 0;
+    const int msub = linear::plain_msub(M);
+    gemm::set_split(P, p.skp, p.skf, linear::sk_pairs(), tiles_of(M, K, msub), msub);
     if ((st = gemm::launch_plain<gemm::DX>(P, maps, s)) != PACKR_OK) return st;
   }
   if (dw || dl) {
