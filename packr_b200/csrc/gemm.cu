@@ -71,7 +71,7 @@ constexpr int BN_CTA = 128;      // B columns held by each CTA
 constexpr int BK = 64, UK = 16;
 constexpr int MAX_STAGES = 6;
 constexpr int TILE_Q = 4;        // dynamic-tile queue slots
-constexpr int kSegBlocks = 32;   // k-blocks of one accumulator of an f32 output (2048 elements)
+constexpr int kSegBlocks = 16;   // k-blocks of one accumulator of an f32 output (1024 elements)
 constexpr int kMore = 4;         // Unit::kind flag
 constexpr int BARS_BYTES = 512;  // shared memory reserved for struct Bars
 constexpr int A_BYTES = BM * BK * 2;      // 16 KB
@@ -847,9 +847,9 @@ __global__ void __launch_bounds__(Cfg<MODE, BSRC, MSUB, EPI>::kThreads, 1)
   // state.  False past the last unit or on an abort.
   // An f32 output takes its reduction in segments of kSegBlocks k-blocks: the
   // tensor cores truncate each f32 accumulation, which adds up to 1e-9 of the
-  // result per reduction element, one way (measured 4.2e-6 at 4096, 1.1e-5 at
-  // 11008), so the segments' accumulators are added by the epilogue instead,
-  // rounded to nearest.  kMore marks a unit whose sum goes on in the next.
+  // result per reduction element, one way (measured 8.9e-7 at 1024, 4.2e-6 at
+  // 4096, 1.1e-5 at 11008), so the segments' accumulators are added by the
+  // epilogue instead, rounded to nearest.  kMore marks a unit whose sum goes on in the next.
   Unit rest{-1, 0, 0, 0};  // (producer) what is left of a segmented unit
   auto unit_push = [&](int i, Sched& sc, Unit& x) -> bool {
     const int slot = i % TILE_Q;
