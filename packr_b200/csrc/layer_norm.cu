@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(512) fwd_wide_kernel(const void* __restrict__ 
                                                        int wf, float eps, void* __restrict__ y,
                                                        float* __restrict__ mean_out, float* __restrict__ rstd_out,
                                                        long long M, long long N) {
-  __shared__ float bufs[2][32];
+  __shared__ __align__(16) float bufs[2][32];
   const int t = threadIdx.x, nt = blockDim.x;
   for (long long row = blockIdx.x; row < M; row += gridDim.x) {
     auto at = [&](long long c) {
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(512)
     bwd_wide_kernel(const void* __restrict__ dy, const void* __restrict__ x, const void* __restrict__ res, int xf,
                     const void* __restrict__ weight, int wf, const float* __restrict__ mean_in,
                     const float* __restrict__ rstd_in, void* __restrict__ dx, long long M, long long N) {
-  __shared__ float bufs[2][32];
+  __shared__ __align__(16) float bufs[2][32];
   const int t = threadIdx.x, nt = blockDim.x;
   for (long long row = blockIdx.x; row < M; row += gridDim.x) {
     const float mean = mean_in[row], rstd = rstd_in[row];

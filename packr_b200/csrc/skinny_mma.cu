@@ -286,9 +286,9 @@ __global__ void __launch_bounds__(128) skinny_mma_reduce_kernel(const float* __r
                                                                 const void* __restrict__ bias, int bias_f32,
                                                                 const Epilogue epi) {
   const int qpr = N / 4;
-  const int q = blockIdx.x * blockDim.x + threadIdx.x;
-  if (q >= M * qpr) return;
-  const int m = q / qpr, n = (q - m * qpr) * 4;
+  const long long q = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (q >= (long long)M * qpr) return;
+  const int m = (int)(q / qpr), n = (int)(q - (long long)m * qpr) * 4;
   const long long o = (long long)m * N + n;
   float r[4] = {0.0f, 0.0f, 0.0f, 0.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll

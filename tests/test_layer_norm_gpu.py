@@ -190,3 +190,102 @@ def test_module_follows_torch(cuda):
     want = norm64(x.view(20, 96), r.view(20, 96), m.weight, m.bias, 1e-12)
     check("y", m(x, residual=r), want["y"])
     assert repr(m).startswith("PackRLayerNorm((96,)")
+
+
+def test_captured_training_step(cuda):
+    """Forward and backward in one graph, replayed on new inputs; a second graph
+    of the same tensors beside it."""
+    c = case(60, 384, BF16, F32, seed=7)
+    leaves = {k: c[k].detach().clone().requires_grad_(True) for k in ("x", "residual", "weight", "bias")}
+    dy = c["dy"].clone()
+
+    def step():
+        y = packr.packr_layer_norm(leaves["x"], leaves["weight"], leaves["bias"], 1e-5, leaves["residual"])
+        return (y, *torch.autograd.grad(y, list(leaves.values()), dy))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step())
+        graphs.append(g)
+    c2 = case(60, 384, BF16, F32, seed=70)
+    with torch.no_grad():
+        for k, v in leaves.items():
+            v.copy_(c2[k])
+        dy.copy_(c2["dy"])
+    for g in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    want = run(c2)
+    for out in outs:
+        for a, b in zip(out, (want["y"], want["dx"], want["dresidual"], want["dweight"], want["dbias"])):
+            assert torch.equal(a, b)
+
+
+def test_two_streams_at_once(cuda):
+    cs = [case(2000, 1001, BF16, F32, seed=i) for i in range(2)]
+    want = [run(c) for c in cs]
+    streams = [torch.cuda.Stream() for _ in cs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for c, s in zip(cs, streams):
+            with torch.cuda.stream(s):
+                got.append(run(c))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        for k, v in want[i % 2].items():
+            assert torch.equal(g[k], v), k
+
+
+def test_tensors_beyond_32_bit_offsets(cuda):
+    M, N = 140001, 16384  # 2.29e9 elements; the last rows start past 2^31
+    assert M * N > 1 << 31
+    x = torch.zeros(M, N, dtype=BF16, device="cuda")
+    tail = case(5, N, BF16, BF16, seed=3, residual=False)
+    x[-5:] = tail["x"]
+    w, b = tail["weight"].requires_grad_(True), tail["bias"].requires_grad_(True)
+    x.requires_grad_(True)
+    y = packr.packr_layer_norm(x, w, b)
+    dy = torch.zeros_like(y)
+    dy[-5:] = tail["dy"]
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+    want = norm64(tail["x"], None, w, b, 1e-5, tail["dy"])
+    check("y", y[-5:], want["y"], 2.4e-3)
+    check("dx", dx[-5:], want["dx"], 2.4e-3)
+    check("dweight", dw, want["dweight"])
+    check("dbias", db, want["dbias"])
+    assert not dx[:10].any() and torch.equal(y[0], b.detach())
+
+
+def test_second_derivative_is_refused(cuda):
+    c = case(4, 64, F32, F32, seed=1)
+    x = c["x"].requires_grad_(True)
+    y = packr.packr_layer_norm(x, c["weight"], c["bias"])
+    g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+
+
+def test_refused_arguments(cuda):
+    x = torch.zeros(4, 8, device="cuda")
+    w = torch.ones(8, device="cuda")
+    for bad in (dict(weight=torch.ones(7, device="cuda")), dict(weight=torch.ones(8)), dict(weight=w.half()),
+                dict(weight=w, residual=x[:2]), dict(weight=w, residual=x.bfloat16()), dict(weight=w, residual=x.cpu()),
+                dict(weight=w, eps=-1.0), dict(weight=w, eps=float("nan"))):
+        with pytest.raises(ValueError):
+            packr.packr_layer_norm(x, **bad)
+    with pytest.raises(TypeError):
+        packr.packr_layer_norm(x, w, w.bfloat16())
+    with pytest.raises(TypeError):
+        packr.packr_layer_norm(x.half(), w)
+    with pytest.raises(ValueError):
+        packr.packr_layer_norm(torch.zeros(4, 0, device="cuda"))
+    with pytest.raises(ValueError):
+        packr.PackRLayerNorm(9, device="cuda")(x)

@@ -312,3 +312,127 @@ def test_f32_output_of_a_long_reduction(cuda, M, K, N):
     want = linear64(c["x"], c["W_p"], c["W_f"], c["lut"], c["bias"], "none", None, F32)["out"][0]
     got = call(c, "none", F32).double()
     assert float((got - want).norm() / want.norm()) < 3e-6
+
+
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("M", [6, 200])
+def test_captured_training_step(cuda, M, act):
+    """Forward and backward in one graph, replayed on new inputs; a second graph
+    of the same tensors beside it."""
+    c = case(M, 128, 256, BF16, BF16, seed=M)
+    names = ("x", "W_f", "bias", "residual") + (("lut",) if act == "none" else ())
+    leaves = {k: c[k].detach().clone().requires_grad_(True) for k in names}
+    d = {**c, **leaves, "W_p": c["W_p"].clone(), "lut": leaves.get("lut", c["lut"].clone())}
+    dout = c["dout"].clone()
+
+    def step():
+        y = call(d, act, BF16)
+        return (y, *torch.autograd.grad(y, list(leaves.values()), dout))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step())
+        graphs.append(g)
+    c2 = case(M, 128, 256, BF16, BF16, seed=M + 90)
+    with torch.no_grad():
+        for k, v in d.items():
+            if k in c2 and k != "dY":
+                v.copy_(c2[k]) if k != "dout" else None
+        dout.copy_(c2["dout"])
+    for g in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    want = grads(c2, act, BF16, need=names)
+    for out in outs:
+        for name, a in zip(("out",) + tuple("d" + n for n in names), out):
+            if name == "dlut":  # f32 atomics over CTAs
+                assert torch.allclose(a, want[name], rtol=1e-3, atol=1e-5)
+            else:
+                assert torch.equal(a, want[name]), name
+
+
+@pytest.mark.parametrize("M", [1, 12, 60, 300])
+def test_two_streams_at_once(cuda, M):
+    cs = [case(M, 520, 1040, BF16, BF16, seed=i) for i in range(2)]
+    need = ("x", "W_f", "bias")
+    want = [grads(c, "silu", BF16, need=need) for c in cs]
+    streams = [torch.cuda.Stream() for _ in cs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for c, s in zip(cs, streams):
+            with torch.cuda.stream(s):
+                got.append(grads(c, "silu", BF16, need=need))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        for k, v in want[i % 2].items():
+            assert torch.equal(g[k], v), k
+
+
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_output_beyond_32_bit_offsets(cuda, out):
+    M, K, N = 200005, 32, 11008  # 2.2e9 outputs
+    assert M * N > 1 << 31
+    c = case(5, K, N, BF16, out, seed=3, residual=False)
+    x = torch.zeros(M, K, dtype=BF16, device="cuda")
+    x[-5:] = c["x"]
+    y = packr.packr_linear_act(x, c["W_p"], c["W_f"], c["lut"], c["bias"], activation="gelu", out_dtype=out)
+    want = linear64(c["x"], c["W_p"], c["W_f"], c["lut"], c["bias"], "gelu", None, out)["out"]
+    check("out", y[-5:], want)
+    bias = linear64(torch.zeros_like(c["x"]), c["W_p"], c["W_f"], c["lut"], c["bias"], "gelu", None, out)["out"]
+    check("out", y[M // 2:M // 2 + 5], bias)
+
+
+def test_second_derivative_is_refused(cuda):
+    c = case(4, 64, 64, F32, F32, seed=1)
+    x = c["x"].requires_grad_(True)
+    y = packr.packr_linear_act(x, c["W_p"], c["W_f"], c["lut"], activation="silu")
+    g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+
+
+def test_refused_arguments(cuda):
+    c = case(4, 64, 96, BF16, BF16, seed=1)
+    ok = dict(x=c["x"], W_p=c["W_p"], W_f=c["W_f"], lut=c["lut"], bias=c["bias"], out_dtype=BF16)
+    packr.packr_linear_act(**ok)
+    bad_values = [dict(x=c["x"][:, :63]), dict(W_p=c["W_p"][:, :95]), dict(W_p=c["W_p"].t()), dict(lut=c["lut"][:255]),
+                  dict(bias=c["bias"][:95]), dict(bias=c["bias"].double()), dict(bias=c["bias"].cpu()),
+                  dict(residual=c["residual"][:3]), dict(residual=c["residual"].float()),
+                  dict(residual=c["residual"].cpu()), dict(activation="tanh"), dict(W_f=c["W_f"].cpu()),
+                  dict(counts=torch.zeros(256, device="cuda")), dict(counts=torch.zeros(256, dtype=torch.int32))]
+    for bad in bad_values:
+        with pytest.raises(ValueError):
+            packr.packr_linear_act(**{**ok, **bad})
+    for bad in (dict(x=c["x"].half()), dict(out_dtype=torch.float16), dict(W_f=c["W_f"].float()),
+                dict(W_p=c["W_p"].int()), dict(lut=c["lut"].double())):
+        with pytest.raises(TypeError):
+            packr.packr_linear_act(**{**ok, **bad})
+
+
+def test_c_entry_refuses_a_small_workspace_and_a_misaligned_x(cuda):
+    from packr_b200 import _lib
+    lib = _lib.load()
+    for M in (8, 64, 200):
+        c = case(M, 64, 96, BF16, BF16, seed=1, residual=False)
+        out = torch.zeros(M, 96, dtype=BF16, device="cuda")
+        wp, wf = c["W_p"].data_ptr(), c["W_f"].data_ptr()
+        need = lib.packr_linear_act_workspace_bytes(M, 64, 96, 1, 1, wp, wf)
+        ws = torch.zeros(need + 256, dtype=torch.uint8, device="cuda")
+
+        def fwd(x, ws_ptr, nbytes):
+            return lib.packr_linear_act_forward(x, 1, wp, wf, c["lut"].data_ptr(), None, 0, 0, None, out.data_ptr(), None,
+                                                1, M, 64, 96, ws_ptr, nbytes, None)
+
+        x = c["x"].data_ptr()
+        assert need > 0 and fwd(x, ws.data_ptr(), need - 1) == 4 and fwd(x, None, need) == 4
+        assert fwd(x, ws.data_ptr() + 16, need) == 4 and fwd(x + 2, ws.data_ptr(), need) == 3
+        torch.cuda.synchronize()
+        assert not out.any()  # nothing ran
