@@ -222,8 +222,8 @@ int packr_predecode_route(int64_t M, int64_t K, int64_t N, const uint8_t* W_p, c
  * input.
  * A caller that will run the backward of an activation passes z, which gets
  * the pre-activation.  activation: PACKR_ACT_*.  M = 0 is a no-op.  x, when it
- * is bf16 and K % 8 == 0, is read by TMA and must be 16-byte aligned from 5
- * rows on.  The workspace query takes W_p and W_f because the route depends
+ * is bf16 and K % 8 == 0, is read by TMA and must be 16-byte aligned from 3
+ * rows on (PACKR_ERR_ALIGNMENT).  The workspace query takes W_p and W_f because the route depends
  * on their alignment; 256-byte aligned workspace, PACKR_ERR_WORKSPACE below
  * the query's size.  The reference runs packr_matmul, then torch kernels for
  * the bias, activation and residual (packr/layer.py:96-97 and the host
