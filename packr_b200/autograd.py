@@ -18,6 +18,7 @@ ignored; evict_cb still fires at the end of backward.
 from __future__ import annotations
 
 import os
+import weakref
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -38,17 +39,40 @@ def grad_sink(param: torch.Tensor) -> torch.Tensor | None:
     Only offered while param.grad is None: the backward then writes the
     gradient straight into the buffer and autograd adopts the view as
     param.grad without a copy; with a gradient already present, autograd
-    accumulates into it as usual."""
-    if param is None or param.grad is not None:
-        return None
+    accumulates into it as usual.  Not offered either while a view lent before
+    is still held: by autograd, when the parameter is used more than once and
+    its gradients are yet to be summed, or by a caller of torch.autograd.grad."""
     spec = getattr(param, "_packr_grad_sink", None)
-    if spec is None:
+    if spec is None or param.grad is not None:
         return None
     buf, off = spec
     n = param.numel()
     if buf.dtype != param.dtype or buf.device != param.device or off + n > buf.numel():
         return None
-    return buf[off:off + n].view(param.shape)
+    lent = getattr(param, "_packr_grad_lent", None)
+    if lent is None:
+        lent = param._packr_grad_lent = _Lent()
+    if lent.held():
+        return None
+    view = buf[off:off + n].view(param.shape)
+    lent.ref = weakref.ref(view)
+    return view
+
+
+class _Lent:
+    """The last view of a gradient buffer that was given out; copies and
+    pickles start empty (a weak reference has no place in a saved model)."""
+
+    __slots__ = ("ref",)
+
+    def __init__(self):
+        self.ref = None
+
+    def held(self) -> bool:
+        return self.ref is not None and self.ref() is not None
+
+    def __reduce__(self):
+        return _Lent, ()
 
 
 def _forward_keep_w(ctx, x, W_p, W_f, lut, bias):

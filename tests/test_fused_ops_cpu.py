@@ -1,12 +1,15 @@
 """What the fused feed-forward operators refuse, without a GPU, and their
 64-bit reference forms against torch's own functions."""
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
 
 import packr_b200 as packr
 from packr_b200 import _lib
+from packr_b200.autograd import grad_sink
 from fused_reference import ACTS, act64, linear64, norm64, slope64, weights64
 
 
@@ -198,3 +201,53 @@ def test_layer_takes_known_activations():
     with pytest.raises(ValueError):
         packr.PackRLinear(4, 8, activation="tanh")
     assert packr.PackRConfig().fuse_epilogues is False
+
+
+class _Scale(torch.autograd.Function):
+    """x * w whose backward writes w's gradient into the buffer it is lent."""
+
+    @staticmethod
+    def forward(ctx, x, w):
+        ctx.save_for_backward(x)
+        ctx.w = w
+        return x * w
+
+    @staticmethod
+    def backward(ctx, g):
+        x, = ctx.saved_tensors
+        out = grad_sink(ctx.w)
+        return None, g * x if out is None else torch.mul(g, x, out=out)
+
+
+def _parameter_with_sink():
+    w = torch.nn.Parameter(torch.ones(4))
+    w._packr_grad_sink = (torch.zeros(6), 2)
+    return w, w._packr_grad_sink[0][2:].data_ptr()
+
+
+def test_gradients_of_a_parameter_used_twice_are_summed():
+    w, at = _parameter_with_sink()
+    x = torch.arange(4.0)
+    for _ in range(2):
+        (_Scale.apply(x, w).sum() + _Scale.apply(5 * x, w).sum()).backward()
+        assert torch.equal(w.grad, 6 * x)
+        w.grad = None
+    for k in range(3):  # used once, the buffer itself becomes the gradient
+        _Scale.apply(k * x, w).sum().backward()
+        assert torch.equal(w.grad, k * x) and w.grad.data_ptr() == at
+        w.grad = None
+
+
+def test_a_gradient_in_hand_is_not_overwritten():
+    w, _ = _parameter_with_sink()
+    x = torch.arange(4.0)
+    a, = torch.autograd.grad(_Scale.apply(x, w).sum(), w)
+    b, = torch.autograd.grad(_Scale.apply(3 * x, w).sum(), w)
+    assert torch.equal(a, x) and torch.equal(b, 3 * x)
+
+
+def test_a_parameter_with_a_buffer_can_be_copied():
+    w, _ = _parameter_with_sink()
+    _Scale.apply(torch.ones(4), w).sum().backward()
+    assert torch.equal(copy.deepcopy(w), w)
+    assert torch.equal(pickle.loads(pickle.dumps(w)), w)

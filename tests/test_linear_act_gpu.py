@@ -199,6 +199,21 @@ def test_weight_gradient_lands_in_the_optimizer_buffer(cuda):
     assert torch.equal(W_f.grad, grads(c, "gelu", BF16, need=("W_f",))["dW_f"])
 
 
+def test_shared_weights_with_an_optimizer_buffer(cuda):
+    """A layer applied twice: the two gradients are summed, not the second one
+    written over the first."""
+    c = case(40, 96, 96, BF16, BF16, seed=2, residual=False)
+    got = []
+    for sink in (False, True):
+        W_f = torch.nn.Parameter(c["W_f"])
+        if sink:
+            W_f._packr_grad_sink = (torch.zeros(96 * 96, dtype=BF16, device="cuda"), 0)
+        d = {**c, "W_f": W_f}
+        call({**d, "x": call(d, "gelu", BF16)}, "gelu", BF16).backward(c["dout"])
+        got.append(W_f.grad)
+    assert torch.equal(got[0], got[1])
+
+
 def test_other_stream_and_captured_graph(cuda):
     for M in (2, 8, 40, 200):
         c = case(M, 128, 256, BF16, BF16, seed=M)
