@@ -66,8 +66,11 @@ __device__ __forceinline__ float slope(float z) {
     return fmaf(z * e, kInvSqrt2Pi, p);
   }
   if (ACT == PACKR_ACT_GELU_TANH) {
-    const float s = sigmoid(2.0f * kTanhC * fmaf(kTanhK * z * z, z, z));
-    return fmaf(z * s * (1.0f - s), 2.0f * kTanhC * fmaf(3.0f * kTanhK, z * z, 1.0f), s);
+    // s is 0 or 1 from |z| = 20 on, far below; z * z beyond the type's range would
+    // make the product 0 * infinity
+    const float zz = fminf(z * z, 400.0f);
+    const float s = sigmoid(2.0f * kTanhC * fmaf(kTanhK * zz, z, z));
+    return fmaf(z * s * (1.0f - s), 2.0f * kTanhC * fmaf(3.0f * kTanhK, zz, 1.0f), s);
   }
   if (ACT == PACKR_ACT_SILU) {
     const float s = sigmoid(z);

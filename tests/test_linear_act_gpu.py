@@ -78,6 +78,23 @@ def test_gradients(cuda, M, K, N, xt, out):
         compare(c, grads(c, act, out), act, out)
 
 
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M", [1, 8, 30, 140])
+def test_activations_of_huge_values(cuda, act, M):
+    """z = +-1e30, whose square is past the type's range: act and slope are those
+    of the limits, 0 and z, 0 and 1."""
+    K, N = 64, 96
+    z = torch.where(torch.arange(N, device="cuda") % 2 == 0, 1e30, -1e30)
+    c = dict(x=torch.zeros(M, K, dtype=BF16, device="cuda"), W_p=torch.zeros(K, N, dtype=torch.uint8, device="cuda"),
+             W_f=torch.zeros(K, N, dtype=BF16, device="cuda"), lut=torch.zeros(256, device="cuda"),
+             bias=z.clone().requires_grad_(True))
+    y = packr.packr_linear_act(**c, activation=act)
+    db, = torch.autograd.grad(y, c["bias"], torch.ones_like(y))
+    kept = z if act == "none" else z.clamp_min(0.0)
+    assert torch.equal(y, kept.expand(M, N))
+    assert torch.equal(db, torch.full_like(z, float(M)) if act == "none" else M * (z > 0).float())
+
+
 @pytest.mark.parametrize("need", [("x",), ("W_f",), ("lut",), ("bias",), ("residual",), ("x", "bias")])
 def test_only_the_gradients_asked_for(cuda, need):
     c = case(140, 128, 144, BF16, BF16, seed=2)
