@@ -287,6 +287,15 @@ inline long long tiles_of(long long rows, long long cols, int msub) {
   return (rows + 256LL * msub - 1) / (256 * msub) * ((cols + 255) / 256);
 }
 
+// Largest dimension: tiles and slabs of rows that start inside it end within an int.
+constexpr long long kMaxDim = 0x7F000000ll;
+
+int check_args(const void* x, int x_dtype, const uint8_t* W_p, const uint16_t* W_f, const float* lut, long long M,
+               long long K, long long N) {
+  if (M > kMaxDim || K > kMaxDim || N > kMaxDim) return PACKR_ERR_SHAPE;
+  return linear::check_common(x, x_dtype, W_p, W_f, lut, M, K, N);
+}
+
 inline bool act_ok(int a) { return a >= PACKR_ACT_NONE && a <= PACKR_ACT_SILU; }
 inline bool io_ok(int d) { return d == PACKR_DTYPE_F32 || d == PACKR_DTYPE_BF16; }
 inline size_t io_size(int d) { return d == PACKR_DTYPE_F32 ? 4 : 2; }
@@ -359,7 +368,7 @@ extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_
                                         int64_t N, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace packr;
   using namespace packr::linear_act;
-  int st = linear::check_common(x, x_dtype, W_p, W_f, lut, M, K, N);
+  int st = check_args(x, x_dtype, W_p, W_f, lut, M, K, N);
   if (st != PACKR_OK) return st;
   if (!act_ok(activation) || !io_ok(out_dtype) || (bias != nullptr && !io_ok(bias_dtype)))
     return PACKR_ERR_INVALID_ARGUMENT;
@@ -431,7 +440,7 @@ extern "C" int packr_linear_act_backward(const void* dout, const void* z, int ou
                                          size_t workspace_bytes, void* stream) {
   using namespace packr;
   using namespace packr::linear_act;
-  int st = linear::check_common(x, x_dtype, W_p, W_f, lut, M, K, N);
+  int st = check_args(x, x_dtype, W_p, W_f, lut, M, K, N);
   if (st != PACKR_OK) return st;
   if (!act_ok(activation) || !io_ok(out_dtype) || (dbias != nullptr && !io_ok(dbias_dtype)) ||
       (flags & ~PACKR_BWD_DW_SPLIT) != 0)

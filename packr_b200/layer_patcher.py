@@ -124,7 +124,11 @@ class PackRAddNorm(nn.Module):
 
     def forward(self, hidden_states, input_tensor):
         h = self.dropout(self.dense(hidden_states))
-        return self.LayerNorm(h, residual=input_tensor.to(h.dtype))
+        # the sum's type is the wider one's, as h + input_tensor's; fp16 is
+        # widened (the norm takes f32 and bf16)
+        t = torch.promote_types(h.dtype, input_tensor.dtype)
+        t = torch.float32 if t == torch.float16 else t
+        return self.LayerNorm(h.to(t), residual=input_tensor.to(t))
 
 
 def fuse_epilogues(model: nn.Module):
@@ -136,7 +140,8 @@ def fuse_epilogues(model: nn.Module):
     * blocks that add their input before a layer norm (BERT's BertOutput and
       BertSelfOutput, and their Roberta and Electra twins) become PackRAddNorm.
 
-    Activations other than relu, gelu (either form) and silu stay as they are.
+    Activations other than relu, gelu (either form) and silu stay as they are,
+    and so do norms whose weights are neither f32 nor bf16.
     Parameters, their names and the model's results (up to rounding) do not
     change.  Returns the model."""
     for name, module in list(model.named_modules()):
@@ -151,7 +156,8 @@ def fuse_epilogues(model: nn.Module):
                     setattr(module, act, nn.Identity())
         if type(module).__name__ in _ADD_NORM_CLASSES and name:
             norm = getattr(module, "LayerNorm", None)
-            if type(norm) is nn.LayerNorm and len(norm.normalized_shape) == 1:
+            if (type(norm) is nn.LayerNorm and len(norm.normalized_shape) == 1
+                    and (norm.weight is None or norm.weight.dtype in (torch.float32, torch.bfloat16))):
                 fused = PackRAddNorm(module.dense, norm, module.dropout)
                 fused.train(module.training)
                 _replace_module(model, name, fused)

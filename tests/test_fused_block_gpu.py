@@ -127,3 +127,18 @@ def test_layer_attributes_change_the_route_only(cuda):
     lin.activation, lin.out_dtype = None, BF16
     assert torch.allclose(lin(x).float(), plain, rtol=2.0 ** -8, atol=1e-5)
     assert torch.equal(lin(x.half()), lin(x.half().float()))
+
+
+@pytest.mark.parametrize("dense,given", [(BF16, F32), (F32, BF16), (torch.float16, F32), (torch.float16, torch.float16)])
+def test_add_norm_of_mixed_types(cuda, dense, given):
+    """The sum is taken in the wider type: a residual stream of f32 is not rounded
+    to a bf16 projection's type.  f32 sums of 64 terms: 1e-5 covers them."""
+    from packr_b200.layer_patcher import PackRAddNorm
+    lin = torch.nn.Linear(64, 64, device="cuda", dtype=dense)
+    norm = torch.nn.LayerNorm(64, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(5, 64, generator=g, device="cuda").to(dense)
+    r = torch.randn(5, 64, generator=g, device="cuda").to(given)
+    got = PackRAddNorm(lin, norm)(x, r)
+    want = norm(lin(x).float() + r.float())
+    assert got.dtype == F32 and torch.allclose(got, want, rtol=1e-5, atol=1e-5)

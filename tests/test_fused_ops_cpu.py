@@ -53,6 +53,17 @@ def test_linear_act_c_entry_refuses_bad_arguments():
     assert bwd(db=a, dbd=2) == 1 and bwd(dout=odd) == 3 and bwd(dw=odd) == 3 and bwd(db=_fake(2), dbd=0) == 3
 
 
+@pytest.mark.parametrize("dim", ["M", "K", "N"])
+def test_linear_act_c_entry_refuses_dimensions_next_to_2_31(dim):
+    """A tile or a slab that starts inside them would end past an int's range."""
+    lib, a = _lib.load(), _fake()
+    d = {"M": 4, "K": 8, "N": 8, dim: 0x7FFFFFFF}
+    assert lib.packr_linear_act_forward(a, 1, a, a, a, None, 0, 0, None, a, None, 1, d["M"], d["K"], d["N"], None, 0,
+                                        None) == 2
+    assert lib.packr_linear_act_backward(a, a, 1, 2, a, 1, a, a, a, None, a, a, None, None, 0, d["M"], d["K"], d["N"], 0,
+                                         None, 0, None) == 2
+
+
 def test_layer_norm_c_entry_refuses_bad_arguments():
     lib = _lib.load()
     a, odd = _fake(), _fake(1)
@@ -192,6 +203,20 @@ def test_plain_linears_keep_their_activation():
     b = Block()
     packr.fuse_epilogues(b)
     assert isinstance(b.activation_fn, torch.nn.ReLU)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_norms_of_other_types_stay(dtype):
+    class BertOutput(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.dense = torch.nn.Linear(8, 8)
+            self.LayerNorm = torch.nn.LayerNorm(8, dtype=dtype)
+            self.dropout = torch.nn.Dropout(0.0)
+
+    model = torch.nn.Sequential(BertOutput())
+    packr.fuse_epilogues(model)
+    assert (type(model[0]).__name__ == "PackRAddNorm") == (dtype != torch.float16)
 
 
 def test_layer_takes_known_activations():
