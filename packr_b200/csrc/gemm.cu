@@ -1817,7 +1817,9 @@ int launch_plain(Params P, const Maps& maps, cudaStream_t stream) {
 }
 
 // dW without the lut gradient: P.sk_flags (nullable) one word for the tile
-// counter.  512-row tiles when there are waves of them and a long reduction.
+// counter.  512-row tiles when there are waves of them and a long reduction (4096
+// tokens, 4096 x 11008: 264 us, 320 with 256-row tiles); fewer of them than CTA
+// pairs would leave SMs idle.
 int launch_dw_plain(Params P, const Maps& maps, cudaStream_t stream) {
   P.out_vec = aligned(P.out, 16);
   P.n_tiles = (P.Ng + BN - 1) / BN;
@@ -1832,11 +1834,9 @@ int launch_dw_plain(Params P, const Maps& maps, cudaStream_t stream) {
 // accumulator takes the next tile or, for an f32 output, the next segment.
 // Measured at 4096 rows: 4096 -> 11008 311 us with 512, 339 with 256; 768 -> 2048
 // 66 and 46.
-#ifndef PACKR_EPI_MSUB2_MIN_K
-#define PACKR_EPI_MSUB2_MIN_K 2048
-#endif
+constexpr long long kEpiMsub2MinK = 2048;
 inline int epi_msub(long long M, long long K, int io_f32) {
-  return !io_f32 && M >= PACKR_PLAIN_MSUB2_MIN_M && K >= PACKR_EPI_MSUB2_MIN_K ? 2 : 1;
+  return !io_f32 && M >= PACKR_PLAIN_MSUB2_MIN_M && K >= kEpiMsub2MinK ? 2 : 1;
 }
 
 // The plain forward with the fused epilogue P.epi.

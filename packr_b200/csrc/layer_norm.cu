@@ -209,7 +209,7 @@ struct Rows {
     const long long n = (total - i) * (long long)sizeof(T);
     return n < 16 ? (int)n : 16;
   }
-  // copies the row `ahead` rows on into stage `stage`; `last`: it is the tensor's last row
+  // copies the row `ahead` rows on into stage `stage`; `last`: its last chunk may pass the tensor's end
   __device__ __forceinline__ void issue(const L& l, int ahead, int stage, bool last) const {
     const long long i0 = at + ahead * stride;
     const uint32_t dst = smem + stage * (NT * L::NV) * pitch;
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(TMAX, ctas_per_sm(false, E, TMAX))
   in.pitch = (uint32_t)(nt * blockDim.y) * 16;
   in.smem = (uint32_t)__cvta_generic_to_shared(ring) + (uint32_t)(group * nt + t) * 16;
   int left = (int)((M - 1 - row) / step);        // rows after this one
-  const bool ends = row + left * step == M - 1;  // the last of them is the tensor's last
+  const bool ends = (M - 1 - row - left * step) * N < L::VW;  // the last of them shares the tensor's last chunk
   if (RING) {
     in.clear(l, stages);
     for (int s = 0; s < stages - 1; ++s) {
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(TMAX, ctas_per_sm(true, E, TMAX))
   in.pitch = (uint32_t)(nt * groups) * 16;
   in.smem = (uint32_t)__cvta_generic_to_shared(ring) + (uint32_t)(group * nt + t) * 16;
   int left = row0 < M ? (int)((M - 1 - row0) / step) : -1;  // rows after the first, -1: no row at all
-  const bool ends = row0 + left * step == M - 1;
+  const bool ends = left >= 0 && (M - 1 - row0 - left * step) * N < L::VW;  // the last row shares the tensor's last chunk
   if (RING) {
     in.clear(l, stages);
     for (int s = 0; s < stages - 1; ++s) {

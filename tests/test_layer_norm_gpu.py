@@ -289,3 +289,34 @@ def test_refused_arguments(cuda):
         packr.packr_layer_norm(torch.zeros(4, 0, device="cuda"))
     with pytest.raises(ValueError):
         packr.PackRLayerNorm(9, device="cuda")(x)
+
+
+@pytest.mark.parametrize("xt", [BF16, F32])
+@pytest.mark.parametrize("M,N", [(13, 1), (3, 1), (11, 2), (9, 3), (7, 5), (1201, 1), (5003, 3), (6001, 7)])
+def test_rows_shorter_than_a_chunk_inside_larger_buffers(cuda, xt, M, N):
+    """Several rows share the tensor's last 16 bytes; what lies behind it is
+    neither read into a result nor written."""
+    c = case(M, N, xt, xt, seed=M + N)
+    inner = {}
+    for k in ("x", "residual", "dy"):
+        buf = torch.full((M * N + 64,), float("nan"), dtype=xt, device="cuda")
+        inner[k] = buf[:M * N].view(M, N)
+        inner[k].copy_(c[k])
+    got = run({**c, **inner})
+    compare(c, got)
+    lib = packr._lib.load()
+    for name in ("y", "dx"):
+        out = torch.full((M * N + 64,), 7.0, dtype=xt, device="cuda")
+        stats = torch.empty(2, M, device="cuda")
+        code = 0 if xt == F32 else 1
+        s = torch.cuda.current_stream().cuda_stream
+        p = lambda t: t.data_ptr()  # noqa: E731
+        other = torch.empty_like(c["x"])
+        assert lib.packr_layer_norm_forward(p(inner["x"]), p(inner["residual"]), code, p(c["weight"]), p(c["bias"]), code,
+                                            1e-5, p(out if name == "y" else other), p(stats), p(stats) + 4 * M, M, N,
+                                            s) == 0
+        if name == "dx":
+            assert lib.packr_layer_norm_backward(p(inner["dy"]), p(inner["x"]), p(inner["residual"]), code, p(c["weight"]),
+                                                 code, p(stats), p(stats) + 4 * M, p(out), None, None, M, N, None, 0, s) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out[:M * N].view(M, N), got[name]) and bool((out[M * N:] == 7).all())
