@@ -27,10 +27,11 @@ int launch_status();
 // it touches memory.  Saves the launch latency between two kernels of one
 // operator, about 2 us.
 template <class... P, class... A>
-int launch_overlapped(void (*kern)(P...), dim3 grid, dim3 block, cudaStream_t st, A... args) {
+int launch_overlapped(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

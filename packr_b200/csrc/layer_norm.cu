@@ -669,7 +669,7 @@ __global__ void __launch_bounds__(512) reduce_cols_kernel(const float* __restric
 // ------------------------------------------------------------------ host
 template <class W>
 int reduce_cols(const float* partial, int slabs, int planes, long long N, W* out0, W* out1, cudaStream_t st) {
-  return launch_overlapped(reduce_cols_kernel<W>, dim3((unsigned)((N + 31) / 32), (unsigned)planes), dim3(512), st,
+  return launch_overlapped(reduce_cols_kernel<W>, dim3((unsigned)((N + 31) / 32), (unsigned)planes), dim3(512), 0, st,
                            partial, slabs, planes, N, out0, out1);
 }
 

@@ -108,9 +108,26 @@ __global__ void __launch_bounds__(kSmThreads, 1)
   volatile int* const abort_flag = &bars->abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int u0 = sm_start(plan, blockIdx.x), count = sm_start(plan, blockIdx.x + 1) - u0, k_blocks = plan.k_blocks;
-  // the reduction may be set up now; it waits for this grid's end before it reads
-  let_next_kernel_start();
-  if (threadIdx.x == 0) {
+  int tile = u0 / k_blocks, kb = u0 % k_blocks;
+  const bool producer = threadIdx.x == kSmWarps * 32;
+  int it = 0;  // (producer) next stage to fill
+  auto fill = [&] {
+    const int s = it % S;
+    uint8_t* const st = smem + s * C::kStageBytes;
+    mbar_arrive_expect_tx(&bars->full[s], C::kStageBytes);
+    tma_load_2d(st, &maps.wf, &bars->full[s], tile * kSmCols, kb * BK);
+    tma_load_2d(st + 8192, &maps.wf, &bars->full[s], tile * kSmCols + 64, kb * BK);
+    tma_load_2d(st + C::kWBytes, &maps.wp, &bars->full[s], tile * kSmCols, kb * BK);
+    tma_load_2d(st + C::kWBytes + C::kPBytes, &maps.x, &bars->full[s], kb * BK, 0);
+    if (++kb == k_blocks) {
+      kb = 0;
+      ++tile;
+    }
+  };
+  if (producer) {
+    prefetch_tmap(&maps.wf);
+    prefetch_tmap(&maps.wp);
+    prefetch_tmap(&maps.x);
     for (int s = 0; s < S; ++s) {
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], kSmWarps / 2);
@@ -118,6 +135,12 @@ __global__ void __launch_bounds__(kSmThreads, 1)
     bars->abort = 0;
     fence_barrier_init();
   }
+  // this kernel may start before the one in front of it ends, and lets the
+  // reduction start; every read of global memory comes after the wait
+  wait_previous_kernel();
+  let_next_kernel_start();
+  if (producer)  // the ring's first round, under the lut's set-up
+    for (; it < count && it < S; ++it) fill();
   if (warp < 8) {  // entry e of lane l at e * 128 + l * 4, rotated stores
     const int e = threadIdx.x;
     const uint32_t v = f32_to_bf16_rne(__ldg(lut + e));
@@ -125,29 +148,14 @@ __global__ void __launch_bounds__(kSmThreads, 1)
     for (int l = 0; l < 32; ++l) *reinterpret_cast<uint32_t*>(lut_b + e * 128 + ((l + lane) & 31) * 4) = v;
   }
   __syncthreads();
-  int tile = u0 / k_blocks, kb = u0 % k_blocks;
 
   if (warp == kSmWarps) {
     // ------------------------------------------------ TMA producer
-    if (lane == 0) {
-      prefetch_tmap(&maps.wf);
-      prefetch_tmap(&maps.wp);
-      prefetch_tmap(&maps.x);
-      int it = 0;
+    if (producer) {
       bool ok = true;
       for (; it < count; ++it) {
-        const int s = it % S;
-        if (!(ok = mbar_wait(&bars->empty[s], ((uint32_t)(it / S) & 1u) ^ 1u, abort_flag))) break;
-        uint8_t* const st = smem + s * C::kStageBytes;
-        mbar_arrive_expect_tx(&bars->full[s], C::kStageBytes);
-        tma_load_2d(st, &maps.wf, &bars->full[s], tile * kSmCols, kb * BK);
-        tma_load_2d(st + 8192, &maps.wf, &bars->full[s], tile * kSmCols + 64, kb * BK);
-        tma_load_2d(st + C::kWBytes, &maps.wp, &bars->full[s], tile * kSmCols, kb * BK);
-        tma_load_2d(st + C::kWBytes + C::kPBytes, &maps.x, &bars->full[s], kb * BK, 0);
-        if (++kb == k_blocks) {
-          kb = 0;
-          ++tile;
-        }
+        if (!(ok = mbar_wait(&bars->empty[it % S], ((uint32_t)(it / S) & 1u) ^ 1u, abort_flag))) break;
+        fill();
       }
       if (!ok) {  // gave up: the copies in flight still land before the CTA ends
         volatile int none = 0;
@@ -167,7 +175,6 @@ __global__ void __launch_bounds__(kSmThreads, 1)
     const uint32_t x_off = (uint32_t)(C::kWBytes + C::kPBytes + g * 128 + 4 * t);
     const uint32_t smem0 = smem_u32(smem), lut0 = smem_u32(lut_b);
     bool ok = true;
-    int it = 0;
     for (int slot = 0; it < count; ++slot, ++tile, kb = 0) {
       const int end = min(count, it + k_blocks - kb);  // of this tile's stages
       float acc[4][MT][4];
@@ -285,6 +292,8 @@ __global__ void __launch_bounds__(128) skinny_mma_reduce_kernel(const float* __r
                                                                 int slot_floats, const SmPlan plan,
                                                                 const void* __restrict__ bias, int bias_f32,
                                                                 const Epilogue epi) {
+  // (what a next call's kernel reads and writes, it does after this one's end)
+  let_next_kernel_start();
   const int qpr = N / 4;
   const long long q = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (q >= (long long)M * qpr) return;
@@ -336,10 +345,10 @@ int sm_launch(const SmMaps& maps, const float* lut, const void* bias, int bias_f
     done[dev & 63].store(1, std::memory_order_relaxed);
   }
   const SmPlan p = sm_plan(K, N);
-  skinny_mma_kernel<MT><<<p.ctas, kSmThreads, C::kSmemBytes, st>>>(maps, lut, partial, (int)K, p);
-  int rc = launch_status();
+  const int rc = launch_overlapped(skinny_mma_kernel<MT>, dim3((unsigned)p.ctas), dim3(kSmThreads), C::kSmemBytes, st, maps,
+                                   lut, partial, (int)K, p);
   if (rc != PACKR_OK) return rc;
-  return launch_overlapped(skinny_mma_reduce_kernel, dim3((unsigned)((M * (N / 4) + 127) / 128)), dim3(128), st, partial,
+  return launch_overlapped(skinny_mma_reduce_kernel, dim3((unsigned)((M * (N / 4) + 127) / 128)), dim3(128), 0, st, partial,
                            (int)M, (int)N, MT * 8 * kSmCols, p, bias, bias_f32, epi);
 }
 
