@@ -341,6 +341,9 @@ __global__ void __launch_bounds__(TMAX, ctas_per_sm(false, E, TMAX))
   constexpr int P = E / 2;  // pairs
   __shared__ __align__(16) float bufs[kMaxGroups][2][32];
   extern __shared__ __align__(16) uint8_t ring[];
+  // may start before the kernel in front of it ends, and lets the next one start
+  wait_previous_kernel();
+  let_next_kernel_start();
   const int t = threadIdx.x, nt = blockDim.x, group = threadIdx.y;
   const long long step = (long long)gridDim.x * blockDim.y;
   long long row = (long long)blockIdx.x * blockDim.y + group;
@@ -455,6 +458,7 @@ __global__ void __launch_bounds__(TMAX, ctas_per_sm(true, E, TMAX))
   const int t = threadIdx.x, nt = blockDim.x, group = threadIdx.y, groups = blockDim.y;
   const long long step = (long long)gridDim.x * groups;
   const long long row0 = (long long)blockIdx.x * groups + group;
+  wait_previous_kernel();
   let_next_kernel_start();
   const L l(t, nt, row0, N);  // the same phase in every row of this group
   Rows<T, E, RAGGED, NT, RING> in;
@@ -749,9 +753,8 @@ int launch_fwd(const Shape& s, const void* x, const void* res, const void* w, co
   static std::atomic<int> done[2][64];
   const int rc = allow_smem(kern, s.smem, done[s.ragged]);
   if (rc != PACKR_OK) return rc;
-  kern<<<s.grid, dim3(s.nt, s.groups), s.smem, st>>>(static_cast<const T*>(x), static_cast<const T*>(res), w, b, wf, eps,
-                                                     static_cast<T*>(y), mean, rstd, M, (int)N, s.stages);
-  return launch_status();
+  return launch_overlapped(kern, dim3((unsigned)s.grid), dim3(s.nt, s.groups), s.smem, st, static_cast<const T*>(x),
+                           static_cast<const T*>(res), w, b, wf, eps, static_cast<T*>(y), mean, rstd, M, (int)N, s.stages);
 }
 
 template <class T>
@@ -782,10 +785,9 @@ int launch_bwd(const Shape& s, const void* dy, const void* x, const void* res, c
   static std::atomic<int> done[2][64];
   const int rc = allow_smem(kern, s.smem, done[s.ragged]);
   if (rc != PACKR_OK) return rc;
-  kern<<<s.grid, dim3(s.nt, s.groups), s.smem, st>>>(static_cast<const T*>(dy), static_cast<const T*>(x),
-                                                     static_cast<const T*>(res), w, wf, mean, rstd,
-                                                     static_cast<T*>(dx), partial, M, (int)N, s.stages);
-  return launch_status();
+  return launch_overlapped(kern, dim3((unsigned)s.grid), dim3(s.nt, s.groups), s.smem, st, static_cast<const T*>(dy),
+                           static_cast<const T*>(x), static_cast<const T*>(res), w, wf, mean, rstd, static_cast<T*>(dx),
+                           partial, M, (int)N, s.stages);
 }
 
 template <class T>

@@ -123,6 +123,10 @@ __global__ void __launch_bounds__(SkCfg<MODE, NPAD>::kThreads, 1)
     tmem_alloc(&bars->tmem_base, C::kTmemCols);
     tmem_relinquish();
   }
+  // may start before the kernel in front of it ends, and lets the reduction
+  // start; every read of global memory comes after the wait
+  wait_previous_kernel();
+  let_next_kernel_start();
   if (warp >= C::kDecWarp0) {
     const int dw = warp - C::kDecWarp0;
     for (int e = dw; e < 256; e += C::kDecWarps) lut_s[e * 32 + lane] = f32_to_bf16_rne(__ldg(P.dec.lut + e));
@@ -315,8 +319,7 @@ int skinny_launch(const SkParams& P, const SkMaps& maps, int grid, cudaStream_t 
                               C::kSmemBytes) != cudaSuccess;
   });
   if (rc) return PACKR_ERR_CUDA;
-  skinny_kernel<MODE, NPAD><<<grid, C::kThreads, C::kSmemBytes, st>>>(P, maps);
-  return launch_status();
+  return launch_overlapped(skinny_kernel<MODE, NPAD>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmemBytes, st, P, maps);
 }
 
 // The skinny GEMM's main launch: act_bf16 [M, ld_act] (x for FWD, bf16(dY)
@@ -425,6 +428,7 @@ int skinny_forward(const uint16_t* x_bf16, long long ldx, const uint8_t* W_p, co
 __global__ void __launch_bounds__(256) skinny_reduce_epi_kernel(const float* __restrict__ partial, int splits, int M,
                                                                 int N, const void* __restrict__ bias, int bias_f32,
                                                                 const Epilogue epi) {
+  let_next_kernel_start();
   const int qpr = N / 4;
   const long long q = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (q >= (long long)M * qpr) return;
@@ -437,6 +441,7 @@ __global__ void __launch_bounds__(256) skinny_reduce_epi_kernel(const float* __r
 #pragma unroll
     for (int j = 0; j < 4; ++j) r[j] = load_io(epi.residual, o + j, epi.io_f32);
   }
+  wait_previous_kernel();
   int sp = 0;
   for (; sp + 4 <= splits; sp += 4) {  // four splits in flight
     float4 v[4];
@@ -477,9 +482,8 @@ int skinny_forward_epi(const uint16_t* x_bf16, long long ldx, const uint8_t* W_p
   SkPlan pl;
   int rc = skinny_run<FWD>(x_bf16, ldx, W_p, W_f, lut, M, K, N, partial, pl, st, epi.io_f32 ? kSegBlocks : 0);
   if (rc != PACKR_OK) return rc;
-  skinny_reduce_epi_kernel<<<gemv::reduce_blocks(M, N), 256, 0, st>>>(partial, pl.splits, (int)M, (int)N, bias,
-                                                                      bias_f32, epi);
-  return launch_status();
+  return launch_overlapped(skinny_reduce_epi_kernel, dim3((unsigned)gemv::reduce_blocks(M, N)), dim3(256), 0, st, partial,
+                           pl.splits, (int)M, (int)N, bias, bias_f32, epi);
 }
 
 }  // namespace gemm
