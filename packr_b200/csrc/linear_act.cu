@@ -7,11 +7,12 @@
 // is stored in that type: its rounding moves act'(z) by at most the half step
 // of the type, which is what a bf16 layer followed by a bf16 activation keeps.
 //
-// Routes (forward): 1 and 2 rows the CUDA-core GEMV; 3..16 the mma.sync kernel
-// and 17..128 the skinny tcgen05 GEMM, each with its reduction; from 129 rows, and wherever W's rows do not
-// allow TMA (N % 16 != 0 or a misaligned base), W is decoded once into the
-// workspace, with rows padded to a multiple of 8, and read by TMA, so that odd
-// widths take the same tensor-core GEMM as even ones.  The backward takes dz
+// Routes (forward): 1 and 2 rows the CUDA-core GEMV; 3..16, and 1 or 2 with a long
+// reduction, the mma.sync kernel and 17..128 the skinny tcgen05 GEMM, each with its
+// reduction; from 129 rows, and wherever W's rows do not allow TMA (N % 16 != 0 or a
+// misaligned base), W is decoded once into the workspace, with rows padded to a
+// multiple of 8, and read by TMA, so that odd widths take the same tensor-core GEMM
+// as even ones (1 and 2 rows stay with the GEMV where it can).  The backward takes dz
 // in one pass over dout and z (bf16 operand, optional residual part of the
 // split, column sums), then the existing dX and dW GEMMs.
 #include "activation.cuh"
@@ -216,15 +217,24 @@ int dz_launch(int a, const void* dout, const void* z, long long M, long long N, 
 
 // ------------------------------------------------------------------ plans
 enum Route { GEMV, SKINNY_MMA, SKINNY, PLAIN };
-// Rows of the mma.sync route, where W's layout allows its TMA.  Measured (us; 11008
-// -> 4096 / 4096 -> 11008 / 1024 -> 4096): 2 rows 29.5 / 29.5 / 8.6 with it, 34.2 /
-// 27.6 / 7.4 with the GEMV; 3 and 4 rows 29.8 / 29.3 / 8.8 and 40.7 / 32.3 / 9.4; 16
-// rows 31.8 / 30.9 / 9.9 with it, 42.2 / 41.6 / 13.1 with the tcgen05 skinny GEMM.
-// (24 rows in a four-group instance: 46.9 against 42.3.)
-constexpr long long kSkinnyMmaMinM = 3, kSkinnyMmaMaxM = 16;
+// The mma.sync route's rows, where W's layout allows its TMA.  Measured (us in a
+// graph; 11008 -> 4096 / 4096 -> 11008 / 1024 -> 4096): 16 rows 29.3 / 28.7 / 8.4
+// with it, 40.2 / 40.4 / 12.0 with the tcgen05 skinny GEMM (24 rows in a four-group
+// instance: 46.9 against 42.3); 3 rows 27.4 / 27.1 / 7.3 with it, 40.8 / 32.0 / 8.7
+// with the GEMV.  2 rows 27.3 / 27.1 / 7.3 and 34.3 / 27.4 / 7.3, 1 row 27.2 / 27.1 /
+// 7.1 and 29.7 / 25.1 / 6.7: the GEMV cuts K over at most 16 CTAs, which a long
+// reduction leaves uneven (16384 -> 256, 1 row: 12.9 and 17.3; 8192 -> 2048: 14.2 and
+// 17.0), and is ahead where it is one launch's latency that counts (1024 x 1024, 2
+// rows: 5.8 and 5.0; 4096 x 4096: 14.4 and 16.1).
+constexpr long long kSkinnyMmaMaxM = 16;
+inline bool skinny_mma_pays(long long M, long long K, long long N) {
+  if (M > kSkinnyMmaMaxM) return false;
+  if (M >= 3) return true;
+  return M == 2 ? K >= 8192 || K * N >= 1 << 23 : K >= 8192 && K >= 2 * N;
+}
 
 inline Route route(long long M, long long K, long long N, const uint8_t* W_p, const uint16_t* W_f) {
-  if (M >= kSkinnyMmaMinM && M <= kSkinnyMmaMaxM && gemm::wtma_ok(W_p, W_f, N)) return SKINNY_MMA;
+  if (skinny_mma_pays(M, K, N) && gemm::wtma_ok(W_p, W_f, N)) return SKINNY_MMA;
   if (linear::skinny_eligible(M, N) && gemm::wtma_ok(W_p, W_f, N)) return SKINNY;
   if (gemv::eligible(M, K, N, W_p, W_f)) return GEMV;
   return PLAIN;

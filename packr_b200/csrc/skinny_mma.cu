@@ -1,4 +1,4 @@
-// The fused linear layer's forward for 3 to 16 rows, where streaming W once is
+// The fused linear layer's forward for up to 16 rows, where streaming W once is
 // the bound (3 bytes a weight):
 //   out^T[n, m] = sum over k of W[k, n] x[m, k]
 // TMA brings 64 x 128 tiles of W_f and W_p (and the 64-column tile of x) into a
@@ -8,9 +8,10 @@
 // stage stays taken from its TMA over the decode, which writes it back to shared
 // memory, to the end of its MMAs, three latencies in turn, and six stages cover
 // only half of HBM's rate; here a stage turns over with its TMA, and the tensor
-// rate of mma.sync is far from the bound.  16 x 11008 -> 4096 (135 MB of W): 31.8
-// us with the reduction, 4.3 TB/s, against 42.2 us.  What bounds it now is the
-// decode's instructions (8 rows, half the MMAs: 29.7 us).
+// rate of mma.sync is far from the bound.  16 x 11008 -> 4096 (135 MB of W): 29.3
+// us with the reduction, 4.6 TB/s, against 40.2 us.  An SM streams at 5.7 TB/s'
+// share while its CTA lives (23.6 us); the rest is the start, the sums' last adds
+// and the reduction (1 row: 27.2 us).
 //
 // Lane (g, t) = (lane / 4, lane % 4) of a warp takes, of 16 rows and 64 columns of
 // a stage, rows 2t, 2t + 1, 2t + 8, 2t + 9 (the MMA's k order) and columns 8g ..
@@ -311,13 +312,22 @@ __global__ void __launch_bounds__(128) skinny_mma_reduce_kernel(const float* __r
   // the first range may have begun in an earlier tile; the others begin in this one
   const int slot0 = tile - sm_start(plan, c0) / plan.k_blocks;
   wait_previous_kernel();
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(p + ((long long)c * plan.slots + (c == c0 ? slot0 : 0)) * slot_floats));
-    s[0] = __fadd_rn(s[0], v.x);
-    s[1] = __fadd_rn(s[1], v.y);
-    s[2] = __fadd_rn(s[2], v.z);
-    s[3] = __fadd_rn(s[3], v.w);
+  constexpr int kAhead = 8;  // slots in flight
+  for (int c = c0; c <= c1; c += kAhead) {
+    float4 v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (c + i <= c1)
+        v[i] = __ldcg(reinterpret_cast<const float4*>(
+            p + ((long long)(c + i) * plan.slots + (c + i == c0 ? slot0 : 0)) * slot_floats));
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (c + i > c1) break;
+      s[0] = __fadd_rn(s[0], v[i].x);
+      s[1] = __fadd_rn(s[1], v[i].y);
+      s[2] = __fadd_rn(s[2], v[i].z);
+      s[3] = __fadd_rn(s[3], v[i].w);
+    }
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {

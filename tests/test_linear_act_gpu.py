@@ -468,3 +468,13 @@ def test_c_entry_refuses_a_small_workspace_and_a_misaligned_x(cuda):
         assert fwd(x, ws.data_ptr() + 16, need) == 4 and fwd(x + 2, ws.data_ptr(), need) == 3
         torch.cuda.synchronize()
         assert not out.any()  # nothing ran
+
+
+@pytest.mark.parametrize("xt,out", [(BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("M,K,N", [(1, 8192, 272), (2, 8200, 16), (2, 4100, 2064), (1, 9001, 1040), (5, 16400, 144),
+                                   (16, 20000, 16)])
+def test_few_rows_of_a_long_reduction(cuda, M, K, N, xt, out):
+    """One tile's sum is cut into up to one share per SM."""
+    c = case(M, K, N, xt, out, seed=M + K)
+    for act in ("none", "gelu"):
+        compare(c, {"out": call(c, act, out)}, act, out)
