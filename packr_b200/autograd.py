@@ -203,7 +203,8 @@ def packr_linear_act(x, W_p, W_f, lut, bias=None, activation=None, residual=None
     W = bf16(W_f + bf16(lut[W_p])) at every row count.  With bf16 x the
     gradient of the pre-activation enters the weight and lut gradients rounded
     to bf16, as in PackRLinear; with f32 x as bf16 hi + lo parts
-    (PACKR_DW_PRECISION)."""
+    (PACKR_DW_PRECISION).  The f32 lut gradient is short by about 1e-9 of itself
+    per token (the tensor cores truncate the sums it is taken from)."""
     if not x.is_cuda:
         raise RuntimeError("packr_linear_act runs on CUDA tensors only (no CPU path in the B200 build)")
     act = _lib.ACTIVATIONS.get("none" if activation is None else activation)
