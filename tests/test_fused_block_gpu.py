@@ -142,3 +142,85 @@ def test_add_norm_of_mixed_types(cuda, dense, given):
     got = PackRAddNorm(lin, norm)(x, r)
     want = norm(lin(x).float() + r.float())
     assert got.dtype == F32 and torch.allclose(got, want, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("M", [1, 2, 8, 40, 200])
+def test_chain_of_overlapped_launches(cuda, M):
+    """Eight pre-norm blocks in a row, each kernel reading what the one before it
+    wrote: in a stream, in a graph and with a synchronisation after every call the
+    results are the same bits, also right after the input and a weight were
+    overwritten in place."""
+    K, H = 512, 2048
+    ups = [packr.PackRLinear.synthetic(K, H, seed=i, lut_std=0.05, wf_std=0.005) for i in range(8)]
+    downs = [packr.PackRLinear.synthetic(H, K, seed=50 + i, lut_std=0.02, wf_std=0.005) for i in range(8)]
+    for lin in ups + downs:
+        lin.out_dtype = BF16
+    for lin in ups:
+        lin.activation = "silu"
+    norms = [packr.PackRLayerNorm(K, dtype=BF16, device="cuda") for _ in range(8)]
+    g = torch.Generator(device="cuda").manual_seed(M)
+    xs = [torch.randn(M, K, generator=g, device="cuda").bfloat16() for _ in range(3)]
+    x = xs[0].clone()
+
+    @torch.no_grad()
+    def chain(each=lambda: None):
+        h = x
+        for norm, up, down in zip(norms, ups, downs):
+            n = norm(h)
+            each()
+            a = up(n)
+            each()
+            h = down(a, residual=h)
+            each()
+        return h
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        chain()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain()
+    for new in xs:
+        with torch.no_grad():
+            norms[0].weight.mul_(1.25)
+            ups[3].W_f.mul_(1.5)
+        x.copy_(new)
+        got = [chain() for _ in range(3)]
+        graph.replay()
+        got.append(out.clone())
+        torch.cuda.synchronize()
+        want = chain(torch.cuda.synchronize)
+        for y in got:
+            assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("M", [1, 8, 40])
+def test_overlapped_launches_after_a_copy_and_on_two_streams(cuda, M):
+    """The kernel in front is a copy, a fill or another stream's; the one behind
+    overwrites the inputs."""
+    lin = packr.PackRLinear.synthetic(2048, 4096, seed=1, lut_std=0.05, wf_std=0.005)
+    lin.out_dtype = BF16
+    norm = packr.PackRLayerNorm(4096, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(M)
+    host = [torch.randn(M, 2048, generator=g, device="cuda").bfloat16().cpu().pin_memory() for _ in range(4)]
+
+    @torch.no_grad()
+    def f(x):
+        return norm(lin(x))
+
+    want = [f(h.cuda()) for h in host]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    bufs = [torch.empty(M, 2048, dtype=BF16, device="cuda") for _ in streams]
+    got = []
+    for rep in range(8):
+        for s, x in zip(streams, bufs):
+            with torch.cuda.stream(s):
+                x.copy_(host[rep % 4], non_blocking=True)
+                got.append(f(x))
+                x.zero_()
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i // 2 % 4])
