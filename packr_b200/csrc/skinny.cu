@@ -428,7 +428,6 @@ int skinny_forward(const uint16_t* x_bf16, long long ldx, const uint8_t* W_p, co
 __global__ void __launch_bounds__(256) skinny_reduce_epi_kernel(const float* __restrict__ partial, int splits, int M,
                                                                 int N, const void* __restrict__ bias, int bias_f32,
                                                                 const Epilogue epi) {
-  let_next_kernel_start();
   const int qpr = N / 4;
   const long long q = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (q >= (long long)M * qpr) return;
@@ -442,6 +441,7 @@ __global__ void __launch_bounds__(256) skinny_reduce_epi_kernel(const float* __r
     for (int j = 0; j < 4; ++j) r[j] = load_io(epi.residual, o + j, epi.io_f32);
   }
   wait_previous_kernel();
+  let_next_kernel_start();
   int sp = 0;
   for (; sp + 4 <= splits; sp += 4) {  // four splits in flight
     float4 v[4];

@@ -293,8 +293,6 @@ __global__ void __launch_bounds__(128) skinny_mma_reduce_kernel(const float* __r
                                                                 int slot_floats, const SmPlan plan,
                                                                 const void* __restrict__ bias, int bias_f32,
                                                                 const Epilogue epi) {
-  // (what a next call's kernel reads and writes, it does after this one's end)
-  let_next_kernel_start();
   const int qpr = N / 4;
   const long long q = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (q >= (long long)M * qpr) return;
@@ -312,6 +310,7 @@ __global__ void __launch_bounds__(128) skinny_mma_reduce_kernel(const float* __r
   // the first range may have begun in an earlier tile; the others begin in this one
   const int slot0 = tile - sm_start(plan, c0) / plan.k_blocks;
   wait_previous_kernel();
+  let_next_kernel_start();
   constexpr int kAhead = 8;  // slots in flight
   for (int c = c0; c <= c1; c += kAhead) {
     float4 v[kAhead];
