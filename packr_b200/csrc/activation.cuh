@@ -120,6 +120,11 @@ struct Epilogue {
 __device__ __forceinline__ float load_io(const void* p, long long i, int f32) {
   return f32 ? __ldg(static_cast<const float*>(p) + i) : bf16_to_f32(__ldg(static_cast<const uint16_t*>(p) + i));
 }
+// The same for kernels that may start before their inputs are written
+// (launch_overlapped).
+__device__ __forceinline__ float load_io_late(const void* p, long long i, int f32) {
+  return f32 ? __ldcg(static_cast<const float*>(p) + i) : bf16_to_f32(__ldcg(static_cast<const uint16_t*>(p) + i));
+}
 __device__ __forceinline__ void store_io(void* p, long long i, int f32, float v) {
   if (f32)
     static_cast<float*>(p)[i] = v;

@@ -23,10 +23,21 @@ int check_device();
 int launch_status();
 
 // Launches a kernel that may be set up while the previous kernel of the stream
-// still runs; it waits for that kernel's end itself (griddepcontrol.wait) before
-// it touches memory.  Saves the launch latency between two kernels, about 2 us.
-// A kernel that lets the next one start early does so after its own wait, so that
-// whoever waits for it has waited for all that came before.
+// still runs and that waits for that kernel's end itself (griddepcontrol.wait).
+// Saves the launch latency between two kernels, about 2 us.  The rules that keep
+// such a chain in order:
+// * What the kernel in front may write is read, and anything at all is written,
+//   only after the wait.  A kernel that lets the next one start
+//   (launch_dependents) does so after its own wait: whoever starts behind it
+//   starts when all that came before it has ended, and whoever waits for it has
+//   waited for all of that too.  So a kernel that is always launched behind one
+//   that waits first (a reduction behind its split kernel) may read before its own
+//   wait what neither of the two writes: bias and residual.
+// * Such a kernel can begin while its inputs are being written, so they are not
+//   read-only over its life: it reads global memory with coherent loads (__ldcg,
+//   __ldcs, cp.async, TMA; load_io_late), never with __ldg or through a const
+//   __restrict__ pointer, which may be moved above the wait or served from a
+//   line fetched before it.
 template <class... P, class... A>
 int launch_overlapped(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};

@@ -138,24 +138,23 @@ __global__ void __launch_bounds__(kThreads, (MB <= 2 ? PACKR_GEMV_MIN_CTAS : 2))
   const int k0 = rank * rows_per_cta;
   const int k1 = min(K, k0 + rows_per_cta);
   const int nrows_cta = max(0, k1 - k0);
-  // The fused form is set up while the kernel in front of it ends (1 row, 4096 ->
+  // The fused form is set up while the kernel in front of it ends, so it reads
+  // global memory by coherent loads only (launch_overlapped; 1 row, 4096 ->
   // 11008, calls in a row: 26.0 us, 27.7 without).  It does not let the next one
   // start: whose CTAs would take places that this grid leaves free, 26.1 us.
   if (EPI) wait_previous_kernel();
   {
     // thread t loads lut[t] once and writes its 32 lane copies, rotated so
     // that the warp's stores fall in 32 different banks
-    const uint32_t v = EPI ? f32_to_bf16_rne(__ldg(lut + threadIdx.x))
-                           : __float_as_uint(__half2float(__float2half_rn(__ldg(lut + threadIdx.x))));
+    const float entry = __ldcg(lut + threadIdx.x);
+    const uint32_t v = EPI ? f32_to_bf16_rne(entry) : __float_as_uint(__half2float(__float2half_rn(entry)));
 #pragma unroll 8
     for (int l = 0; l < 32; ++l) lut_s[threadIdx.x * 32 + ((l + lane) & 31)] = v;
   }
   for (int i = threadIdx.x; i < nrows_cta * MB; i += kThreads) {
     const int r = i / MB, m = i - r * MB;
     const long long src = (long long)m * K + k0 + r;
-    float v = m >= Mr ? 0.0f
-                      : x_f32 ? __ldg(static_cast<const float*>(x) + src)
-                              : bf16_to_f32(__ldg(static_cast<const uint16_t*>(x) + src));
+    float v = m >= Mr ? 0.0f : load_io_late(x, src, x_f32);
     if (EPI && x_f32) v = __uint_as_float(pack_bf16x2_rne(0.0f, v));
     xs[i] = pk2(v, v);
   }
@@ -274,14 +273,12 @@ __global__ void __launch_bounds__(kThreads, (MB <= 2 ? PACKR_GEMV_MIN_CTAS : 2))
     float t = 0.0f;
     for (int q = 0; q < C; ++q) t = __fadd_rn(t, ld_cluster_f32(sm100::mapa(part_s + 4u * (uint32_t)(m * kCols + c), q)));
     if (m < Mr && n < N) {
-      if (bias != nullptr)
-        t = __fadd_rn(t, bias_f32 ? __ldg(static_cast<const float*>(bias) + n)
-                                  : bf16_to_f32(__ldg(static_cast<const uint16_t*>(bias) + n)));
+      if (bias != nullptr) t = __fadd_rn(t, load_io_late(bias, n, bias_f32));
       const long long o = (long long)m * N + n;
       if (EPI) {
         if (epi.z != nullptr) store_io(epi.z, o, epi.io_f32, t);
         act::apply_all<1>(epi.act, &t);
-        if (epi.residual != nullptr) t = __fadd_rn(t, load_io(epi.residual, o, epi.io_f32));
+        if (epi.residual != nullptr) t = __fadd_rn(t, load_io_late(epi.residual, o, epi.io_f32));
         store_io(epi.out, o, epi.io_f32, t);
       } else {
         out[o] = t;

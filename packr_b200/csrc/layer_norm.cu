@@ -162,9 +162,9 @@ struct Layout {
           d[0] = d[1] = splat(absent);
           if (!any(v)) continue;
           if (f32) {
-            unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(p) + col(v * VW) + k)), d, float());
+            unpack(__ldcg(reinterpret_cast<const uint4*>(static_cast<const float*>(p) + col(v * VW) + k)), d, float());
           } else {
-            const uint2 q = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + col(v * VW) + k));
+            const uint2 q = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + col(v * VW) + k));
             d[0] = pk2(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xFFFF0000u));
             d[1] = pk2(__uint_as_float(q.y << 16), __uint_as_float(q.y & 0xFFFF0000u));
           }
@@ -175,8 +175,8 @@ struct Layout {
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
       float a = absent, b = absent;
-      if (p != nullptr && inside(e)) a = load_io(p, col(e), f32);
-      if (p != nullptr && inside(e + 1)) b = load_io(p, col(e + 1), f32);
+      if (p != nullptr && inside(e)) a = load_io_late(p, col(e), f32);
+      if (p != nullptr && inside(e + 1)) b = load_io_late(p, col(e + 1), f32);
       x[e / 2] = pk2(a, b);
     }
   }
@@ -249,8 +249,8 @@ struct Rows {
           f32x2 f[L::VW / 2];
 #pragma unroll
           for (int j = 0; j < L::VW; j += 2)
-            f[j / 2] = pk2(i + j < total ? Elem<T>::get(p[a][i + j]) : 0.0f,
-                           i + j + 1 < total ? Elem<T>::get(p[a][i + j + 1]) : 0.0f);
+            f[j / 2] = pk2(i + j < total ? Elem<T>::get(__ldcg(p[a] + i + j)) : 0.0f,
+                           i + j + 1 < total ? Elem<T>::get(__ldcg(p[a] + i + j + 1)) : 0.0f);
           q = pack(f, T());
         }
       }
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(TMAX, ctas_per_sm(true, E, TMAX))
   f32x2 w[P];
   l.load_vector(weight, wf, 1.0f, w);
   const float *mean_p = mean_in + row0, *rstd_p = rstd_in + row0;
-  float mean_n = left >= 0 ? __ldg(mean_p) : 0.0f, rstd_n = left >= 0 ? __ldg(rstd_p) : 0.0f;
+  float mean_n = left >= 0 ? __ldcg(mean_p) : 0.0f, rstd_n = left >= 0 ? __ldcg(rstd_p) : 0.0f;
   int parity = 0;
   for (int s = 0; left >= 0; in.at += in.stride, --left, parity ^= 1) {
     if (RING) {
@@ -510,8 +510,8 @@ __global__ void __launch_bounds__(TMAX, ctas_per_sm(true, E, TMAX))
     if (left > 0) {
       mean_p += step;
       rstd_p += step;
-      mean_n = __ldg(mean_p);
-      rstd_n = __ldg(rstd_p);
+      mean_n = __ldcg(mean_p);
+      rstd_n = __ldcg(rstd_p);
     }
     f32x2 h[P], g[P];
     in.template get<false>(l, s, 0, g);

@@ -124,12 +124,13 @@ __global__ void __launch_bounds__(SkCfg<MODE, NPAD>::kThreads, 1)
     tmem_relinquish();
   }
   // may start before the kernel in front of it ends, and lets the reduction
-  // start; every read of global memory comes after the wait
+  // start; every read of global memory comes after the wait, by coherent loads
+  // (launch_overlapped)
   wait_previous_kernel();
   let_next_kernel_start();
   if (warp >= C::kDecWarp0) {
     const int dw = warp - C::kDecWarp0;
-    for (int e = dw; e < 256; e += C::kDecWarps) lut_s[e * 32 + lane] = f32_to_bf16_rne(__ldg(P.dec.lut + e));
+    for (int e = dw; e < 256; e += C::kDecWarps) lut_s[e * 32 + lane] = f32_to_bf16_rne(__ldcg(P.dec.lut + e));
   }
   tc_fence_before();
   __syncthreads();
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(256) skinny_reduce_epi_kernel(const float* __r
   float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (epi.residual != nullptr) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = load_io(epi.residual, o + j, epi.io_f32);
+    for (int j = 0; j < 4; ++j) r[j] = load_io_late(epi.residual, o + j, epi.io_f32);
   }
   wait_previous_kernel();
   let_next_kernel_start();
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(256) skinny_reduce_epi_kernel(const float* __r
   }
   if (bias != nullptr) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = __fadd_rn(s[j], load_io(bias, n + j, bias_f32));
+    for (int j = 0; j < 4; ++j) s[j] = __fadd_rn(s[j], load_io_late(bias, n + j, bias_f32));
   }
   if (epi.z != nullptr) {
 #pragma unroll

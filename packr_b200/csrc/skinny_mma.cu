@@ -137,14 +137,15 @@ __global__ void __launch_bounds__(kSmThreads, 1)
     fence_barrier_init();
   }
   // this kernel may start before the one in front of it ends, and lets the
-  // reduction start; every read of global memory comes after the wait
+  // reduction start; every read of global memory comes after the wait, by
+  // coherent loads (launch_overlapped)
   wait_previous_kernel();
   let_next_kernel_start();
   if (producer)  // the ring's first round, under the lut's set-up
     for (; it < count && it < S; ++it) fill();
   if (warp < 8) {  // entry e of lane l at e * 128 + l * 4, rotated stores
     const int e = threadIdx.x;
-    const uint32_t v = f32_to_bf16_rne(__ldg(lut + e));
+    const uint32_t v = f32_to_bf16_rne(__ldcg(lut + e));
 #pragma unroll 8
     for (int l = 0; l < 32; ++l) *reinterpret_cast<uint32_t*>(lut_b + e * 128 + ((l + lane) & 31) * 4) = v;
   }
@@ -301,8 +302,8 @@ __global__ void __launch_bounds__(128) skinny_mma_reduce_kernel(const float* __r
   float r[4] = {0.0f, 0.0f, 0.0f, 0.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if (epi.residual != nullptr) r[j] = load_io(epi.residual, o + j, epi.io_f32);
-    if (bias != nullptr) b[j] = load_io(bias, n + j, bias_f32);
+    if (epi.residual != nullptr) r[j] = load_io_late(epi.residual, o + j, epi.io_f32);
+    if (bias != nullptr) b[j] = load_io_late(bias, n + j, bias_f32);
   }
   const int tile = n / kSmCols, first = tile * plan.k_blocks, last = first + plan.k_blocks - 1;
   const int c0 = sm_owner(plan, first), c1 = sm_owner(plan, last);

@@ -320,3 +320,58 @@ def test_rows_shorter_than_a_chunk_inside_larger_buffers(cuda, xt, M, N):
                                                  code, p(stats), p(stats) + 4 * M, p(out), None, None, M, N, None, 0, s) == 0
         torch.cuda.synchronize()
         assert torch.equal(out[:M * N].view(M, N), got[name]) and bool((out[M * N:] == 7).all())
+
+
+@pytest.mark.parametrize("M,N,xt,wt", [(1, 4096, BF16, BF16), (300, 768, F32, F32), (2000, 1001, BF16, F32),
+                                       (600, 8192, BF16, BF16), (70, 16384, BF16, F32)])
+def test_training_chain_of_overlapped_launches(cuda, M, N, xt, wt):
+    """Four norms forward, then their backward passes, each kernel set up while the
+    one in front of it writes what it reads (statistics directly before the
+    backward, sums before their reduction), in buffers that the allocator gives out
+    again and with inputs and weights overwritten between the passes: the same bits
+    as with a synchronisation after every call."""
+    cs = [case(M, N, xt, wt, seed=i) for i in range(3)]
+    x = cs[0]["x"].clone().requires_grad_(True)
+    ws = [(cs[0]["weight"].clone().requires_grad_(True), cs[0]["bias"].clone().requires_grad_(True)) for _ in range(4)]
+    leaves = [x] + [t for w in ws for t in w]
+
+    def step(dy):
+        h = x
+        for w, b in ws:
+            h = packr.packr_layer_norm(h, w, b, residual=x)
+        return (h, *torch.autograd.grad(h, leaves, dy))
+
+    def alone(dy):
+        """The same, every backward pass by itself."""
+        hs, h = [], x
+        for w, b in ws:
+            i = h.detach().requires_grad_(True)
+            r = x.detach().requires_grad_(True)
+            o = packr.packr_layer_norm(i, w, b, residual=r)
+            torch.cuda.synchronize()
+            hs.append((i, r, w, b, o))
+            h = o
+        out, d, params = h.detach(), dy, []
+        for i, r, w, b, o in reversed(hs):
+            di, _, dw, db = torch.autograd.grad(o, [i, r, w, b], d)
+            torch.cuda.synchronize()
+            params = [dw, db] + params
+            d = di
+        return out, params
+
+    for c in cs:
+        with torch.no_grad():
+            x.copy_(c["x"])
+            for w, b in ws:
+                w.copy_(c["weight"]).mul_(1.25)
+                b.copy_(c["bias"])
+        dy = c["dy"].clone()
+        got = [step(dy) for _ in range(4)]
+        out, params = alone(dy)
+        torch.cuda.synchronize()
+        for g in got:
+            assert torch.equal(g[0], out)
+            for a, b in zip(g[2:], params):
+                assert torch.equal(a, b)
+        for g in got[1:]:
+            assert torch.equal(g[1], got[0][1])
