@@ -34,14 +34,10 @@
 
 #include "activation.cuh"
 #include "common.cuh"
+#include "layer_norm_shape.cuh"
 
 namespace packr {
 namespace norm {
-
-constexpr int kMaxRowThreads = 1024;
-constexpr long long kMaxRegN = 16LL * kMaxRowThreads;  // widest row held in registers
-constexpr int kMaxGroups = 8;                          // rows in flight per CTA (named barriers 1..8)
-constexpr int kMaxSmem = 220 * 1024;                   // dynamic shared memory a CTA may ask for
 
 template <class T>
 struct Elem;
@@ -322,13 +318,6 @@ __device__ __forceinline__ float group_sum(float v, float* buf, int group, int n
     s += (q.x + q.y) + (q.z + q.w);
   }
   return s;
-}
-
-// CTAs of TMAX threads per SM that the register bounds are set for: 80 registers
-// a thread, 128 where more values are held, 64 with 1024 threads.  Two or three
-// small CTAs hide one another's reductions.
-__host__ __device__ constexpr int ctas_per_sm(bool bwd, int e, int tmax) {
-  return tmax > 256 ? 1 : e == 8 || (e == 16 && !bwd) ? 3 : 2;
 }
 
 template <class T, int E, bool RAGGED, bool RES, int TMAX>
@@ -679,54 +668,10 @@ int reduce_cols(const float* partial, int slabs, int planes, long long N, W* out
 
 constexpr int kWideSlabs = 64;  // row slabs of bwd_wide_cols_kernel
 
-struct Shape {
-  int e, nt, groups, grid, stages;
-  bool ragged;  // rows are not whole 16-byte chunks
-  size_t smem;
-};
-
-// Elements per thread: 8 up to 1024 columns, 16 beyond (fewer threads to reduce
-// over), in the forward 32 beyond 4096 (CTAs of at most 512 threads).  The
-// backward's column sums leave registers for 16 elements only: beyond 4096
-// columns it has one CTA of up to 1024 threads per SM, and beyond 8192 the sums
-// move to shared memory.  Rows per CTA: about 256 threads.  Grid: as many CTAs
-// as registers and shared memory hold, a whole number of phases when rows are
-// not whole chunks.  Ring: up to 3 stages, what fits.
-inline Shape shape(long long M, long long N, int esize, int tensors, bool bwd) {
-  Shape s{};
-  const int vw = 16 / esize;
-  s.e = N <= 1024 ? 8 : N <= 4096 || bwd ? 16 : 32;
-  s.ragged = N % vw != 0;
-  const long long span = s.ragged ? N + vw - 1 : N;
-  s.nt = (int)((span + 32LL * s.e - 1) / (32LL * s.e) * 32);
-  s.groups = 256 / s.nt;
-  s.groups = s.groups < 1 ? 1 : s.groups > kMaxGroups ? kMaxGroups : s.groups;
-  if (s.groups > M) s.groups = (int)M;
-  const int threads = s.nt * s.groups;
-  // column sums: 1024-thread CTAs keep them here, several groups add them here
-  const size_t acc = !bwd ? 0 : s.nt > 512 ? (size_t)2 * s.e * s.nt * 4 : s.groups > 1 ? (size_t)2 * N * 4 : 0;
-  const size_t stage = (size_t)tensors * s.e * esize * threads;  // at most 128 KB, with a ring
-  s.stages = bwd && s.nt > 512 ? 0 : (int)((kMaxSmem - acc) / stage);
-  if (s.stages > 3) s.stages = 3;
-  s.smem = acc + stage * s.stages;
-  const int regs = ctas_per_sm(bwd, s.e, 256) == 3 ? 80 : threads > 512 ? 64 : 128;
-  int per_sm = 65536 / (regs * threads);
-  if (per_sm > 4) per_sm = 4;
-  if (s.smem > 0 && per_sm > (int)(kMaxSmem / s.smem)) per_sm = (int)(kMaxSmem / s.smem);
-  if (per_sm < 1) per_sm = 1;
-  const long long want = (M + s.groups - 1) / s.groups;
-  long long cap = (long long)sm_count() * per_sm;
-  if (s.ragged && want > cap) cap = cap / vw * vw;
-  s.grid = (int)(want < cap ? want : cap);
-  return s;
-}
-// Rows this wide have no register path (a ragged row spans up to 7 more columns).
-inline bool wide(long long N) { return N > kMaxRegN || (N > kMaxRegN - 8 && N % 8 != 0); }
-
 // CTAs of the backward, each leaving one slab of column sums.
 inline int bwd_slabs(long long M, long long N, int esize, bool res, bool vec) {
   if (!vec || wide(N)) return (int)(M < kWideSlabs ? M : kWideSlabs);
-  return shape(M, N, esize, res ? 3 : 2, true).grid;
+  return shape(M, N, esize, res ? 3 : 2, true, sm_count()).grid;
 }
 
 // Raises a kernel's dynamic shared-memory limit to kMaxSmem, once per device
@@ -751,6 +696,7 @@ int launch_fwd(const Shape& s, const void* x, const void* res, const void* w, co
                float* mean, float* rstd, long long M, long long N, cudaStream_t st) {
   auto kern = s.ragged ? fwd_kernel<T, E, true, RES, TMAX> : fwd_kernel<T, E, false, RES, TMAX>;
   static std::atomic<int> done[2][64];
+  if (s.tmax > TMAX) return PACKR_ERR_LAUNCH;  // the rule and the dispatch disagree
   const int rc = allow_smem(kern, s.smem, done[s.ragged]);
   if (rc != PACKR_OK) return rc;
   return launch_overlapped(kern, dim3((unsigned)s.grid), dim3(s.nt, s.groups), s.smem, st, static_cast<const T*>(x),
@@ -767,13 +713,13 @@ int forward(const void* x, const void* res, const void* w, const void* b, int wf
                                                                                mean, rstd, M, N);
     return launch_status();
   }
-  const Shape s = shape(M, N, sizeof(T), res ? 2 : 1, false);
+  const Shape s = shape(M, N, sizeof(T), res ? 2 : 1, false, sm_count());
 #define PACKR_NORM_FWD(E, TMAX)                                                              \
   return res ? launch_fwd<T, E, true, TMAX>(s, x, res, w, b, wf, eps, y, mean, rstd, M, N, st) \
              : launch_fwd<T, E, false, TMAX>(s, x, res, w, b, wf, eps, y, mean, rstd, M, N, st)
   if (s.e == 8) PACKR_NORM_FWD(8, 256);
   if (s.e == 16) PACKR_NORM_FWD(16, 256);
-  if (s.nt <= 256) PACKR_NORM_FWD(32, 256);
+  if (s.tmax == 256) PACKR_NORM_FWD(32, 256);
   PACKR_NORM_FWD(32, 512);
 #undef PACKR_NORM_FWD
 }
@@ -783,6 +729,7 @@ int launch_bwd(const Shape& s, const void* dy, const void* x, const void* res, c
                const float* rstd, void* dx, float* partial, long long M, long long N, cudaStream_t st) {
   auto kern = s.ragged ? bwd_kernel<T, E, true, RES, TMAX> : bwd_kernel<T, E, false, RES, TMAX>;
   static std::atomic<int> done[2][64];
+  if (s.tmax > TMAX) return PACKR_ERR_LAUNCH;  // the rule and the dispatch disagree
   const int rc = allow_smem(kern, s.smem, done[s.ragged]);
   if (rc != PACKR_OK) return rc;
   return launch_overlapped(kern, dim3((unsigned)s.grid), dim3(s.nt, s.groups), s.smem, st, static_cast<const T*>(dy),
@@ -815,15 +762,15 @@ int backward(const void* dy, const void* x, const void* res, const void* w, int 
       rc = launch_status();
     }
   } else {
-    const Shape s = shape(M, N, sizeof(T), res ? 3 : 2, true);
+    const Shape s = shape(M, N, sizeof(T), res ? 3 : 2, true, sm_count());
 #define PACKR_NORM_BWD(E, TMAX)                                                                  \
   rc = res ? launch_bwd<T, E, true, TMAX>(s, dy, x, res, w, wf, mean, rstd, dx, partial, M, N, st) \
            : launch_bwd<T, E, false, TMAX>(s, dy, x, res, w, wf, mean, rstd, dx, partial, M, N, st)
     if (s.e == 8)
       PACKR_NORM_BWD(8, 256);
-    else if (s.nt <= 256)
+    else if (s.tmax == 256)
       PACKR_NORM_BWD(16, 256);
-    else if (s.nt <= 512)
+    else if (s.tmax == 512)
       PACKR_NORM_BWD(16, 512);
     else
       PACKR_NORM_BWD(16, 1024);

@@ -375,3 +375,17 @@ def test_training_chain_of_overlapped_launches(cuda, M, N, xt, wt):
                 assert torch.equal(a, b)
         for g in got[1:]:
             assert torch.equal(g[1], got[0][1])
+
+
+# both sides of the widths where the launch rule changes: 1024, 4096, 8192 and
+# 16384 columns, and the ragged rows just below, which cover more than they have
+EDGES = [1017, 1023, 1024, 1025, 4089, 4090, 4093, 4094, 4095, 4097, 8185, 8191, 16369, 16375, 16376, 16377]
+
+
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("xt,wt", [(BF16, F32), (F32, F32)])
+@pytest.mark.parametrize("N", EDGES)
+def test_widths_around_the_thresholds(cuda, N, xt, wt, residual):
+    c = case(9, N, xt, wt, seed=N, residual=residual)
+    compare(c, run(c))
+    compare(c, run(c, need=()))
