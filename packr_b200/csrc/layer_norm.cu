@@ -508,8 +508,8 @@ __global__ void __launch_bounds__(TMAX, ctas_per_sm(true, E, TMAX))
     if (RES) in.template get<true>(l, s, RES ? 2 : 0, h);
 #pragma unroll
     for (int k = 0; k < P; ++k) h[k] = mul2(sub2(h[k], mean), rstd);
-    if (RAGGED) l.clear_outside(g);
-    if (RAGGED) l.clear_outside(h);  // whole chunks outside the row: g is zero there
+    if (RAGGED) l.clear_outside(g);  // whole chunks outside the row read as zero
+    l.clear_outside(h);  // -mean * rstd there, whose product with g's zeros may be a NaN
     f32x2 s1 = 0ull, s2 = 0ull;
 #pragma unroll
     for (int k = 0; k < P; ++k) {

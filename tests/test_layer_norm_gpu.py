@@ -389,3 +389,25 @@ def test_widths_around_the_thresholds(cuda, N, xt, wt, residual):
     c = case(9, N, xt, wt, seed=N, residual=residual)
     compare(c, run(c))
     compare(c, run(c, need=()))
+
+
+@pytest.mark.parametrize("xt", [BF16, F32])
+@pytest.mark.parametrize("N", [16, 64, 512, 2048, 8192, 16384])
+def test_gradients_of_huge_constant_rows(cuda, N, xt):
+    """mean * rstd past f32's range: h is zero all the same, and what a thread holds
+    outside the row adds nothing.  N is a power of two, so the mean is exact;
+    dx = rstd * (g - mean(g)), sums of N products: 2^-17 of the largest covers them
+    in f32, half a step more in bf16."""
+    g = torch.Generator(device="cuda").manual_seed(N)
+    x = torch.full((5, N), 2.0 ** 112, device="cuda").to(xt)  # 2^112 * 2^14 columns stays finite
+    x[1] = 0.0
+    w = torch.randn(N, generator=g, device="cuda")
+    dy = torch.randn(5, N, generator=g, device="cuda").to(xt)
+    eps = 1e-12
+    assert 2.0 ** 112 * eps ** -0.5 > torch.finfo(F32).max
+    got = run({"x": x, "residual": None, "weight": w, "bias": torch.zeros_like(w), "dy": dy}, eps=eps)
+    assert not got["y"].any() and not got["dweight"].any()
+    gw = dy.double() * w.double()
+    want = (gw - gw.mean(1, keepdim=True)) * eps ** -0.5
+    off = (got["dx"].double() - want).abs()
+    assert (off <= 2.0 ** -17 * want.abs().max() + torch.finfo(xt).eps / 2 * want.abs()).all()
