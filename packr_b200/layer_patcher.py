@@ -4,6 +4,7 @@ fuse_epilogues, which moves what a model computes around its packed layers
 (activation, residual sum, layer norm) into their kernels."""
 from __future__ import annotations
 
+import collections
 import copy
 import inspect
 import operator
@@ -262,18 +263,20 @@ def fuse_epilogues(model: nn.Module):
     paths, is seen to do just that: one that gates, normalises or splits the
     layer's output first, uses the activation a second time, takes optional
     arguments (decoder layers that hold fc1 themselves) or cannot be followed
-    stays as it is.  A block without a forward of its own is taken when it is the
-    model itself.
+    stays as it is, and so does a layer that more than one block holds.  A block
+    without a forward of its own is taken when it is the model itself.
 
     Activations other than relu, gelu (either form) and silu stay as they are,
     and so do norms whose weights are neither f32 nor bf16.
     Parameters, their names and the model's results (up to rounding) do not
     change.  Returns the model."""
+    holders = collections.Counter(id(m) for parent in model.modules() for m in parent._modules.values())
     for name, module in list(model.named_modules()):
         for layer, act in _ACTIVATED:
             lin = getattr(module, layer, None)
             known = _activation_name(getattr(module, act, None))
-            if isinstance(lin, PackRLinear) and lin.activation is None and known is not None:
+            if (isinstance(lin, PackRLinear) and lin.activation is None and known is not None
+                    and holders[id(lin)] == 1):
                 if not (_only_activates(module, layer, act) if _own_forward(module)
                         else name == "" and not isinstance(module, nn.ModuleDict)):
                     continue

@@ -224,3 +224,14 @@ def test_which_add_norm_blocks_are_replaced(forward, taken):
     model = nn.Sequential(add_norm(forward)())
     packr.fuse_epilogues(model)
     assert isinstance(model[0], packr.PackRAddNorm) == taken
+
+
+def test_a_layer_that_two_blocks_hold_is_left_alone():
+    """Its activation would be applied by the layer and again by the other block."""
+    a, b = Mlp(), Mlp()
+    b.fc1 = a.fc1
+    for model in (nn.Sequential(a, b), nn.Sequential(a, a.fc1)):
+        packr.fuse_epilogues(model)
+        assert a.fc1.activation is None and isinstance(a.activation_fn, nn.GELU) and isinstance(b.activation_fn, nn.GELU)
+    # the same block in two places is one holder
+    assert packr.fuse_epilogues(nn.Sequential(a, a))[0].fc1.activation == "gelu"
