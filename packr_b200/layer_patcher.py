@@ -142,6 +142,13 @@ class _Tracer(torch.fx.Tracer):
         return self.asked <= len(self.decisions) and self.decisions[self.asked - 1]
 
 
+def _hooked(module):
+    """Whether somebody watches or replaces what `module` computes."""
+    return isinstance(module, nn.Module) and bool(
+        "forward" in module.__dict__ or module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+        or module._backward_pre_hooks)
+
+
 def _own_forward(module):
     """Whether the module's class computes something of its own when called."""
     return type(module).forward is not nn.Module.forward
@@ -154,7 +161,7 @@ def _paths(module, parameters, **markers):
     exactly `parameters` arguments without defaults are, as a test for None or for
     a type cannot be seen in a trace."""
     forward = type(module).forward
-    if "forward" in module.__dict__:
+    if "forward" in module.__dict__:  # not the class's
         return None
     ps = list(inspect.signature(forward).parameters.values())[1:]
     if len(ps) != parameters or any(p.default is not p.empty or p.kind is not p.POSITIONAL_OR_KEYWORD for p in ps):
@@ -264,7 +271,10 @@ def fuse_epilogues(model: nn.Module):
     layer's output first, uses the activation a second time, takes optional
     arguments (decoder layers that hold fc1 themselves) or cannot be followed
     stays as it is, and so does a layer that more than one block holds.  A block
-    without a forward of its own is taken when it is the model itself.
+    without a forward of its own is taken when it is the model itself.  Where the
+    layer, the activation, the norm or a block that would be replaced carries hooks
+    (or a forward set on the instance), they would see other values or none at all,
+    so it stays too.
 
     Activations other than relu, gelu (either form) and silu stay as they are,
     and so do norms whose weights are neither f32 nor bf16.
@@ -276,7 +286,7 @@ def fuse_epilogues(model: nn.Module):
             lin = getattr(module, layer, None)
             known = _activation_name(getattr(module, act, None))
             if (isinstance(lin, PackRLinear) and lin.activation is None and known is not None
-                    and holders[id(lin)] == 1):
+                    and holders[id(lin)] == 1 and not _hooked(lin) and not _hooked(getattr(module, act))):
                 if not (_only_activates(module, layer, act) if _own_forward(module)
                         else name == "" and not isinstance(module, nn.ModuleDict)):
                     continue
@@ -290,6 +300,7 @@ def fuse_epilogues(model: nn.Module):
             # a block without a forward of its own: its submodules keep what they do
             if (type(norm) is nn.LayerNorm and len(norm.normalized_shape) == 1
                     and (norm.weight is None or norm.weight.dtype in (torch.float32, torch.bfloat16))
+                    and not _hooked(module) and not _hooked(norm)
                     and (not _own_forward(module) or _only_adds_and_normalises(module))):
                 fused = PackRAddNorm(module.dense, norm, module.dropout)
                 fused.train(module.training)

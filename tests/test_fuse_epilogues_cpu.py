@@ -235,3 +235,36 @@ def test_a_layer_that_two_blocks_hold_is_left_alone():
         assert a.fc1.activation is None and isinstance(a.activation_fn, nn.GELU) and isinstance(b.activation_fn, nn.GELU)
     # the same block in two places is one holder
     assert packr.fuse_epilogues(nn.Sequential(a, a))[0].fc1.activation == "gelu"
+
+
+HOOKS = ["register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook",
+         "register_full_backward_pre_hook", "forward"]
+
+
+def watch(module, how):
+    if how == "forward":
+        module.forward = type(module).forward.__get__(module)
+    else:
+        getattr(module, how)(lambda *a: None)
+
+
+@pytest.mark.parametrize("how", HOOKS)
+def test_watched_modules_are_left_alone(how):
+    for part in ("fc1", "activation_fn"):
+        b = Mlp()
+        watch(getattr(b, part), how)
+        assert not fused(b), part
+    b = Mlp()
+    watch(b.fc2, how)  # a part that stays as it is
+    assert fused(b)
+    for part in (None, "LayerNorm"):
+        model = nn.Sequential(add_norm(lambda self, h, x: self.LayerNorm(self.dropout(self.dense(h)) + x))())
+        watch(model[0] if part is None else model[0].LayerNorm, how)
+        before = model[0]
+        packr.fuse_epilogues(model)
+        assert model[0] is before, part
+    model = nn.Sequential(add_norm(lambda self, h, x: self.LayerNorm(self.dropout(self.dense(h)) + x))())
+    watch(model[0].dense, how)
+    dense = model[0].dense
+    packr.fuse_epilogues(model)
+    assert isinstance(model[0], packr.PackRAddNorm) and model[0].dense is dense
