@@ -49,30 +49,23 @@ def grad_sink(param: torch.Tensor) -> torch.Tensor | None:
     n = param.numel()
     if buf.dtype != param.dtype or buf.device != param.device or off + n > buf.numel():
         return None
-    lent = getattr(param, "_packr_grad_lent", None)
-    if lent is None:
-        lent = param._packr_grad_lent = _Lent()
-    if lent.held():
-        return None
+    key = id(param)
+    lent = _lent.get(key)
+    if lent is not None and lent[0]() is param:
+        if lent[1]() is not None:
+            return None
+        owner = lent[0]
+    else:
+        owner = weakref.ref(param, lambda _: _lent.pop(key, None))
     view = buf[off:off + n].view(param.shape)
-    lent.ref = weakref.ref(view)
+    _lent[key] = owner, weakref.ref(view)
     return view
 
 
-class _Lent:
-    """The last view of a gradient buffer that was given out; copies and
-    pickles start empty (a weak reference has no place in a saved model)."""
-
-    __slots__ = ("ref",)
-
-    def __init__(self):
-        self.ref = None
-
-    def held(self) -> bool:
-        return self.ref is not None and self.ref() is not None
-
-    def __reduce__(self):
-        return _Lent, ()
+# id of a parameter -> (the parameter, the last view of its gradient buffer that
+# was given out), both weak.  Not an attribute of the parameter, which would have
+# to be saved and loaded with it.
+_lent: dict = {}
 
 
 def _forward_keep_w(ctx, x, W_p, W_f, lut, bias):

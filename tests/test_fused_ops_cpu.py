@@ -276,3 +276,20 @@ def test_a_parameter_with_a_buffer_can_be_copied():
     _Scale.apply(torch.ones(4), w).sum().backward()
     assert torch.equal(copy.deepcopy(w), w)
     assert torch.equal(pickle.loads(pickle.dumps(w)), w)
+
+
+def test_a_parameter_with_a_buffer_can_be_saved_and_loaded(tmp_path):
+    """With torch.load's default, which takes tensors and plain values only."""
+    w, _ = _parameter_with_sink()
+    _Scale.apply(torch.ones(4), w).sum().backward()
+    torch.save({"w": w}, tmp_path / "w.pt")
+    assert torch.equal(torch.load(tmp_path / "w.pt")["w"], w)
+
+
+def test_a_copied_parameter_has_a_loan_of_its_own():
+    w, _ = _parameter_with_sink()
+    c = pickle.loads(pickle.dumps(w))
+    x = torch.arange(4.0)
+    g, = torch.autograd.grad(_Scale.apply(x, w).sum(), w)  # w's buffer is lent
+    _Scale.apply(x, c).sum().backward()
+    assert c.grad.data_ptr() == c._packr_grad_sink[0][2:].data_ptr() and torch.equal(g, x)
