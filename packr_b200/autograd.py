@@ -197,7 +197,9 @@ def packr_linear_act(x, W_p, W_f, lut, bias=None, activation=None, residual=None
     gradient of the pre-activation enters the weight and lut gradients rounded
     to bf16, as in PackRLinear; with f32 x as bf16 hi + lo parts
     (PACKR_DW_PRECISION).  The f32 lut gradient is short by about 1e-9 of itself
-    per token (the tensor cores truncate the sums it is taken from)."""
+    per token (the tensor cores truncate the sums it is taken from).
+    Backward mode, once: second and forward-mode derivatives are refused."""
+    _k.refuse_tangents("packr_linear_act", x, W_f, lut, bias, residual)
     if not x.is_cuda:
         raise RuntimeError("packr_linear_act runs on CUDA tensors only (no CPU path in the B200 build)")
     act = _lib.ACTIVATIONS.get("none" if activation is None else activation)

@@ -19,6 +19,7 @@ import ctypes
 import os
 
 import torch
+import torch.autograd.forward_ad as _fwd_ad
 
 from . import _lib
 
@@ -65,6 +66,13 @@ def _ptr(t):
 def _addr(t) -> int | None:
     """The tensor's address as a plain number (ctypes converts it), or None."""
     return None if t is None else t.data_ptr()
+
+
+def refuse_tangents(op: str, *tensors) -> None:
+    """Raises when a tensor carries a forward-mode derivative, which a kernel that
+    is called past autograd would drop (the result's would read as zero)."""
+    if _fwd_ad._current_level >= 0 and any(t is not None and _fwd_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{op}: forward-mode derivatives are not implemented")
 
 
 def _workspace(nbytes: int, device) -> torch.Tensor | None:

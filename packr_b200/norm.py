@@ -18,7 +18,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernel import _addr, _on_device, _raw_stream
+from .kernel import _addr, _on_device, _raw_stream, refuse_tangents
 
 _F32, _BF16 = torch.float32, torch.bfloat16
 _CODE = {_F32: _lib.PACKR_DTYPE_F32, _BF16: _lib.PACKR_DTYPE_BF16}
@@ -103,7 +103,9 @@ def packr_layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
         bias:     [N] of weight's dtype, or None
         eps:      added to the variance
         residual: tensor of x's shape and dtype added to x first, or None
-    """
+
+    Backward mode, once: second and forward-mode derivatives are refused."""
+    refuse_tangents("packr_layer_norm", x, weight, bias, residual)
     if not x.is_cuda:
         raise RuntimeError("packr_layer_norm runs on CUDA tensors only (no CPU path in the B200 build)")
     if x.dtype not in _CODE:

@@ -293,3 +293,26 @@ def test_a_copied_parameter_has_a_loan_of_its_own():
     g, = torch.autograd.grad(_Scale.apply(x, w).sum(), w)  # w's buffer is lent
     _Scale.apply(x, c).sum().backward()
     assert c.grad.data_ptr() == c._packr_grad_sink[0][2:].data_ptr() and torch.equal(g, x)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(grad):
+    """No input requires a gradient, so the operators call their kernels past
+    autograd; a tangent must not be dropped there.  Refused before the device is
+    looked at."""
+    from torch.autograd import forward_ad
+    x, w = torch.ones(2, 8), torch.ones(8)
+    W_p, W_f = torch.zeros(8, 4, dtype=torch.uint8), torch.zeros(8, 4, dtype=torch.bfloat16)
+    lut, bias, res = torch.zeros(256), torch.zeros(4), torch.zeros(2, 4)
+    norm = dict(x=x, weight=w, bias=w, residual=x)
+    lin = dict(x=x, W_p=W_p, W_f=W_f, lut=lut, bias=bias, residual=res)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        for f, args in ((packr.packr_layer_norm, norm), (packr.packr_linear_act, lin)):
+            with pytest.raises(RuntimeError, match="CUDA"):  # nothing dual: the usual checks
+                f(**args)
+            for name, t in args.items():
+                if t.is_floating_point():
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        f(**{**args, name: forward_ad.make_dual(t, torch.ones_like(t))})
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            packr.PackRLayerNorm(8)(forward_ad.make_dual(x, x))
