@@ -145,7 +145,8 @@ def _check_vector(name, t, x):
 class PackRLayerNorm(nn.LayerNorm):
     """nn.LayerNorm over one dimension, run by packr_layer_norm; forward takes
     an optional residual that is added to the input first (post-norm blocks:
-    norm(dense(x), residual=x))."""
+    norm(dense(x), residual=x)).  Under autocast it is computed and returned in
+    f32, as nn.LayerNorm is."""
 
     def __init__(self, normalized_shape, eps=1e-5, elementwise_affine=True, bias=True, device=None, dtype=None):
         super().__init__(normalized_shape, eps=eps, elementwise_affine=elementwise_affine, bias=bias, device=device,
@@ -156,6 +157,10 @@ class PackRLayerNorm(nn.LayerNorm):
     def forward(self, x, residual=None):
         if x.shape[-1:] != torch.Size(self.normalized_shape):
             raise ValueError(f"PackRLayerNorm: last dimension {tuple(x.shape[-1:])} != {tuple(self.normalized_shape)}")
+        if torch.is_autocast_enabled(x.device.type):
+            # f64 stays (and is refused), as autocast leaves it
+            x = x.float() if x.dtype != torch.float64 else x
+            residual = residual.float() if residual is not None and residual.dtype != torch.float64 else residual
         return packr_layer_norm(x, self.weight, self.bias, self.eps, residual)
 
     @classmethod

@@ -316,3 +316,29 @@ def test_forward_mode_derivatives_are_refused(grad):
                         f(**{**args, name: forward_ad.make_dual(t, torch.ones_like(t))})
         with pytest.raises(NotImplementedError, match="forward-mode"):
             packr.PackRLayerNorm(8)(forward_ad.make_dual(x, x))
+
+
+def test_norm_module_follows_autocast(monkeypatch):
+    """What reaches the operator: nn.LayerNorm's types, f32 under autocast."""
+    from packr_b200 import norm
+    seen = []
+
+    def plain(x, weight=None, bias=None, eps=1e-5, residual=None):
+        seen.append((x.dtype, None if residual is None else residual.dtype))
+        s = x if residual is None else x + residual
+        return torch.nn.functional.layer_norm(s, s.shape[-1:], None, None, eps)
+
+    monkeypatch.setattr(norm, "packr_layer_norm", plain)
+    m, ref = packr.PackRLayerNorm(8), torch.nn.LayerNorm(8)
+    bf, f16, f32 = torch.bfloat16, torch.float16, torch.float32
+    x = torch.randn(2, 8)
+    for dtype in (bf, f16, f32):
+        with torch.autocast("cpu", dtype=bf):
+            assert m(x.to(dtype), residual=x.to(bf)).dtype == f32 and seen[-1] == (f32, f32)
+            assert m(x.to(dtype)).dtype == f32 and seen[-1] == (f32, None)
+    with torch.autocast("cpu", dtype=bf, enabled=False):
+        assert m(x.to(bf), residual=x.to(bf)).dtype == bf and seen[-1] == (bf, bf)
+    with torch.autocast("cuda", dtype=bf):  # another device type's
+        m(x.to(bf))
+        assert seen[-1] == (bf, None)
+    assert ref(x).dtype == f32

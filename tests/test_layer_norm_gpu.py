@@ -411,3 +411,17 @@ def test_gradients_of_huge_constant_rows(cuda, N, xt):
     want = (gw - gw.mean(1, keepdim=True)) * eps ** -0.5
     off = (got["dx"].double() - want).abs()
     assert (off <= 2.0 ** -17 * want.abs().max() + torch.finfo(xt).eps / 2 * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_module_under_autocast(cuda, dtype):
+    """f32 arithmetic on the same values in both: 64 roundings
+    of values up to 4 are 1.5e-5."""
+    ref = torch.nn.LayerNorm(96, device="cuda")
+    m = packr.PackRLayerNorm.from_layer_norm(ref)
+    x = torch.randn(5, 96, device="cuda").to(dtype).requires_grad_(True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        a, b = m(x), ref(x)
+    assert a.dtype == b.dtype == torch.float32 and torch.allclose(a, b, rtol=1e-5, atol=2e-5)
+    ga, = torch.autograd.grad(a.square().sum(), x)
+    assert ga.dtype == dtype
