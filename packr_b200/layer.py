@@ -86,8 +86,14 @@ class PackRLinear(nn.Module):
         if residual is not None or self.activation not in (None, "none") or self.out_dtype != torch.float32:
             if x.dtype not in (torch.bfloat16, torch.float32):
                 x = x.float()
-            return packr_linear_act(x, self.W_p, self.W_f, self.lut, self.bias_f, self.activation, residual,
-                                    self.out_dtype, self.lut_counts() if self.lut.requires_grad else None)
+            # a lut or bias that model.to(dtype) converted is widened, as on the plain route
+            lut, bias = self.lut, self.bias_f
+            if lut.dtype != torch.float32:
+                lut = lut.float()
+            if bias is not None and bias.dtype not in (torch.bfloat16, torch.float32):
+                bias = bias.float()
+            return packr_linear_act(x, self.W_p, self.W_f, lut, bias, self.activation, residual,
+                                    self.out_dtype, self.lut_counts() if lut.requires_grad else None)
         orig_shape = x.shape
         if x.dim() == 3:
             x = x.reshape(-1, x.shape[-1])

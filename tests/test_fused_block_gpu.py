@@ -224,3 +224,36 @@ def test_overlapped_launches_after_a_copy_and_on_two_streams(cuda, M):
     torch.cuda.synchronize()
     for i, y in enumerate(got):
         assert torch.equal(y, want[i // 2 % 4])
+
+
+@pytest.mark.parametrize("lut,bias", [(BF16, BF16), (torch.float16, torch.float16), (torch.float64, torch.float64)])
+def test_layer_with_converted_parameters(cuda, lut, bias):
+    """model.to(dtype) converts the lut and the bias; the fused layer takes what the
+    plain one takes, and its gradients come back in the parameters' types.  18 rows:
+    both routes decode W alike (f32 sums of 96 terms: 1e-5)."""
+    lin = packr.PackRLinear.synthetic(96, 160, seed=3, lut_std=0.05)
+    torch.nn.init.normal_(lin.bias_f, std=0.2)
+    lin.lut.data = lin.lut.data.to(lut)
+    lin.bias_f.data = lin.bias_f.data.to(bias)
+    x = torch.randn(18, 96, device="cuda").bfloat16()
+    plain = lin(x)
+    want = torch.autograd.grad(plain.clamp_min(0).sum(), [lin.lut, lin.bias_f])
+    lin.activation = "relu"
+    got = lin(x)
+    assert got.dtype == F32 and torch.allclose(got, plain.clamp_min(0), rtol=1e-5, atol=1e-5)
+    for a, b in zip(torch.autograd.grad(got.sum(), [lin.lut, lin.bias_f]), want):
+        assert a.dtype == b.dtype and rel(a, b) < 2e-2
+    lin.activation = None
+    assert torch.allclose(lin(x, residual=torch.ones_like(plain)), plain + 1, rtol=1e-5, atol=1e-5)
+
+
+def test_whole_layer_converted_to_bf16(cuda):
+    lin = packr.PackRLinear.synthetic(96, 160, seed=3)
+    lin.activation, lin.out_dtype = "gelu", BF16
+    lin.to(BF16)
+    assert lin.lut.dtype == BF16 and lin.W_p.dtype == torch.uint8
+    for M in (1, 8, 40, 200):
+        y = lin(torch.randn(M, 96, device="cuda").bfloat16())
+        y.sum().backward()
+        assert y.shape == (M, 160) and lin.lut.grad.dtype == BF16
+        lin.zero_grad()
