@@ -251,6 +251,23 @@ int packr_linear_act_backward(const void* dout, const void* z, int out_dtype, in
                               int dbias_dtype, int64_t M, int64_t K, int64_t N, int flags, void* workspace,
                               size_t workspace_bytes, void* stream);
 
+/* The same over a W that the caller decoded (Wd [K, N] bf16, 16-byte aligned, equal
+ * to packr_predecode_bf16(W_p, W_f, lut)), N % 8 == 0: the forward reads it in the
+ * place of W, at every M by the GEMM that packr_linear_act_forward runs over its own
+ * decode from 129 rows on (the same bits there); the backward reads it where it would decode W for dX
+ * and ignores it otherwise (few rows).  No decoded W in these workspaces. */
+size_t packr_linear_act_forward_decoded_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, int out_dtype);
+int packr_linear_act_forward_decoded(const void* x, int x_dtype, const uint16_t* Wd, const void* bias, int bias_dtype,
+                                     int activation, const void* residual, void* out, void* z, int out_dtype, int64_t M,
+                                     int64_t K, int64_t N, void* workspace, size_t workspace_bytes, void* stream);
+size_t packr_linear_act_backward_decoded_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, int flags,
+                                                         const uint8_t* W_p, const uint16_t* W_f);
+int packr_linear_act_backward_decoded(const void* dout, const void* z, int out_dtype, int activation, const void* x,
+                                      int x_dtype, const uint8_t* W_p, const uint16_t* W_f, const float* lut,
+                                      const uint16_t* Wd, const int32_t* lut_counts, void* dX, uint16_t* dW_f,
+                                      float* dlut, void* dbias, int dbias_dtype, int64_t M, int64_t K, int64_t N,
+                                      int flags, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- layer norm over the last dimension, with a residual sum ---------------
  *   s = x + residual (f32);  y = (s - mean) * rstd * weight + bias,
  *   rstd = 1 / sqrt(mean((s - mean)^2) + eps)

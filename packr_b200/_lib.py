@@ -77,6 +77,12 @@ SIGNATURES = {
     "packr_linear_act_backward_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32, _I32, _VP, _VP]),
     "packr_linear_act_backward": (_I32, [_VP, _VP, _I32, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I32,
                                          _I64, _I64, _I64, _I32, _VP, _SZ, _VP]),
+    "packr_linear_act_forward_decoded_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32, _I32]),
+    "packr_linear_act_forward_decoded": (_I32, [_VP, _I32, _VP, _VP, _I32, _I32, _VP, _VP, _VP, _I32, _I64, _I64, _I64,
+                                                _VP, _SZ, _VP]),
+    "packr_linear_act_backward_decoded_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32, _I32, _VP, _VP]),
+    "packr_linear_act_backward_decoded": (_I32, [_VP, _VP, _I32, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP,
+                                                 _VP, _I32, _I64, _I64, _I64, _I32, _VP, _SZ, _VP]),
     "packr_layer_norm_forward": (_I32, [_VP, _VP, _I32, _VP, _VP, _I32, _F32, _VP, _VP, _VP, _I64, _I64, _VP]),
     "packr_layer_norm_backward_workspace_bytes": (_SZ, [_I64, _I64]),
     "packr_layer_norm_backward": (_I32, [_VP, _VP, _VP, _I32, _VP, _I32, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _VP, _SZ,

@@ -141,7 +141,8 @@ def _linear_act_backward(ctx, grad_out):
     g = _aligned16(g.contiguous())
     dX, dW, dlut, dbias = _k.linear_act_backward(g, z, ctx.activation, x, W_p, W_f, lut, counts, nx, nwf, nlut,
                                                  ctx.bias_dtype if nb else None,
-                                                 dW_out=grad_sink(ctx.wf_param) if nwf else None)
+                                                 dW_out=grad_sink(ctx.wf_param) if nwf else None, Wd=ctx.wd)
+    ctx.wd = None
     return dX, None, dW, dlut, dbias, grad_out if nr else None, None, None, None
 
 
@@ -150,12 +151,16 @@ _linear_act_backward_once = once_differentiable(_linear_act_backward)
 
 class PackRLinearActFunction(torch.autograd.Function):
     """out = act(x @ W + bias) + residual on contiguous 2-D operands; keeps x
-    and, for an activation, z = x @ W + bias in out's dtype."""
+    and, for an activation, z = x @ W + bias in out's dtype, and with
+    KEEP_DECODED_W the decoded W (see there)."""
 
     @staticmethod
     def forward(ctx, x, W_p, W_f, lut, bias, residual, activation, out_dtype, counts):
+        ctx.wd = None
+        if KEEP_DECODED_W and ctx.needs_input_grad[0] and _k.predecode_route(x.shape[0], *W_p.shape, W_p, W_f):
+            ctx.wd = _k.predecode_bf16(W_p, W_f, lut)
         out, z = _k.linear_act_forward(x, W_p, W_f, lut, bias, activation, residual, out_dtype,
-                                       keep_z=activation != _NO_ACTIVATION)
+                                       keep_z=activation != _NO_ACTIVATION, Wd=ctx.wd)
         ctx.save_for_backward(x, W_p, W_f, lut, z, counts)
         ctx.activation, ctx.out_dtype = activation, out_dtype
         ctx.bias_dtype = None if bias is None else bias.dtype

@@ -246,7 +246,8 @@ struct Fwd {
   int* skf;
 };
 
-size_t plan_forward(Carve& c, Fwd& p, Route r, long long M, long long K, long long N, int x_dtype, int io_f32) {
+size_t plan_forward(Carve& c, Fwd& p, Route r, long long M, long long K, long long N, int x_dtype, int io_f32,
+                    bool wd_given = false) {
   p = Fwd{};
   if (r == GEMV) return 0;
   p.xh = linear::x_needs_copy(x_dtype, K) ? c.take<uint16_t>((size_t)M * round8(K)) : nullptr;
@@ -255,7 +256,7 @@ size_t plan_forward(Carve& c, Fwd& p, Route r, long long M, long long K, long lo
   } else if (r == SKINNY) {
     p.part = c.take<float>(gemm::skinny_partial_bytes(M, K, N, io_f32 ? gemm::kSegBlocks : 0) / sizeof(float));
   } else {
-    p.wd = c.take<uint16_t>((size_t)K * round8(N));
+    p.wd = wd_given ? nullptr : c.take<uint16_t>((size_t)K * round8(N));
     p.skp = c.take<float>(gemm::sk_partial_bytes(linear::sk_pairs(), gemm::epi_msub(M, K, io_f32)) / sizeof(float));
     p.skf = c.take<int>(gemm::sk_flag_bytes(linear::sk_pairs(), 16) / sizeof(int));
   }
@@ -270,14 +271,14 @@ struct Bwd {
 };
 
 size_t plan_backward(Carve& c, Bwd& p, long long M, long long K, long long N, int x_dtype, int flags, bool direct,
-                     bool skinny, bool dx, bool dw, bool dlut, bool dbias, bool have_counts) {
+                     bool skinny, bool dx, bool dw, bool dlut, bool dbias, bool have_counts, bool wd_given = false) {
   p = Bwd{};
   const bool need_x = dw || dlut;
   const bool split = (flags & PACKR_BWD_DW_SPLIT) != 0 && need_x;
   if (dx && skinny) {
     p.part = c.take<float>(gemm::skinny_partial_bytes(M, N, K) / sizeof(float));
   } else if (dx) {
-    p.wd = c.take<uint16_t>((size_t)K * round8(N));
+    p.wd = wd_given ? nullptr : c.take<uint16_t>((size_t)K * round8(N));
     p.skp = c.take<float>(gemm::sk_partial_bytes(linear::sk_pairs(), linear::plain_msub(M)) / sizeof(float));
     p.skf = c.take<int>(gemm::sk_flag_bytes(linear::sk_pairs()) / sizeof(int));
   }
@@ -372,14 +373,15 @@ extern "C" size_t packr_linear_act_workspace_bytes(int64_t M, int64_t K, int64_t
                                   out_dtype == PACKR_DTYPE_F32);
 }
 
-extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_t* W_p, const uint16_t* W_f,
-                                        const float* lut, const void* bias, int bias_dtype, int activation,
-                                        const void* residual, void* out, void* z, int out_dtype, int64_t M, int64_t K,
-                                        int64_t N, void* workspace, size_t workspace_bytes, void* stream) {
-  using namespace packr;
-  using namespace packr::linear_act;
-  int st = check_args(x, x_dtype, W_p, W_f, lut, M, K, N);
-  if (st != PACKR_OK) return st;
+namespace packr {
+namespace linear_act {
+// The forward of checked W (W_p, W_f, lut), or of W decoded by the caller (Wd, N %
+// 8 == 0), which then goes to the GEMM over a decoded W at every M.
+int forward_impl(const void* x, int x_dtype, const uint8_t* W_p, const uint16_t* W_f, const float* lut,
+                 const uint16_t* Wd, const void* bias, int bias_dtype, int activation, const void* residual, void* out,
+                 void* z, int out_dtype, long long M, long long K, long long N, void* workspace, size_t workspace_bytes,
+                 void* stream) {
+  int st;
   if (!act_ok(activation) || !io_ok(out_dtype) || (bias != nullptr && !io_ok(bias_dtype)))
     return PACKR_ERR_INVALID_ARGUMENT;
   if (M > 0 && out == nullptr) return PACKR_ERR_INVALID_ARGUMENT;
@@ -390,10 +392,10 @@ extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_
   if ((st = check_device()) != PACKR_OK) return st;
   if (M == 0) return PACKR_OK;
   cudaStream_t s = as_stream(stream);
-  const Route r = route(M, K, N, W_p, W_f);
+  const Route r = Wd != nullptr ? PLAIN : route(M, K, N, W_p, W_f);
   Carve c{static_cast<uint8_t*>(workspace)};
   Fwd p;
-  const size_t need = linear_act::plan_forward(c, p, r, M, K, N, x_dtype, out_dtype == PACKR_DTYPE_F32);
+  const size_t need = linear_act::plan_forward(c, p, r, M, K, N, x_dtype, out_dtype == PACKR_DTYPE_F32, Wd != nullptr);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, linear::kAlign)))
     return PACKR_ERR_WORKSPACE;
   Epilogue e{};
@@ -417,8 +419,8 @@ extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_
                                     p.part, s);
   gemm::Maps maps;
   if ((st = gemm::make_map(&maps.a[0], a, K, M, lda * 2, gemm::BM)) != PACKR_OK) return st;
-  if ((st = gemm::make_map(&maps.b[0], p.wd, N, K, round8(N) * 2, 64)) != PACKR_OK) return st;
-  if ((st = decode(W_p, W_f, lut, p.wd, K, N, s)) != PACKR_OK) return st;
+  if ((st = gemm::make_map(&maps.b[0], Wd != nullptr ? Wd : p.wd, N, K, round8(N) * 2, 64)) != PACKR_OK) return st;
+  if (Wd == nullptr && (st = decode(W_p, W_f, lut, p.wd, K, N, s)) != PACKR_OK) return st;
   gemm::Params P{};
   P.Mg = (int)M;
   P.Ng = (int)N;
@@ -432,10 +434,43 @@ extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_
   gemm::set_split(P, p.skp, p.skf, linear::sk_pairs(), tiles_of(M, N, msub), msub);
   return gemm::launch_plain_epi(P, maps, s);
 }
+}  // namespace linear_act
+}  // namespace packr
+
+extern "C" int packr_linear_act_forward(const void* x, int x_dtype, const uint8_t* W_p, const uint16_t* W_f,
+                                        const float* lut, const void* bias, int bias_dtype, int activation,
+                                        const void* residual, void* out, void* z, int out_dtype, int64_t M, int64_t K,
+                                        int64_t N, void* workspace, size_t workspace_bytes, void* stream) {
+  const int st = linear_act::check_args(x, x_dtype, W_p, W_f, lut, M, K, N);
+  if (st != PACKR_OK) return st;
+  return linear_act::forward_impl(x, x_dtype, W_p, W_f, lut, nullptr, bias, bias_dtype, activation, residual, out, z,
+                                  out_dtype, M, K, N, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t packr_linear_act_forward_decoded_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype,
+                                                                   int out_dtype) {
+  if (M <= 0 || K <= 0 || N <= 0) return 0;
+  linear::Carve c{nullptr};
+  linear_act::Fwd p;
+  return linear_act::plan_forward(c, p, linear_act::PLAIN, M, K, N, x_dtype, out_dtype == PACKR_DTYPE_F32, true);
+}
+
+extern "C" int packr_linear_act_forward_decoded(const void* x, int x_dtype, const uint16_t* Wd, const void* bias,
+                                                int bias_dtype, int activation, const void* residual, void* out, void* z,
+                                                int out_dtype, int64_t M, int64_t K, int64_t N, void* workspace,
+                                                size_t workspace_bytes, void* stream) {
+  if ((N & 7) != 0 && N > 0) return PACKR_ERR_SHAPE;  // Wd rows must be 16-byte multiples for TMA
+  // Wd in the places of what it was decoded from, for the checks of pointers
+  const int st = linear_act::check_args(x, x_dtype, reinterpret_cast<const uint8_t*>(Wd), Wd,
+                                        reinterpret_cast<const float*>(Wd), M, K, N);
+  if (st != PACKR_OK) return st;
+  if (!aligned(Wd, 16)) return PACKR_ERR_ALIGNMENT;
+  return linear_act::forward_impl(x, x_dtype, nullptr, nullptr, nullptr, Wd, bias, bias_dtype, activation, residual, out,
+                                  z, out_dtype, M, K, N, workspace, workspace_bytes, stream);
+}
 
 extern "C" size_t packr_linear_act_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype, int flags,
                                                             const uint8_t* W_p, const uint16_t* W_f) {
-  using namespace packr;
   if (M <= 0 || K <= 0 || N <= 0) return 0;
   linear::Carve c{nullptr};
   linear_act::Bwd p;
@@ -443,13 +478,15 @@ extern "C" size_t packr_linear_act_backward_workspace_bytes(int64_t M, int64_t K
   return linear_act::plan_backward(c, p, M, K, N, x_dtype, flags, false, skinny, true, true, true, true, false);
 }
 
-extern "C" int packr_linear_act_backward(const void* dout, const void* z, int out_dtype, int activation, const void* x,
-                                         int x_dtype, const uint8_t* W_p, const uint16_t* W_f, const float* lut,
-                                         const int32_t* lut_counts, void* dX, uint16_t* dW_f, float* dlut, void* dbias,
-                                         int dbias_dtype, int64_t M, int64_t K, int64_t N, int flags, void* workspace,
-                                         size_t workspace_bytes, void* stream) {
-  using namespace packr;
-  using namespace packr::linear_act;
+namespace packr {
+namespace linear_act {
+// The backward; wd_given (nullable) is W as the caller decoded it, used by the plain
+// dX GEMM in place of a decode of its own.
+int backward_impl(const void* dout, const void* z, int out_dtype, int activation, const void* x, int x_dtype,
+                  const uint8_t* W_p, const uint16_t* W_f, const float* lut, const uint16_t* wd_given,
+                  const int32_t* lut_counts, void* dX, uint16_t* dW_f, float* dlut, void* dbias, int dbias_dtype,
+                  long long M, long long K, long long N, int flags, void* workspace, size_t workspace_bytes,
+                  void* stream) {
   int st = check_args(x, x_dtype, W_p, W_f, lut, M, K, N);
   if (st != PACKR_OK) return st;
   if (!act_ok(activation) || !io_ok(out_dtype) || (dbias != nullptr && !io_ok(dbias_dtype)) ||
@@ -477,7 +514,7 @@ extern "C" int packr_linear_act_backward(const void* dout, const void* z, int ou
   Carve c{static_cast<uint8_t*>(workspace)};
   Bwd p;
   const size_t need = linear_act::plan_backward(c, p, M, K, N, x_dtype, flags, direct, skinny, dx, dw, dl, db,
-                                                lut_counts != nullptr);
+                                                lut_counts != nullptr, wd_given != nullptr);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, linear::kAlign)))
     return PACKR_ERR_WORKSPACE;
   const long long ldN = round8(N);
@@ -502,8 +539,9 @@ extern "C" int packr_linear_act_backward(const void* dout, const void* z, int ou
   } else if (dx) {
     gemm::Maps maps;
     if ((st = gemm::make_map(&maps.a[0], dh, N, M, ldN * 2, gemm::BM)) != PACKR_OK) return st;
-    if ((st = gemm::make_map(&maps.b[0], p.wd, N, K, ldN * 2, gemm::BN_CTA)) != PACKR_OK) return st;
-    if ((st = decode(W_p, W_f, lut, p.wd, K, N, s)) != PACKR_OK) return st;
+    if ((st = gemm::make_map(&maps.b[0], wd_given != nullptr ? wd_given : p.wd, N, K, ldN * 2, gemm::BN_CTA)) != PACKR_OK)
+      return st;
+    if (wd_given == nullptr && (st = decode(W_p, W_f, lut, p.wd, K, N, s)) != PACKR_OK) return st;
     gemm::Params P{};
     P.Mg = (int)M;
     P.Ng = (int)K;
@@ -559,4 +597,38 @@ extern "C" int packr_linear_act_backward(const void* dout, const void* z, int ou
     return prep::finalize(dlut, p.dlut_sum, counts, nullptr, nullptr, 0, s);
   }
   return PACKR_OK;
+}
+}  // namespace linear_act
+}  // namespace packr
+
+extern "C" int packr_linear_act_backward(const void* dout, const void* z, int out_dtype, int activation, const void* x,
+                                         int x_dtype, const uint8_t* W_p, const uint16_t* W_f, const float* lut,
+                                         const int32_t* lut_counts, void* dX, uint16_t* dW_f, float* dlut, void* dbias,
+                                         int dbias_dtype, int64_t M, int64_t K, int64_t N, int flags, void* workspace,
+                                         size_t workspace_bytes, void* stream) {
+  return linear_act::backward_impl(dout, z, out_dtype, activation, x, x_dtype, W_p, W_f, lut, nullptr, lut_counts, dX,
+                                   dW_f, dlut, dbias, dbias_dtype, M, K, N, flags, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t packr_linear_act_backward_decoded_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype,
+                                                                    int flags, const uint8_t* W_p,
+                                                                    const uint16_t* W_f) {
+  if (M <= 0 || K <= 0 || N <= 0) return 0;
+  linear::Carve c{nullptr};
+  linear_act::Bwd p;
+  const bool skinny = linear::skinny_dx_eligible(M, N) && gemm::wtma_ok(W_p, W_f, N);
+  return linear_act::plan_backward(c, p, M, K, N, x_dtype, flags, false, skinny, true, true, true, true, false, true);
+}
+
+extern "C" int packr_linear_act_backward_decoded(const void* dout, const void* z, int out_dtype, int activation,
+                                                 const void* x, int x_dtype, const uint8_t* W_p, const uint16_t* W_f,
+                                                 const float* lut, const uint16_t* Wd, const int32_t* lut_counts,
+                                                 void* dX, uint16_t* dW_f, float* dlut, void* dbias, int dbias_dtype,
+                                                 int64_t M, int64_t K, int64_t N, int flags, void* workspace,
+                                                 size_t workspace_bytes, void* stream) {
+  if ((N & 7) != 0 && N > 0) return PACKR_ERR_SHAPE;
+  if (Wd == nullptr) return PACKR_ERR_INVALID_ARGUMENT;
+  if (!aligned(Wd, 16)) return PACKR_ERR_ALIGNMENT;
+  return linear_act::backward_impl(dout, z, out_dtype, activation, x, x_dtype, W_p, W_f, lut, Wd, lut_counts, dX, dW_f,
+                                   dlut, dbias, dbias_dtype, M, K, N, flags, workspace, workspace_bytes, stream);
 }

@@ -325,10 +325,11 @@ def from_linear_encode(weight: torch.Tensor, codebook: torch.Tensor, scale: torc
 
 def linear_act_forward(x: torch.Tensor, W_p: torch.Tensor, W_f: torch.Tensor, lut: torch.Tensor,
                        bias: torch.Tensor | None, activation: int, residual: torch.Tensor | None,
-                       out_dtype: torch.dtype, keep_z: bool = False):
+                       out_dtype: torch.dtype, keep_z: bool = False, Wd: torch.Tensor | None = None):
     """(out, z) with z = x @ W + bias and out = act(z) + residual, both [M, N]
     of out_dtype (z None unless keep_z).  x is contiguous 2-D, activation a
-    PACKR_ACT_* code."""
+    PACKR_ACT_* code.  Wd: optional W decoded by predecode_bf16, read in the
+    place of W_p, W_f and lut."""
     lib = _lib.load()
     M, K = x.shape
     N = W_p.shape[1]
@@ -339,6 +340,14 @@ def linear_act_forward(x: torch.Tensor, W_p: torch.Tensor, W_f: torch.Tensor, lu
     wp, wf = W_p.data_ptr(), W_f.data_ptr()
     with _on_device(dev):
         od = _dtype_code(out)
+        if Wd is not None:
+            nbytes = lib.packr_linear_act_forward_decoded_workspace_bytes(M, K, N, xd, od)
+            ws = _workspace(nbytes, dev)
+            code = lib.packr_linear_act_forward_decoded(
+                x.data_ptr(), xd, Wd.data_ptr(), _addr(bias), _dtype_code(bias) if bias is not None else 0, activation,
+                _addr(residual), out.data_ptr(), _addr(z), od, M, K, N, _addr(ws), nbytes, _raw_stream(dev))
+            _lib.check("packr_linear_act_forward_decoded", code)
+            return out, z
         nbytes = lib.packr_linear_act_workspace_bytes(M, K, N, xd, od, wp, wf)
         ws = _workspace(nbytes, dev)
         code = lib.packr_linear_act_forward(
@@ -353,10 +362,10 @@ def linear_act_forward(x: torch.Tensor, W_p: torch.Tensor, W_f: torch.Tensor, lu
 def linear_act_backward(dout: torch.Tensor, z: torch.Tensor | None, activation: int, x: torch.Tensor,
                         W_p: torch.Tensor, W_f: torch.Tensor, lut: torch.Tensor, counts: torch.Tensor | None,
                         need_dx: bool, need_dw: bool, need_dlut: bool, dbias_dtype: torch.dtype | None,
-                        dW_out: torch.Tensor | None = None):
+                        dW_out: torch.Tensor | None = None, Wd: torch.Tensor | None = None):
     """Returns (dX, dW_f, dlut, dbias); entries not requested are None (dbias:
     dbias_dtype None).  dout is contiguous [M, N] of the forward's out_dtype;
-    dW_out as in backward()."""
+    dW_out and Wd as in backward()."""
     lib = _lib.load()
     M, K = x.shape
     N = W_p.shape[1]
@@ -377,6 +386,15 @@ def linear_act_backward(dout: torch.Tensor, z: torch.Tensor | None, activation: 
     flags = _lib.PACKR_BWD_DW_SPLIT if dw_split_for(x.dtype) else 0
     with _on_device(dev):
         wp, wf = W_p.data_ptr(), W_f.data_ptr()
+        if Wd is not None:
+            nbytes = lib.packr_linear_act_backward_decoded_workspace_bytes(M, K, N, xd, flags, wp, wf)
+            ws = _workspace(nbytes, dev)
+            code = lib.packr_linear_act_backward_decoded(
+                dout.data_ptr(), _addr(z), _dtype_code(dout), activation, x.data_ptr(), xd, wp, wf, lut.data_ptr(),
+                Wd.data_ptr(), _addr(counts), _addr(dX), _addr(dW), _addr(dlut), _addr(dbias),
+                _dtype_code(dbias) if dbias is not None else 0, M, K, N, flags, _addr(ws), nbytes, _raw_stream(dev))
+            _lib.check("packr_linear_act_backward_decoded", code)
+            return dX, dW, dlut, dbias
         nbytes = lib.packr_linear_act_backward_workspace_bytes(M, K, N, xd, flags, wp, wf)
         ws = _workspace(nbytes, dev)
         code = lib.packr_linear_act_backward(

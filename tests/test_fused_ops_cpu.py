@@ -342,3 +342,22 @@ def test_norm_module_follows_autocast(monkeypatch):
         m(x.to(bf))
         assert seen[-1] == (bf, None)
     assert ref(x).dtype == f32
+
+
+def test_decoded_linear_act_c_entries_refuse_bad_arguments():
+    lib, a, odd = _lib.load(), _fake(), _fake(8)
+
+    def fwd(x=a, xd=1, wd=a, out=a, od=1, act=0, M=4, K=8, N=8):
+        return lib.packr_linear_act_forward_decoded(x, xd, wd, None, 0, act, None, out, None, od, M, K, N, None, 0, None)
+
+    assert fwd(M=-1) == 2 and fwd(K=0) == 2 and fwd(N=0) == 2 and fwd(N=12) == 2 and fwd(N=0x7FFFFFF8) == 2
+    assert fwd(wd=None) == 1 and fwd(x=None) == 1 and fwd(out=None) == 1 and fwd(xd=2) == 1 and fwd(act=7) == 1
+    assert fwd(wd=odd) == 3 and fwd(x=_fake(1)) == 3
+
+    def bwd(wd=a, M=4, K=8, N=8, z=a):
+        return lib.packr_linear_act_backward_decoded(a, z, 1, 2, a, 1, a, a, a, wd, None, a, a, None, None, 0, M, K, N, 0,
+                                                     None, 0, None)
+
+    assert bwd(wd=None) == 1 and bwd(wd=odd) == 3 and bwd(N=12) == 2 and bwd(M=-1) == 2 and bwd(z=None) == 1
+    assert lib.packr_linear_act_forward_decoded_workspace_bytes(0, 8, 8, 1, 1) == 0
+    assert lib.packr_linear_act_backward_decoded_workspace_bytes(4, 8, 0, 1, 0, None, None) == 0

@@ -478,3 +478,65 @@ def test_few_rows_of_a_long_reduction(cuda, M, K, N, xt, out):
     c = case(M, K, N, xt, out, seed=M + K)
     for act in ("none", "gelu"):
         compare(c, {"out": call(c, act, out)}, act, out)
+
+
+@pytest.mark.parametrize("xt,out", [(BF16, BF16), (F32, F32), (BF16, F32)])
+@pytest.mark.parametrize("M,K,N", [(129, 72, 144), (300, 256, 512), (1100, 2056, 1040)])
+def test_decoded_weight_kept_for_the_backward(cuda, monkeypatch, M, K, N, xt, out):
+    """PACKR_KEEP_DECODED_W=1: W decoded in the forward serves the dX GEMM; the same
+    bits as with two decodes."""
+    from packr_b200 import autograd
+    c = case(M, K, N, xt, out, seed=M)
+    need = ("x", "W_f", "bias", "residual")
+    for act in ("none", "gelu"):
+        want = grads(c, act, out, need=need)
+        assert not autograd.KEEP_DECODED_W
+        leaf = {**c, "x": c["x"].detach().requires_grad_(True)}
+        assert call(leaf, act, out).grad_fn.wd is None
+        with monkeypatch.context() as m:
+            m.setattr(autograd, "KEEP_DECODED_W", True)
+            y = call(leaf, act, out)
+            node = y.grad_fn
+            assert node.wd.shape == (K, N) and node.wd.dtype == BF16
+            dx, = torch.autograd.grad(y, leaf["x"], c["dout"], retain_graph=True)
+            assert node.wd is None and torch.equal(dx, want["dx"]) and torch.equal(y, want["out"])
+            again, = torch.autograd.grad(y, leaf["x"], c["dout"])  # decoded once more
+            assert torch.equal(again, dx)
+            got = grads(c, act, out, need=need)
+            for k, v in want.items():
+                assert torch.equal(got[k], v), k
+            # not kept where dX is not asked for, few rows, or a width the decode does not take
+            assert grads(c, act, out, need=("W_f",))["out"].grad_fn.wd is None
+            few = {**leaf, "x": leaf["x"][:20], "residual": c["residual"][:20]}
+            assert call(few, act, out).grad_fn.wd is None
+
+
+def test_decoded_weight_through_the_c_entry(cuda):
+    """Every row count reads it, on any stream, with the exact workspace."""
+    from packr_b200 import _lib, kernel
+    lib = _lib.load()
+    for M in (1, 40, 200):
+        c = case(M, 72, 144, BF16, BF16, seed=M)
+        Wd = kernel.predecode_bf16(c["W_p"], c["W_f"], c["lut"])
+        args = (c["x"], c["W_p"], c["W_f"], c["lut"], c["bias"], 2, c["residual"], BF16)
+        got = kernel.linear_act_forward(*args, keep_z=True, Wd=Wd)
+        compare(c, {"out": got[0]}, "gelu", BF16)
+        if M > 128:
+            assert all(torch.equal(a, b) for a, b in zip(got, kernel.linear_act_forward(*args, keep_z=True)))
+        bwd = (c["dout"], got[1], 2, c["x"], c["W_p"], c["W_f"], c["lut"], None, True, True, True, BF16)
+        a, b = kernel.linear_act_backward(*bwd, Wd=Wd), kernel.linear_act_backward(*bwd)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(a[3], b[3])
+        need = lib.packr_linear_act_forward_decoded_workspace_bytes(M, 72, 144, 1, 1)
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+        out = torch.zeros(M, 144, dtype=BF16, device="cuda")
+
+        def fwd(nbytes):
+            return lib.packr_linear_act_forward_decoded(c["x"].data_ptr(), 1, Wd.data_ptr(), None, 0, 0, None,
+                                                        out.data_ptr(), None, 1, M, 72, 144, ws.data_ptr(), nbytes, None)
+
+        assert need > 0 and fwd(need - 1) == 4
+        torch.cuda.synchronize()
+        assert not out.any() and fwd(need) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out, kernel.linear_act_forward(c["x"], c["W_p"], c["W_f"], c["lut"], None, 0, None, BF16,
+                                                          Wd=Wd)[0])
