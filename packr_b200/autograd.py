@@ -138,7 +138,7 @@ def _linear_act_backward(ctx, grad_out):
     x, W_p, W_f, lut, z, counts = ctx.saved_tensors
     nx, _, nwf, nlut, nb, nr = ctx.needs_input_grad[:6]
     g = grad_out if grad_out.dtype == ctx.out_dtype else grad_out.to(ctx.out_dtype)
-    g = _aligned16(g.contiguous())
+    g = _k.aligned16(g.contiguous())
     dX, dW, dlut, dbias = _k.linear_act_backward(g, z, ctx.activation, x, W_p, W_f, lut, counts, nx, nwf, nlut,
                                                  ctx.bias_dtype if nb else None,
                                                  dW_out=grad_sink(ctx.wf_param) if nwf else None, Wd=ctx.wd)
@@ -175,10 +175,6 @@ class PackRLinearActFunction(torch.autograd.Function):
 
 _NO_ACTIVATION = _lib.ACTIVATIONS["none"]
 _FLOATS = (torch.bfloat16, torch.float32)
-
-
-def _aligned16(t):
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def packr_linear_act(x, W_p, W_f, lut, bias=None, activation=None, residual=None, out_dtype=torch.float32, counts=None):
@@ -228,7 +224,7 @@ def packr_linear_act(x, W_p, W_f, lut, bias=None, activation=None, residual=None
         raise ValueError("packr_linear_act: every tensor must be on x's device")
     grad = x.requires_grad or W_f.requires_grad or lut.requires_grad
     flat = x.dim() == 2
-    x2 = _aligned16((x if flat else x.reshape(-1, K)).contiguous())
+    x2 = _k.aligned16((x if flat else x.reshape(-1, K)).contiguous())
     W_f, lut = W_f.contiguous(), lut.contiguous()
     if bias is not None:
         if bias.dim() != 1 or bias.shape[0] != N or bias.dtype not in _FLOATS:

@@ -68,6 +68,12 @@ def _addr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def aligned16(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous t, or a copy of it, that starts on a 16-byte boundary (torch's
+    allocations do; a slice of one need not)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def refuse_tangents(op: str, *tensors) -> None:
     """Raises when a tensor carries a forward-mode derivative, which a kernel that
     is called past autograd would drop (the result's would read as zero)."""

@@ -18,9 +18,18 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernel import _addr, _on_device, _raw_stream, refuse_tangents
+from .kernel import _addr, _on_device, _raw_stream, aligned16, refuse_tangents
 
 _F32, _BF16 = torch.float32, torch.bfloat16
+# A tensor that starts off the 16-byte grid is copied first where its rows are ones
+# that the kernels hold in registers and there are _COPY_FROM elements or more: the
+# kernels' path for any alignment has scalar loads and one CTA per row.  Measured
+# (bf16, calls in a row, us that way / with the copy): forward 2800 x 768 21 / 25,
+# 5600 x 768 39 / 25, 512 x 4096 16 / 25, 1024 x 4096 25 / 25, 16384 x 4096 404 / 142;
+# backward 1400 x 768 34 / 34, 5600 x 768 95 / 34, 512 x 4096 28 / 34, 16384 x 4096
+# 848 / 172.
+_MAX_REGISTER_ROW = 16384
+_COPY_FROM = 1 << 21
 _CODE = {_F32: _lib.PACKR_DTYPE_F32, _BF16: _lib.PACKR_DTYPE_BF16}
 
 
@@ -71,7 +80,7 @@ def _norm_backward(ctx, dy):
     nx, nw, nb, _, nr = ctx.needs_input_grad
     if dy.dtype != x.dtype:
         dy = dy.to(x.dtype)
-    dx, dw, db = layer_norm_backward(dy.contiguous(), x, weight, stats, residual, ctx.w_dtype, nx or nr, nw, nb)
+    dx, dw, db = layer_norm_backward(_operand(dy), x, weight, stats, residual, ctx.w_dtype, nx or nr, nw, nb)
     return dx if nx else None, dw, db, None, dx if nr else None
 
 
@@ -113,7 +122,7 @@ def packr_layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("packr_layer_norm: x needs a last dimension of at least 1")
     grad = x.requires_grad
-    x = x.contiguous()
+    x = _operand(x)
     if weight is not None:
         _check_vector("weight", weight, x)
         grad = grad or weight.requires_grad
@@ -128,13 +137,18 @@ def packr_layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
         if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
             raise ValueError("packr_layer_norm: residual must have x's shape, dtype and device")
         grad = grad or residual.requires_grad
-        residual = residual.contiguous()
+        residual = _operand(residual)
     eps = float(eps)
     if not eps >= 0.0:
         raise ValueError(f"packr_layer_norm: eps must be >= 0, got {eps}")
     if grad and torch.is_grad_enabled():
         return PackRLayerNormFunction.apply(x, weight, bias, eps, residual)
     return layer_norm_forward(x, weight, bias, eps, residual)[0]
+
+
+def _operand(t):
+    t = t.contiguous()
+    return aligned16(t) if t.shape[-1] <= _MAX_REGISTER_ROW and t.numel() >= _COPY_FROM else t
 
 
 def _check_vector(name, t, x):

@@ -425,3 +425,25 @@ def test_module_under_autocast(cuda, dtype):
     assert a.dtype == b.dtype == torch.float32 and torch.allclose(a, b, rtol=1e-5, atol=2e-5)
     ga, = torch.autograd.grad(a.square().sum(), x)
     assert ga.dtype == dtype
+
+
+@pytest.mark.parametrize("xt,wt", [(BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("M,N", [(33, 64), (5, 8192), (40000, 64), (2100, 1001), (260, 8192), (130, 16375), (130, 16640)])
+def test_tensors_off_the_16_byte_grid(cuda, M, N, xt, wt):
+    """Slices that start an element after a boundary.  Large ones take the same path
+    as aligned ones: the same bits up to 16384 columns, forward and backward."""
+    c = case(M, N, xt, wt, seed=N)
+    want = run(c)
+
+    def shifted(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        flat[1:] = t.reshape(-1)
+        s = flat[1:].view(t.shape)
+        assert s.data_ptr() % 16 != 0
+        return s
+
+    for names in (("x",), ("residual",), ("dy",), ("x", "residual", "dy", "weight", "bias")):
+        got = run({**c, **{k: shifted(c[k]) for k in names}})
+        compare(c, got)
+        for k, v in want.items():
+            assert N > 16384 or M * N < 1 << 21 or torch.equal(got[k], v), (names, k)
