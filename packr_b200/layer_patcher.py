@@ -254,6 +254,8 @@ class PackRAddNorm(nn.Module):
         # widened (the norm takes f32 and bf16)
         t = torch.promote_types(h.dtype, input_tensor.dtype)
         t = torch.float32 if t == torch.float16 else t
+        if h.shape != input_tensor.shape:  # the sum's shape, as h + input_tensor's
+            h, input_tensor = torch.broadcast_tensors(h, input_tensor)
         return self.LayerNorm(h.to(t), residual=input_tensor.to(t))
 
 

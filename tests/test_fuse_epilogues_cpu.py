@@ -268,3 +268,24 @@ def test_watched_modules_are_left_alone(how):
     dense = model[0].dense
     packr.fuse_epilogues(model)
     assert isinstance(model[0], packr.PackRAddNorm) and model[0].dense is dense
+
+
+def test_add_norm_broadcasts_its_sum(monkeypatch):
+    """As h + input_tensor does; the norm is handed two tensors of one shape."""
+    from packr_b200 import norm
+    seen = []
+
+    def plain(x, weight, bias, eps, residual):
+        seen.append((x.shape, residual.shape))
+        return nn.functional.layer_norm(x + residual, x.shape[-1:], weight, bias, eps)
+
+    monkeypatch.setattr(norm, "packr_layer_norm", plain)
+    dense, ln = nn.Linear(8, 8), nn.LayerNorm(8)
+    block = packr.PackRAddNorm(dense, ln)
+    h = torch.randn(2, 3, 8, requires_grad=True)
+    for shape in ((2, 3, 8), (1, 3, 8), (3, 8), (8,), (4, 2, 3, 8)):
+        r = torch.randn(shape, requires_grad=True)
+        got, want = block(h, r), ln(dense(h) + r)
+        assert torch.allclose(got, want, rtol=1e-6, atol=1e-6) and seen[-1][0] == seen[-1][1]
+        for a, b in zip(torch.autograd.grad(got.square().sum(), [h, r]), torch.autograd.grad(want.square().sum(), [h, r])):
+            assert a.shape == b.shape and torch.allclose(a, b, rtol=1e-5, atol=1e-5)
