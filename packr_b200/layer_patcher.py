@@ -150,8 +150,8 @@ def _hooked(module):
 
 
 def _own_forward(module):
-    """Whether the module's class computes something of its own when called."""
-    return type(module).forward is not nn.Module.forward
+    """Whether the module computes something of its own when called."""
+    return type(module).forward is not nn.Module.forward or "forward" in module.__dict__
 
 
 def _paths(module, parameters, **markers):
@@ -161,7 +161,7 @@ def _paths(module, parameters, **markers):
     exactly `parameters` arguments without defaults are, as a test for None or for
     a type cannot be seen in a trace."""
     forward = type(module).forward
-    if "forward" in module.__dict__:  # not the class's
+    if "forward" in module.__dict__ or not inspect.isfunction(forward):
         return None
     ps = list(inspect.signature(forward).parameters.values())[1:]
     if len(ps) != parameters or any(p.default is not p.empty or p.kind is not p.POSITIONAL_OR_KEYWORD for p in ps):
@@ -174,18 +174,18 @@ def _paths(module, parameters, **markers):
         todo = [()]
         while todo:
             decisions = todo.pop()
-            # a copy of its own, so that neither the markers nor the trace touch the module
-            probe = copy.copy(module)
-            probe.__dict__.update({k: dict(v) if isinstance(v, dict) else v for k, v in module.__dict__.items()})
-            probe._buffers = {k: None if b is None else b.clone() for k, b in module._buffers.items()}
-            probe.training = training
-            for name, marker in markers.items():
-                probe.__dict__.pop(name, None)
-                probe._modules[name] = marker
             tracer = _Tracer(decisions)
             try:
+                # a copy of its own, so that neither the markers nor the trace touch the module
+                probe = copy.copy(module)
+                probe.__dict__.update({k: dict(v) if isinstance(v, dict) else v for k, v in module.__dict__.items()})
+                probe._buffers = {k: None if b is None else b.clone() for k, b in module._buffers.items()}
+                probe.training = training
+                for name, marker in markers.items():
+                    probe.__dict__.pop(name, None)
+                    probe._modules[name] = marker
                 graphs.append(tracer.trace(probe))
-            except Exception:  # whatever a forward does to a value it cannot read
+            except Exception:  # a module that is not copied, a value that a forward cannot read
                 return None
             todo += [decisions + (False,) * (k - len(decisions)) + (True,) for k in range(len(decisions), tracer.asked)]
     return graphs

@@ -289,3 +289,31 @@ def test_add_norm_broadcasts_its_sum(monkeypatch):
         assert torch.allclose(got, want, rtol=1e-6, atol=1e-6) and seen[-1][0] == seen[-1][1]
         for a, b in zip(torch.autograd.grad(got.square().sum(), [h, r]), torch.autograd.grad(want.square().sum(), [h, r])):
             assert a.shape == b.shape and torch.allclose(a, b, rtol=1e-5, atol=1e-5)
+
+
+def test_forwards_that_cannot_be_followed_are_left_alone():
+    class Own(nn.Module):  # a forward set on the instance of a class without one
+        def __init__(self):
+            super().__init__()
+            self.fc1, self.activation_fn = packr.PackRLinear(8, 16), nn.ReLU()
+            self.forward = lambda x: self.activation_fn(self.fc1(x).flip(-1))
+
+    class NoCopy(Mlp):
+        def __copy__(self):
+            raise RuntimeError("not copied")
+
+    class Scripted(Mlp):
+        forward = torch.no_grad()  # callable, but nothing to read arguments from
+
+    class Loop(Mlp):
+        def forward(self, x):
+            h = self.fc1(x)
+            while h.sum() > 1:
+                h = h / 2
+            return self.activation_fn(h)
+
+    own = Own()
+    packr.fuse_epilogues(own)  # the model itself
+    assert own.fc1.activation is None
+    for block in (Own(), NoCopy(), Scripted(), Loop()):
+        assert not fused(block), type(block).__name__
