@@ -239,7 +239,8 @@ int packr_linear_act_forward(const void* x, int x_dtype, const uint8_t* W_p, con
  *   dW_f[K,N] = bf16(x^T @ dz)  fp32 accumulate          (NULL: skipped)
  *   dlut[256] = sum_{W_p==b} (x^T @ dz) / (count[b] + 1e-8)  (NULL: skipped)
  *   dbias[N]  = sum_m dz, as dbias_dtype, rows added in a fixed order (NULL: skipped)
- * The residual's gradient is dout itself.  dout and z are contiguous [M, N] of
+ * The residual's gradient is dout itself.  dX takes bf16(dz) and is rounded to bf16 for f32
+ * x too, as packr_backward's.  dout and z are contiguous [M, N] of
  * out_dtype; z is the forward's (NULL for PACKR_ACT_NONE).  lut_counts and
  * flags as for packr_backward; with PACKR_BWD_DW_SPLIT dz enters dW as bf16
  * hi + lo parts. */

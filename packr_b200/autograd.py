@@ -194,11 +194,17 @@ def packr_linear_act(x, W_p, W_f, lut, bias=None, activation=None, residual=None
         counts:     int32 [256] bincount of W_p (PackRLinear.lut_counts), used by the lut
                     gradient; counted there when None
 
-    W = bf16(W_f + bf16(lut[W_p])) at every row count.  With bf16 x the
-    gradient of the pre-activation enters the weight and lut gradients rounded
+    W = bf16(W_f + bf16(lut[W_p])) and x rounded to bf16 at every row count, also
+    at the few rows (1 to 4, up to 16 for some widths) where packr_matmul takes f32
+    x and the unrounded sum: there the two differ by those roundings.
+    Gradients: the kept pre-activation has out_dtype (bf16: its slope is off by up
+    to half a step of it).  dX is taken from the pre-activation's gradient rounded
+    to bf16 and is itself rounded to bf16, for f32 x too, as PackRLinear's is.
+    With bf16 x that gradient enters the weight and lut gradients rounded
     to bf16, as in PackRLinear; with f32 x as bf16 hi + lo parts
     (PACKR_DW_PRECISION).  The f32 lut gradient is short by about 1e-9 of itself
-    per token (the tensor cores truncate the sums it is taken from).
+    per token (the tensor cores truncate the sums it is taken from), and its sums
+    over CTAs are added in any order.
     Backward mode, once: second and forward-mode derivatives are refused."""
     _k.refuse_tangents("packr_linear_act", x, W_f, lut, bias, residual)
     if not x.is_cuda:

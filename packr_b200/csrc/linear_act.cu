@@ -9,12 +9,14 @@
 //
 // Routes (forward): 1 and 2 rows the CUDA-core GEMV; 3..16, and 1 or 2 with a long
 // reduction, the mma.sync kernel and 17..128 the skinny tcgen05 GEMM, each with its
-// reduction; from 129 rows, and wherever W's rows do not allow TMA (N % 16 != 0 or a
-// misaligned base), W is decoded once into the workspace, with rows padded to a
-// multiple of 8, and read by TMA, so that odd widths take the same tensor-core GEMM
-// as even ones (1 and 2 rows stay with the GEMV where it can).  The backward takes dz
-// in one pass over dout and z (bf16 operand, optional residual part of the
-// split, column sums), then the existing dX and dW GEMMs.
+// reduction.  Where W's rows do not allow TMA (N % 16 != 0 or a misaligned base), up
+// to 16 rows take the GEMV if it can (gemv::eligible: even N, W aligned to a lane's
+// load, a CTA's share of x in shared memory).  Everything else, and from 129 rows on
+// every width: W is decoded once into the workspace, with rows padded to a multiple
+// of 8, and read by TMA, so that odd widths take the same tensor-core GEMM as even
+// ones.  The backward takes dz in one pass over dout and z (bf16 operand, optional
+// residual part of the split, column sums), then the existing dX and dW GEMMs.  A W
+// that the caller decoded (the _decoded entries) takes the place of either decode.
 #include "activation.cuh"
 
 namespace packr {
@@ -226,6 +228,9 @@ enum Route { GEMV, SKINNY_MMA, SKINNY, PLAIN };
 // reduction leaves uneven (16384 -> 256, 1 row: 12.9 and 17.3; 8192 -> 2048: 14.2 and
 // 17.0), and is ahead where it is one launch's latency that counts (1024 x 1024, 2
 // rows: 5.8 and 5.0; 4096 x 4096: 14.4 and 16.1).
+// Widths that TMA cannot read, GEMV / decode and GEMM: 1024 -> 1002 3 rows 5.7 / 25.1,
+// 16 rows 8.7 / 25.6; 4096 -> 4100 4 rows 18.8 / 64.1, 8 rows 24.7 / 64.3; 4096 -> 11004
+// 8 rows 73 / 98.
 constexpr long long kSkinnyMmaMaxM = 16;
 inline bool skinny_mma_pays(long long M, long long K, long long N) {
   if (M > kSkinnyMmaMaxM) return false;

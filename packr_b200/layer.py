@@ -13,7 +13,10 @@ layer (W_p is frozen) instead of recounted every backward.
 Beyond the reference, `layer.activation`, `layer.out_dtype` and
 forward(x, residual=...) put an activation, a residual sum and the output's
 rounding into the same GEMM epilogue (packr_linear_act); at their defaults the
-layer is the reference's.
+layer is the reference's.  The fused operator rounds x and W to bf16 at every row
+count; the default route takes f32 x and an unrounded W at 1 to 4 rows (up to 16 for
+widths that TMA cannot read), so there setting an attribute moves a result by those
+roundings.
 """
 from __future__ import annotations
 

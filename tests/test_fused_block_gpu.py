@@ -257,3 +257,31 @@ def test_whole_layer_converted_to_bf16(cuda):
         y.sum().backward()
         assert y.shape == (M, 160) and lin.lut.grad.dtype == BF16
         lin.zero_grad()
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 18, 200])
+@pytest.mark.parametrize("xt", [F32, BF16])
+def test_attributes_move_a_result_by_its_operands_rounding_only(cuda, M, xt):
+    """The plain layer's few-row kernel takes f32 x and W = W_f + f16(lut[W_p]) as they
+    are; the fused operator rounds x and W to bf16 at every row count, as both do from
+    many rows on.  Half a step of each operand apart (2^-8 of |x| |W| twice, 2^-8 + 2^-11
+    of |x| |lut| for the two roundings of lut), and f32 sums of 256 terms."""
+    lin = packr.PackRLinear.synthetic(256, 160, seed=3, lut_std=0.05, wf_std=0.01)
+    torch.nn.init.normal_(lin.bias_f, std=0.2)
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = torch.randn(M, 256, generator=g, device="cuda").to(xt)
+    lut = lin.lut.detach()[lin.W_p.long()].double().abs()
+    W = lin.W_f.detach().double().abs() + lut
+    xa = x.double().abs()
+    bound = (2 * 2.0 ** -8 + 2 * 258 * 2.0 ** -23) * (xa @ W) + (2.0 ** -8 + 2.0 ** -11) * (xa @ lut) + 1e-6
+    with torch.no_grad():
+        plain = lin(x).double()
+        fused = lin(x, residual=torch.zeros(M, 160, device="cuda")).double()
+        assert ((fused - plain).abs() <= bound).all()
+        lin.activation = "relu"
+        assert ((lin(x).double() - plain.clamp_min(0)).abs() <= bound).all()
+        # the definition at every row count: rounded operands, f32 sums
+        w = weights64(lin.W_p, lin.W_f, lin.lut)
+        z = x.bfloat16().double() @ w + lin.bias_f.double()
+        zb = 258 * 2.0 ** -23 * (xa @ W + lin.bias_f.double().abs()) * (1 + 2.0 ** -7)
+        assert ((fused - z).abs() <= zb).all()
