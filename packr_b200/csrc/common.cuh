@@ -28,8 +28,8 @@ int launch_status();
 // such a chain in order:
 // * What the kernel in front may write is read, and anything at all is written,
 //   only after the wait.  A kernel that lets the next one start
-//   (launch_dependents) does so after its own wait: whoever starts behind it
-//   starts when all that came before it has ended, and whoever waits for it has
+//   (launch_dependents) does so after its own wait, or is launched normally and
+//   has nothing to wait for (dz_kernel): whoever starts behind it starts when all that came before it has ended, and whoever waits for it has
 //   waited for all of that too.  So a kernel that is always launched behind one
 //   that waits first (a reduction behind its split kernel) may read before its own
 //   wait what neither of the two writes: bias and residual.
