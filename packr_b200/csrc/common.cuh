@@ -29,10 +29,11 @@ int launch_status();
 // * What the kernel in front may write is read, and anything at all is written,
 //   only after the wait.  A kernel that lets the next one start
 //   (launch_dependents) does so after its own wait, or is launched normally and
-//   has nothing to wait for (dz_kernel): whoever starts behind it starts when all that came before it has ended, and whoever waits for it has
-//   waited for all of that too.  So a kernel that is always launched behind one
-//   that waits first (a reduction behind its split kernel) may read before its own
-//   wait what neither of the two writes: bias and residual.
+//   has nothing to wait for (dz_kernel): whoever starts behind it starts when all
+//   that came before it has ended, and whoever waits for it has waited for all of
+//   that too.  So a kernel that is always launched behind one that waits first (a
+//   reduction behind its split kernel) may read before its own wait what neither
+//   of the two writes: bias and residual.
 // * Such a kernel can begin while its inputs are being written, so they are not
 //   read-only over its life: it reads global memory with coherent loads (__ldcg,
 //   __ldcs, cp.async, TMA; load_io_late), never with __ldg or through a const
